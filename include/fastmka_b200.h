@@ -305,6 +305,65 @@ FMKA_API int fmka_l3_recall_gather_bf16(const int32_t* idx, const float* w, int 
                                         int n_chunks, int D, int B, int T, int block_len, void* out, int64_t o_sb,
                                         int64_t o_st, fmka_stream_t stream);
 
+/* -------------------------------------------- packed serving operators ---
+ * Prompts packed one behind the other without padding, requests that share a
+ * prefix, and the per-head norms of newer models (no counterpart in the
+ * reference, whose cache and attention take one padded batch: hf/attention.py:
+ * 110-195). head_dim must be 128; strides in elements, multiples of 8; tensors
+ * 16-byte aligned.
+ *
+ * fmka_qk_norm_rope_bf16: for every token and every head of q [B, T, Hq, 128]
+ * and k [B, T, Hkv, 128] (strides sb, st, sh), n = x * rsqrt(mean(x^2) + eps) *
+ * weight, then the rotate-half rotation by cos/sin, in fp32 with one rounding.
+ * q_weight / k_weight [128]: bf16, or fp32 where bit 0 (q) / bit 1 (k) of
+ * weight_is_f32 is set; NULL leaves the norm out. rope_cos / rope_sin fp32 rows
+ * of 128, both NULL for no rotation: row of token (b, t) at b * rope_sb + t *
+ * rope_st, or, with positions (int32 or int64, [B * T] contiguous), row
+ * positions[b * T + t] of a table of n_positions rows (stride rope_st). A token
+ * at position -1 is padding: its output rows are left as they were; any other
+ * position outside the table does the same and sets FMKA_STATUS_BAD_LAUNCH.
+ * Hkv may be 0 (q only). q_out may be q and k_out may be k. */
+FMKA_API int fmka_qk_norm_rope_bf16(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
+                                    int64_t k_st, int64_t k_sh, const void* q_weight, const void* k_weight,
+                                    int weight_is_f32, float eps, const float* rope_cos, const float* rope_sin,
+                                    int64_t rope_sb, int64_t rope_st, const void* positions, int positions_are_i64,
+                                    int n_positions, void* q_out, int64_t qo_sb, int64_t qo_st, int64_t qo_sh,
+                                    void* k_out, int64_t ko_sb, int64_t ko_st, int64_t ko_sh, int B, int T, int Hq,
+                                    int Hkv, int head_dim, fmka_stream_t stream);
+
+/* fmka_attn_varlen: attention over n_seqs sequences packed one behind the
+ * other. Sequence s owns rows [cu_q[s], cu_q[s+1]) of q and o ([total_q, Hq,
+ * 128], strides st, sh) and rows [cu_k[s], cu_k[s+1]) of k and v ([total_k, Hkv,
+ * 128], common strides). The offsets (device memory, n_seqs + 1 each) must be
+ * non-decreasing within [0, total]; if they are not, no output is written and
+ * FMKA_STATUS_BAD_LAUNCH is set. With causal, token i of a sequence of Lq
+ * queries and Lk keys sees keys j <= i + Lk - Lq (new tokens behind a history);
+ * a row that sees no key gives zeros and a log-sum-exp of -inf. Rows outside
+ * every sequence are left as they were. lse[row * lse_st + head * lse_sh]
+ * (natural log) may be NULL. max_k: an upper bound on the keys of one sequence
+ * (total_k if unknown); it sizes the workspace and never limits what is read. */
+FMKA_API size_t fmka_attn_varlen_workspace_size(int n_seqs, int total_q, int max_k, int Hq, int Hkv);
+FMKA_API int fmka_attn_varlen(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
+                              int64_t kv_sh, const int32_t* cu_q, const int32_t* cu_k, int n_seqs, void* o,
+                              int64_t o_st, int64_t o_sh, float* lse, int64_t lse_st, int64_t lse_sh, int total_q,
+                              int total_k, int max_k, int Hq, int Hkv, int head_dim, int causal, float scale,
+                              void* workspace, size_t workspace_bytes, fmka_stream_t stream);
+
+/* fmka_attn_decode_shared: one query token per request, q[b, hq, :], against a
+ * prefix shared by the whole batch (k_prefix / v_prefix [Hkv, P, 128], strides
+ * p_sh, p_st) followed by the request's own keys (k / v [B, Hkv, Tcap, 128],
+ * the first lens[b] slots; lens in device memory, NULL means Tcap for all,
+ * values are clamped to [0, Tcap]). The prefix is read once for the batch. P or
+ * Tcap may be 0; a request that sees no key gives zeros and -inf. o[b, hq, :] at
+ * (o_sb, o_sh); lse[b * lse_sb + hq] may be NULL. */
+FMKA_API size_t fmka_attn_decode_shared_workspace_size(int B, int Hq, int Hkv, int P, int Tcap);
+FMKA_API int fmka_attn_decode_shared(const void* q, int64_t q_sb, int64_t q_sh, const void* k_prefix,
+                                     const void* v_prefix, int64_t p_sh, int64_t p_st, const void* k, const void* v,
+                                     int64_t kv_sb, int64_t kv_sh, int64_t kv_st, const int32_t* lens, void* o,
+                                     int64_t o_sb, int64_t o_sh, float* lse, int64_t lse_sb, int B, int Hq, int Hkv,
+                                     int P, int Tcap, int head_dim, float scale, void* workspace,
+                                     size_t workspace_bytes, fmka_stream_t stream);
+
 /* ------------------------------------------------ several GPUs of a box ---
  * The ranks of a sequence group (one process per GPU) share buffers through
  * peer mappings: fmka_peer_alloc makes a zero-filled device allocation (the one

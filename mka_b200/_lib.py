@@ -64,6 +64,14 @@ _SIGNATURES = {
     "fmka_attn_decode_workspace_size": (c_size_t, [_I, _I, _I, _I, _I]),
     "fmka_attn_decode_splitkv": (_I, [_P, _L, _L, _P, _P, _L, _L, _L, _P, _L, _L, _P, _L,
                                       _I, _I, _I, _I, _I, _F, _I, _P, c_size_t, _P]),
+    "fmka_qk_norm_rope_bf16": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _F, _P, _P, _L, _L, _P, _I, _I,
+                                    _P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _I, _I, _P]),
+    "fmka_attn_varlen_workspace_size": (c_size_t, [_I, _I, _I, _I, _I]),
+    "fmka_attn_varlen": (_I, [_P, _L, _L, _P, _P, _L, _L, _P, _P, _I, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _I,
+                              _I, _I, _F, _P, c_size_t, _P]),
+    "fmka_attn_decode_shared_workspace_size": (c_size_t, [_I, _I, _I, _I, _I]),
+    "fmka_attn_decode_shared": (_I, [_P, _L, _L, _P, _P, _L, _L, _P, _P, _L, _L, _L, _P, _P, _L, _L, _P, _L,
+                                     _I, _I, _I, _I, _I, _I, _F, _P, c_size_t, _P]),
 }
 
 _lib = None

@@ -1,0 +1,547 @@
+// Attention for few or short rows, on mma.sync: packed sequences of different
+// lengths, and single tokens against a prefix shared by the batch plus the
+// request's own keys.
+//
+//   o_r = sum_{j <= lim(r)} softmax_j(scale * q_r k_j) v_j,  lse_r = log sum_j exp(scale * q_r k_j)
+//
+// A row r is a (token, query head) pair: the G query heads of a kv head are
+// rows of one tile, so grouped heads read each K/V row once. One CTA of four
+// warps holds 16 * WM rows; WK = 4 / WM warps share the same rows and take
+// different keys of each 64-key tile (merged at the end through shared memory).
+// K and V tiles arrive by 16-byte cp.async copies into a ring of three stages;
+// rows past the last visible key are filled with zeros instead of being read,
+// so what lies there (another sequence, an unused slot) has no influence, not
+// even as an infinity times a zero weight.
+//
+// Online softmax in fp32 (running max m and sum l per row, base 2); P is
+// rounded to bf16 for the second product because the tensor cores take bf16:
+// half a step of 2^-9 on each weight, the same size as the rounding of the
+// output.
+#include "fmka_internal.h"
+#include "ptx.cuh"
+
+namespace fmka {
+
+namespace {
+
+constexpr int kHeadDim = 128;
+constexpr int kTileKeys = 64;
+constexpr int kStages = 3;
+constexpr int kTileBytes = kTileKeys * kHeadDim * 2;  // 16 KB
+constexpr int kThreads = 128;
+constexpr int kRingBytes = kStages * 2 * kTileBytes;
+constexpr int kSmemBytes = kRingBytes + 16;
+
+enum RowsMode : int { kModeVarlen = 0, kModePrefix = 1, kModeOwn = 2 };
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16-byte copy global -> shared; live == false writes zeros and reads nothing.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  const int n = live ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Byte offset of 16-byte chunk `chunk` (0..15) of row `row` in a tile of 256-byte rows; the XOR spreads the eight
+// rows of an ldmatrix over all banks.
+__device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
+  return row * 256 + ((chunk ^ (row & 7)) << 4);
+}
+
+// Infinities and NaNs among the eight bf16 of a 16-byte chunk are replaced by zeros; true if there were any.
+__device__ __forceinline__ bool zero_nonfinite(uint4& c) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&c);
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = (w[i] & 0x7F80u) == 0x7F80u;
+    const bool hi = (w[i] & 0x7F800000u) == 0x7F800000u;
+    any |= lo | hi;
+    w[i] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
+  }
+  return any;
+}
+
+struct RowsItem {
+  int row0, n_tok;   // first packed token (request), tokens of this tile
+  int64_t kv_off;    // element offset of key 0 of the kv head
+  int kb, ke;        // keys [kb, ke)
+  int lim0;          // last key token 0 sees (token i sees lim0 + i)
+};
+
+// The tile `idx` of the packed sequences: sequence, tokens and keys. Every warp computes it alike. False when idx is
+// past the last tile, or when the offsets are not non-decreasing within the tensors (the status word then says so).
+__device__ __forceinline__ bool find_tile(const PackedAttnParams& p, int tok_per_tile, int idx, RowsItem& it) {
+  const int lane = lane_id();
+  int base = 0;
+  bool found = false;
+  for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+    const int s = s0 + lane;
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+    if (s < p.n_seqs) {
+      q0 = __ldg(p.cu_q + s);
+      q1 = __ldg(p.cu_q + s + 1);
+      k0 = __ldg(p.cu_k + s);
+      k1 = __ldg(p.cu_k + s + 1);
+    }
+    const bool bad = q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k;
+    if (__any_sync(0xffffffffu, bad)) {
+      if (lane == 0) atomicOr(p.status, kStatusBadLaunch);
+      return false;
+    }
+    const int nt = (q1 - q0 + tok_per_tile - 1) / tok_per_tile;
+    int incl = nt;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += x;
+    }
+    const int excl = base + incl - nt;
+    const unsigned hit = __ballot_sync(0xffffffffu, idx >= excl && idx < excl + nt);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      // the late tiles of a causal sequence have the most keys: they come first
+      const int tile = __shfl_sync(0xffffffffu, nt - 1 - (idx - excl), src);
+      q0 = __shfl_sync(0xffffffffu, q0, src);
+      q1 = __shfl_sync(0xffffffffu, q1, src);
+      k0 = __shfl_sync(0xffffffffu, k0, src);
+      k1 = __shfl_sync(0xffffffffu, k1, src);
+      const int t0 = tile * tok_per_tile;
+      it.row0 = q0 + t0;
+      it.n_tok = min(tok_per_tile, q1 - q0 - t0);
+      it.kv_off = (int64_t)k0 * p.kv_st;
+      it.kb = 0;
+      it.ke = k1 - k0;
+      if (p.causal) {
+        it.lim0 = t0 + (k1 - k0) - (q1 - q0);
+        it.ke = max(0, min(it.ke, it.lim0 + it.n_tok));
+      } else {
+        it.lim0 = k1 - k0;
+      }
+      found = true;  // the rest of the list is still checked
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return found;
+}
+
+template <int WM, int MODE>
+__global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_constant__ PackedAttnParams p) {
+  constexpr int WK = 4 / WM;
+  constexpr int kRows = 16 * WM;
+  constexpr int kWarpKeys = kTileKeys / WK;  // keys of a tile per warp
+  constexpr int NT = kWarpKeys / 8;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = warp_id();
+  const int lane = lane_id();
+  const int wm = warp % WM;
+  const int wk = warp / WM;
+  const int hkv = blockIdx.y / p.n_gs;
+  const int g0 = (blockIdx.y % p.n_gs) * p.Gs;
+  const int gn = min(p.Gs, p.G - g0);
+  const int tpt = kRows / p.Gs;  // tokens per tile
+
+  RowsItem it;
+  if constexpr (MODE == kModeVarlen) {
+    if (!find_tile(p, tpt, blockIdx.x, it)) return;
+    it.kv_off += hkv * p.kv_sh;
+  } else if constexpr (MODE == kModePrefix) {
+    const int tile = blockIdx.x / p.n_splits;
+    it.row0 = tile * tpt;
+    it.n_tok = min(tpt, p.B - it.row0);
+    it.kv_off = hkv * p.kv_sh;
+    it.kb = (blockIdx.x % p.n_splits) * p.keys_per_split;
+    it.ke = min(p.P, it.kb + p.keys_per_split);
+    it.lim0 = p.P;
+  } else {
+    it.row0 = blockIdx.x / p.n_splits;
+    it.n_tok = 1;
+    it.kv_off = it.row0 * p.kv_sb + hkv * p.kv_sh;
+    const int len = p.lens != nullptr ? max(0, min(p.cap, __ldg(p.lens + it.row0))) : p.cap;
+    it.kb = (blockIdx.x % p.n_splits) * p.keys_per_split;
+    it.ke = min(len, it.kb + p.keys_per_split);
+    it.lim0 = p.cap;
+  }
+  // tiles from this one on hold keys that some rows see and others do not
+  const int diag_tile = MODE == kModeVarlen && it.n_tok > 1 ? max(0, it.lim0 + 1 - it.kb) / kTileKeys : 0x7FFFFFFF;
+  volatile int* bad_v = reinterpret_cast<volatile int*>(smem + kRingBytes);
+  if (threadIdx.x == 0) *bad_v = 0;
+  const int n_tiles = it.ke > it.kb ? (it.ke - it.kb + kTileKeys - 1) / kTileKeys : 0;
+
+  const __nv_bfloat16* kp = p.k + it.kv_off;
+  const __nv_bfloat16* vp = p.v + it.kv_off;
+  const uint32_t s_base = smem_u32(smem);
+  auto load_tile = [&](int i) {
+    if (i < n_tiles) {
+      const uint32_t ks = s_base + (i % kStages) * 2 * kTileBytes;
+      const int key0 = it.kb + i * kTileKeys;
+#pragma unroll
+      for (int c = 0; c < kTileKeys * 16 / kThreads; ++c) {
+        const int id = c * kThreads + threadIdx.x;
+        const int row = id >> 4, ch = id & 15;
+        const bool live = key0 + row < it.ke;
+        const int64_t off = live ? (int64_t)(key0 + row) * p.kv_st + ch * 8 : 0;
+        cp_async16(ks + tile_off(row, ch), kp + off, live);
+        cp_async16(ks + kTileBytes + tile_off(row, ch), vp + off, live);
+      }
+    }
+    cp_async_commit();
+  };
+  for (int i = 0; i < kStages - 1; ++i) load_tile(i);
+
+  // rows of this thread: r_lo and r_lo + 8 of the warp's 16
+  const int kq = (lane & 3) * 2;
+  int lim[2], tok[2], head[2];
+  bool row_ok[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = wm * 16 + (lane >> 2) + 8 * e;
+    const int i = r / p.Gs, g = r % p.Gs;
+    row_ok[e] = i < it.n_tok && g < gn;
+    tok[e] = it.row0 + i;
+    head[e] = hkv * p.G + g0 + g;
+    lim[e] = min(it.ke - 1, it.lim0 + i);
+  }
+  uint32_t qa[8][4];
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const __nv_bfloat16* src = p.q + tok[e] * p.q_st + head[e] * p.q_sh + ks * 16 + kq;
+      qa[ks][e] = row_ok[e] ? *reinterpret_cast<const uint32_t*>(src) : 0u;
+      qa[ks][2 + e] = row_ok[e] ? *reinterpret_cast<const uint32_t*>(src + 8) : 0u;
+    }
+  }
+
+  float o[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY};
+  float l[2] = {0.f, 0.f};
+  const int mrow = lane & 7;
+  const int msel = lane >> 3;
+
+  for (int i = 0; i < n_tiles; ++i) {
+    cp_async_wait<kStages - 2>();
+    if (MODE == kModeVarlen && i >= diag_tile) {
+      // this thread's own copies are visible to it before the barrier
+#pragma unroll
+      for (int c = 0; c < kTileKeys * 16 / kThreads; ++c) {
+        const int id = c * kThreads + threadIdx.x;
+        uint4* at = reinterpret_cast<uint4*>(smem + ((i % kStages) * 2 + 1) * kTileBytes + tile_off(id >> 4, id & 15));
+        uint4 x = *at;
+        if (zero_nonfinite(x)) {
+          *at = x;
+          *bad_v = 1;
+        }
+      }
+    }
+    __syncthreads();
+    load_tile(i + kStages - 1);
+    const uint32_t kt = s_base + (i % kStages) * 2 * kTileBytes;
+    const uint32_t vt = kt + kTileBytes;
+    const int key0 = it.kb + i * kTileKeys + wk * kWarpKeys;
+    float sc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+      const int row = wk * kWarpKeys + nt * 8 + mrow;
+#pragma unroll
+      for (int s4 = 0; s4 < 4; ++s4) {
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4(kt + tile_off(row, s4 * 4 + msel), b0, b1, b2, b3);
+        mma16816(sc[nt], qa[2 * s4], b0, b1);
+        mma16816(sc[nt], qa[2 * s4 + 1], b2, b3);
+      }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int key = key0 + nt * 8 + kq + (c & 1);
+        sc[nt][c] = key > lim[c >> 1] ? -INFINITY : sc[nt][c] * p.scale_log2;
+        mx[c >> 1] = fmaxf(mx[c >> 1], sc[nt][c]);
+      }
+    }
+    float al[2], sub[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+      const float mn = fmaxf(m[e], mx[e]);
+      sub[e] = mn == -INFINITY ? 0.f : mn;
+      al[e] = fast_exp2(m[e] - sub[e]);
+      m[e] = mn;
+      l[e] *= al[e];
+    }
+    uint32_t pa[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        sc[nt][c] = fast_exp2(sc[nt][c] - sub[c >> 1]);
+        l[c >> 1] += sc[nt][c];
+      }
+      pa[nt][0] = pack_bf16x2(sc[nt][0], sc[nt][1]);
+      pa[nt][1] = pack_bf16x2(sc[nt][2], sc[nt][3]);
+    }
+#pragma unroll
+    for (int dt = 0; dt < 16; ++dt) {
+      o[dt][0] *= al[0];
+      o[dt][1] *= al[0];
+      o[dt][2] *= al[1];
+      o[dt][3] *= al[1];
+    }
+#pragma unroll
+    for (int kt2 = 0; kt2 < NT / 2; ++kt2) {
+      const uint32_t a[4] = {pa[2 * kt2][0], pa[2 * kt2][1], pa[2 * kt2 + 1][0], pa[2 * kt2 + 1][1]};
+      const int row = wk * kWarpKeys + kt2 * 16 + (msel & 1) * 8 + mrow;
+#pragma unroll
+      for (int dp = 0; dp < 8; ++dp) {
+        uint32_t b0, b1, b2, b3;
+        ldsm_x4_trans(vt + tile_off(row, dp * 2 + (msel >> 1)), b0, b1, b2, b3);
+        mma16816(o[2 * dp], a, b0, b1);
+        mma16816(o[2 * dp + 1], a, b2, b3);
+      }
+    }
+  }
+  if (MODE == kModeVarlen && n_tiles > diag_tile && *bad_v) {
+    // rare: the infinities and NaNs taken out above go to the rows that see them
+    for (int e = 0; e < 2; ++e) {
+      for (int j = it.kb + diag_tile * kTileKeys; row_ok[e] && j <= lim[e]; ++j) {
+        const __nv_bfloat16* src = vp + j * p.kv_st + kq;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) {
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(src + dt * 8);
+          if ((x & 0x7F80u) == 0x7F80u) o[dt][2 * e] += bf16lo_to_f32(x);
+          if ((x & 0x7F800000u) == 0x7F800000u) o[dt][2 * e + 1] += bf16hi_to_f32(x);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+  }
+
+  if constexpr (WK > 1) {
+    // merge the warps that hold other keys of the same rows
+    cp_async_wait<0>();
+    __syncthreads();
+    float* so = reinterpret_cast<float*>(smem);            // [4][16][128]
+    float* sm = so + 4 * 16 * kHeadDim;                     // [4][16][2]
+#pragma unroll
+    for (int dt = 0; dt < 16; ++dt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<float2*>(so + (warp * 16 + (lane >> 2) + 8 * e) * kHeadDim + dt * 8 + kq) =
+            make_float2(o[dt][2 * e], o[dt][2 * e + 1]);
+    }
+    if ((lane & 3) == 0) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sm[(warp * 16 + (lane >> 2) + 8 * e) * 2] = m[e];
+        sm[(warp * 16 + (lane >> 2) + 8 * e) * 2 + 1] = l[e];
+      }
+    }
+    __syncthreads();
+    if (wk != 0) return;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = (lane >> 2) + 8 * e;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WK; ++w) M = fmaxf(M, sm[((w * WM + wm) * 16 + r) * 2]);
+      const float Ms = M == -INFINITY ? 0.f : M;
+      float L = 0.f, wt[WK];
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        wt[w] = fast_exp2(sm[((w * WM + wm) * 16 + r) * 2] - Ms);
+        L += wt[w] * sm[((w * WM + wm) * 16 + r) * 2 + 1];
+      }
+      m[e] = M;
+      l[e] = L;
+#pragma unroll
+      for (int dt = 0; dt < 16; ++dt) {
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float2 x = *reinterpret_cast<const float2*>(so + ((w * WM + wm) * 16 + r) * kHeadDim + dt * 8 + kq);
+          a += wt[w] * x.x;
+          b += wt[w] * x.y;
+        }
+        o[dt][2 * e] = a;
+        o[dt][2 * e + 1] = b;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (!row_ok[e]) continue;
+    const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];  // a row that sees no key gives zeros
+    const float lse2 = l[e] == 0.f ? -INFINITY : m[e] + log2f(l[e]);
+    if constexpr (MODE == kModeVarlen) {
+      __nv_bfloat16* dst = p.o + tok[e] * p.o_st + head[e] * p.o_sh + kq;
+#pragma unroll
+      for (int dt = 0; dt < 16; ++dt)
+        *reinterpret_cast<uint32_t*>(dst + dt * 8) = pack_bf16x2(o[dt][2 * e] * inv, o[dt][2 * e + 1] * inv);
+      if ((lane & 3) == 0 && p.lse != nullptr)
+        p.lse[tok[e] * p.lse_st + head[e] * p.lse_sh] = lse2 * 0.69314718055994531f;
+    } else {
+      const int part = p.part0 + blockIdx.x % p.n_splits;
+      const int64_t rec = (int64_t)part * p.B * p.Hq + (int64_t)tok[e] * p.Hq + head[e];
+      if (l[e] != 0.f) {
+        float* dst = p.part_o + rec * kHeadDim + kq;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt)
+          *reinterpret_cast<float2*>(dst + dt * 8) = make_float2(o[dt][2 * e] * inv, o[dt][2 * e + 1] * inv);
+      }
+      if ((lane & 3) == 0) p.part_lse[rec] = lse2;
+    }
+  }
+}
+
+// Joins the parts of every row: one warp per (request, query head).
+__global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__ PackedAttnParams p, int n_parts) {
+  const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = lane_id();
+  const int rows = p.B * p.Hq;
+  if (row >= rows) return;
+  float M = -INFINITY;
+  for (int s = 0; s < n_parts; ++s) {
+    const float x = p.part_lse[(int64_t)s * rows + row];
+    M = x != x ? x : fmaxf(M, x);  // a NaN stays
+  }
+  const float Ms = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < n_parts; ++s) {
+    const float x = p.part_lse[(int64_t)s * rows + row];
+    if (x == -INFINITY) continue;  // this part saw no key: nothing was written
+    const float w = fast_exp2(x - Ms);
+    const float4 v = reinterpret_cast<const float4*>(p.part_o + ((int64_t)s * rows + row) * kHeadDim)[lane];
+    L += w;
+    acc.x += w * v.x;
+    acc.y += w * v.y;
+    acc.z += w * v.z;
+    acc.w += w * v.w;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int b = row / p.Hq, h = row % p.Hq;
+  reinterpret_cast<uint2*>(p.o + b * p.o_st + h * p.o_sh)[lane] =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[b * p.lse_st + h * p.lse_sh] = L == 0.f ? -INFINITY : (Ms + log2f(L)) * 0.69314718055994531f;
+}
+
+template <int WM, int MODE>
+int launch_rows(const PackedAttnParams& p, int64_t gx, cudaStream_t stream, const char* what) {
+  auto kern = attn_rows_kernel<WM, MODE>;
+  int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes), what);
+  if (rc) return rc;
+  if (gx > 0x7FFFFFFF) return set_error(kErrUnsupported, std::string(what) + ": problem too large");
+  kern<<<dim3((unsigned)gx, (unsigned)(p.Hkv * p.n_gs)), kThreads, kSmemBytes, stream>>>(p);
+  return check_cuda(cudaGetLastError(), what);
+}
+
+void slice_group(PackedAttnParams& p, int rows) {
+  p.n_gs = (p.G + rows - 1) / rows;
+  p.Gs = (p.G + p.n_gs - 1) / p.n_gs;
+}
+
+struct SharedPlan {
+  int prefix_splits, prefix_keys;  // parts over the prefix, keys per part
+  int own_splits, own_keys;
+};
+
+SharedPlan plan_shared(int P, int cap) {
+  SharedPlan s{0, kTileKeys, 0, kTileKeys};
+  if (P > 0) {
+    s.prefix_keys = 512;
+    s.prefix_splits = (P + s.prefix_keys - 1) / s.prefix_keys;
+  }
+  if (cap > 0) {
+    s.own_keys = 512;
+    s.own_splits = (cap + s.own_keys - 1) / s.own_keys;
+  }
+  return s;
+}
+
+}  // namespace
+
+size_t attn_varlen_workspace_bytes(int, int, int, int, int) { return 0; }
+
+int launch_attn_varlen(PackedAttnParams p, int, void*, cudaStream_t stream) {
+  p.status = device_status_word();
+  if (p.status == nullptr) return set_error(kErrDevice, "attn_varlen: device status word unavailable");
+  slice_group(p, 64);
+  const int tpt = 64 / p.Gs;
+  const int64_t tiles = (int64_t)p.total_q / tpt + p.n_seqs;  // at least one tile ends in every sequence
+  return launch_rows<4, kModeVarlen>(p, tiles, stream, "attn_varlen launch");
+}
+
+size_t attn_decode_shared_workspace_bytes(int B, int Hq, int Hkv, int P, int cap) {
+  const SharedPlan s = plan_shared(P, cap);
+  return (size_t)(s.prefix_splits + s.own_splits) * B * Hq * (kHeadDim + 1) * sizeof(float);
+}
+
+int launch_attn_decode_shared(PackedAttnParams p, const __nv_bfloat16* kp, const __nv_bfloat16* vp, int64_t kp_sh,
+                              int64_t kp_st, void* workspace, cudaStream_t stream) {
+  p.status = device_status_word();
+  if (p.status == nullptr) return set_error(kErrDevice, "attn_decode_shared: device status word unavailable");
+  const SharedPlan s = plan_shared(p.P, p.cap);
+  const int parts = s.prefix_splits + s.own_splits;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_lse = p.part_o + (int64_t)parts * p.B * p.Hq * kHeadDim;
+  if (s.prefix_splits > 0) {
+    PackedAttnParams a = p;
+    a.k = kp;
+    a.v = vp;
+    a.kv_sh = kp_sh;
+    a.kv_st = kp_st;
+    a.n_splits = s.prefix_splits;
+    a.keys_per_split = s.prefix_keys;
+    a.part0 = 0;
+    slice_group(a, 64);
+    const int tpt = 64 / a.Gs;
+    int rc = launch_rows<4, kModePrefix>(a, (int64_t)((a.B + tpt - 1) / tpt) * a.n_splits, stream,
+                                         "attn_decode_shared prefix launch");
+    if (rc) return rc;
+  }
+  if (s.own_splits > 0) {
+    PackedAttnParams a = p;
+    a.n_splits = s.own_splits;
+    a.keys_per_split = s.own_keys;
+    a.part0 = s.prefix_splits;
+    slice_group(a, 16);
+    int rc = launch_rows<1, kModeOwn>(a, (int64_t)a.B * a.n_splits, stream, "attn_decode_shared own launch");
+    if (rc) return rc;
+  }
+  const int blocks = (p.B * p.Hq + 7) / 8;
+  join_parts_kernel<<<blocks, 256, 0, stream>>>(p, parts);
+  return check_cuda(cudaGetLastError(), "attn_decode_shared join launch");
+}
+
+}  // namespace fmka

@@ -61,6 +61,12 @@ int launch_attn_decode(const __nv_bfloat16* q, int64_t q_sb, int64_t q_sh, const
                        int64_t o_sb, int64_t o_sh, float* lse, int64_t lse_sb, int B, int Hq, int Hkv, int Tk,
                        int head_dim, float scale, int num_splits, void* workspace, size_t workspace_bytes,
                        cudaStream_t stream);
+int launch_qk_norm_rope(QkNormParams p, cudaStream_t stream);
+size_t attn_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv);
+int launch_attn_varlen(PackedAttnParams p, int max_k, void* workspace, cudaStream_t stream);
+size_t attn_decode_shared_workspace_bytes(int B, int Hq, int Hkv, int P, int cap);
+int launch_attn_decode_shared(PackedAttnParams p, const __nv_bfloat16* kp, const __nv_bfloat16* vp, int64_t kp_sh,
+                              int64_t kp_st, void* workspace, cudaStream_t stream);
 
 // ----------------------------------------------------------------- errors --
 namespace {
@@ -637,6 +643,193 @@ int fmka_attn_decode_splitkv(const void* q, int64_t q_sb, int64_t q_sh, const vo
   return launch_attn_decode(bf(q), q_sb, q_sh, bf(k), bf(v), kv_sb, kv_sh, kv_st, bfw(o), o_sb, o_sh, lse, lse_sb,
                             B, Hq, Hkv, Tk, head_dim, scale, num_splits, workspace, workspace_bytes,
                             as_stream(stream));
+}
+
+// ------------------------------------------------- packed serving operators --
+int fmka_qk_norm_rope_bf16(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k, int64_t k_sb,
+                           int64_t k_st, int64_t k_sh, const void* q_weight, const void* k_weight,
+                           int weight_is_f32, float eps, const float* rope_cos, const float* rope_sin,
+                           int64_t rope_sb, int64_t rope_st, const void* positions, int positions_are_i64,
+                           int n_positions, void* q_out, int64_t qo_sb, int64_t qo_st, int64_t qo_sh, void* k_out,
+                           int64_t ko_sb, int64_t ko_st, int64_t ko_sh, int B, int T, int Hq, int Hkv, int head_dim,
+                           fmka_stream_t stream) {
+  if (q == nullptr || q_out == nullptr || (Hkv > 0 && (k == nullptr || k_out == nullptr)))
+    return set_error(kErrInvalidArgument, "qk_norm_rope: null pointer");
+  if (B <= 0 || T <= 0 || Hq <= 0 || Hkv < 0) return set_error(kErrInvalidArgument, "qk_norm_rope: empty shape");
+  if (head_dim != 128) return set_error(kErrUnsupported, "qk_norm_rope: head_dim must be 128");
+  if (!std::isfinite(eps) || eps < 0.f)
+    return set_error(kErrInvalidArgument, "qk_norm_rope: eps must be finite and >= 0");
+  if ((rope_cos == nullptr) != (rope_sin == nullptr))
+    return set_error(kErrInvalidArgument, "qk_norm_rope: cos and sin go together");
+  if (positions != nullptr && (rope_cos == nullptr || n_positions <= 0))
+    return set_error(kErrInvalidArgument, "qk_norm_rope: positions need cos/sin tables");
+  if (!al16(q) || !al16(k) || !al16(q_out) || !al16(k_out) || !al16(q_weight) || !al16(k_weight) || !al16(rope_cos) ||
+      !al16(rope_sin))
+    return set_error(kErrInvalidArgument, "qk_norm_rope: tensors must be 16-byte aligned");
+  if ((q_sb | q_st | q_sh | k_sb | k_st | k_sh | qo_sb | qo_st | qo_sh | ko_sb | ko_st | ko_sh) & 7)
+    return set_error(kErrInvalidArgument, "qk_norm_rope: strides must be multiples of 8 elements");
+  if ((rope_sb | rope_st) & 3)
+    return set_error(kErrInvalidArgument, "qk_norm_rope: table strides must be multiples of 4 elements");
+  if (positions != nullptr && (reinterpret_cast<uintptr_t>(positions) & (positions_are_i64 ? 7u : 3u)))
+    return set_error(kErrInvalidArgument, "qk_norm_rope: positions must be aligned to their type");
+  QkNormParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.x[0] = bf(q);
+  p.x[1] = bf(k);
+  p.y[0] = bfw(q_out);
+  p.y[1] = bfw(k_out);
+  p.x_sb[0] = q_sb;
+  p.x_st[0] = q_st;
+  p.x_sh[0] = q_sh;
+  p.x_sb[1] = k_sb;
+  p.x_st[1] = k_st;
+  p.x_sh[1] = k_sh;
+  p.y_sb[0] = qo_sb;
+  p.y_st[0] = qo_st;
+  p.y_sh[0] = qo_sh;
+  p.y_sb[1] = ko_sb;
+  p.y_st[1] = ko_st;
+  p.y_sh[1] = ko_sh;
+  p.w[0] = q_weight;
+  p.w[1] = k_weight;
+  p.w_f32[0] = weight_is_f32 & 1;
+  p.w_f32[1] = (weight_is_f32 >> 1) & 1;
+  p.eps = eps;
+  p.cos = rope_cos;
+  p.sin = rope_sin;
+  p.rope_sb = rope_sb;
+  p.rope_st = rope_st;
+  p.positions = positions;
+  p.pos_i64 = positions_are_i64;
+  p.n_pos = n_positions;
+  p.B = B;
+  p.T = T;
+  p.Hq = Hq;
+  p.Hk = Hkv;
+  return launch_qk_norm_rope(p, as_stream(stream));
+}
+
+namespace {
+// What both packed attention entry points ask of their tensors.
+int check_packed_attn(const PackedAttnParams& p, int head_dim, float scale, const char* who) {
+  const std::string w(who);
+  if (p.Hq <= 0 || p.Hkv <= 0) return set_error(kErrInvalidArgument, w + ": empty shape");
+  if (head_dim != 128) return set_error(kErrUnsupported, w + ": head_dim must be 128");
+  if (p.Hq % p.Hkv != 0)
+    return set_error(kErrInvalidArgument, w + ": query heads must be a multiple of kv heads");
+  if (!std::isfinite(scale) || scale < 0.f)
+    return set_error(kErrInvalidArgument, w + ": scale must be finite and >= 0");
+  if ((p.q_st | p.q_sh | p.kv_sb | p.kv_st | p.kv_sh | p.o_st | p.o_sh) & 7)
+    return set_error(kErrInvalidArgument, w + ": strides must be multiples of 8 elements");
+  if (!al16(p.q) || !al16(p.k) || !al16(p.v) || !al16(p.o))
+    return set_error(kErrInvalidArgument, w + ": tensors must be 16-byte aligned");
+  return kOk;
+}
+}  // namespace
+
+size_t fmka_attn_varlen_workspace_size(int n_seqs, int total_q, int max_k, int Hq, int Hkv) {
+  if (n_seqs <= 0 || total_q <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return 0;
+  return attn_varlen_workspace_bytes(n_seqs, total_q, max_k, Hq, Hkv);
+}
+
+int fmka_attn_varlen(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
+                     int64_t kv_sh, const int32_t* cu_q, const int32_t* cu_k, int n_seqs, void* o, int64_t o_st,
+                     int64_t o_sh, float* lse, int64_t lse_st, int64_t lse_sh, int total_q, int total_k, int max_k,
+                     int Hq, int Hkv, int head_dim, int causal, float scale, void* workspace, size_t workspace_bytes,
+                     fmka_stream_t stream) {
+  if (n_seqs < 0 || total_q < 0 || total_k < 0 || max_k < 0)
+    return set_error(kErrInvalidArgument, "attn_varlen: negative size");
+  if (n_seqs == 0 || total_q == 0) return kOk;
+  if (q == nullptr || o == nullptr || cu_q == nullptr || cu_k == nullptr ||
+      (total_k > 0 && (k == nullptr || v == nullptr)))
+    return set_error(kErrInvalidArgument, "attn_varlen: null pointer");
+  if ((reinterpret_cast<uintptr_t>(cu_q) | reinterpret_cast<uintptr_t>(cu_k)) & 3u)
+    return set_error(kErrInvalidArgument, "attn_varlen: the offsets must be 4-byte aligned");
+  PackedAttnParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = bf(q);
+  p.q_st = q_st;
+  p.q_sh = q_sh;
+  p.k = bf(k);
+  p.v = bf(v);
+  p.kv_st = kv_st;
+  p.kv_sh = kv_sh;
+  p.cu_q = cu_q;
+  p.cu_k = cu_k;
+  p.n_seqs = n_seqs;
+  p.o = bfw(o);
+  p.o_st = o_st;
+  p.o_sh = o_sh;
+  p.lse = lse;
+  p.lse_st = lse_st;
+  p.lse_sh = lse_sh;
+  p.total_q = total_q;
+  p.total_k = total_k;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.causal = causal;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  const int rc = check_packed_attn(p, head_dim, scale, "attn_varlen");
+  if (rc) return rc;
+  p.G = Hq / Hkv;
+  const size_t need = attn_varlen_workspace_bytes(n_seqs, total_q, max_k, Hq, Hkv);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return set_error(kErrWorkspace, "attn_varlen: workspace too small (need " + std::to_string(need) + " bytes)");
+  if (!al16(workspace)) return set_error(kErrInvalidArgument, "attn_varlen: workspace must be 16-byte aligned");
+  return launch_attn_varlen(p, max_k, workspace, as_stream(stream));
+}
+
+size_t fmka_attn_decode_shared_workspace_size(int B, int Hq, int Hkv, int P, int Tcap) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || P < 0 || Tcap < 0) return 0;
+  return attn_decode_shared_workspace_bytes(B, Hq, Hkv, P, Tcap);
+}
+
+int fmka_attn_decode_shared(const void* q, int64_t q_sb, int64_t q_sh, const void* k_prefix, const void* v_prefix,
+                            int64_t p_sh, int64_t p_st, const void* k, const void* v, int64_t kv_sb, int64_t kv_sh,
+                            int64_t kv_st, const int32_t* lens, void* o, int64_t o_sb, int64_t o_sh, float* lse,
+                            int64_t lse_sb, int B, int Hq, int Hkv, int P, int Tcap, int head_dim, float scale,
+                            void* workspace, size_t workspace_bytes, fmka_stream_t stream) {
+  if (B <= 0 || P < 0 || Tcap < 0) return set_error(kErrInvalidArgument, "attn_decode_shared: empty shape");
+  if (q == nullptr || o == nullptr || (P > 0 && (k_prefix == nullptr || v_prefix == nullptr)) ||
+      (Tcap > 0 && (k == nullptr || v == nullptr)))
+    return set_error(kErrInvalidArgument, "attn_decode_shared: null pointer");
+  if (reinterpret_cast<uintptr_t>(lens) & 3u)
+    return set_error(kErrInvalidArgument, "attn_decode_shared: lens must be 4-byte aligned");
+  PackedAttnParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = bf(q);
+  p.q_st = q_sb;
+  p.q_sh = q_sh;
+  p.k = bf(k);
+  p.v = bf(v);
+  p.kv_sb = kv_sb;
+  p.kv_sh = kv_sh;
+  p.kv_st = kv_st;
+  p.lens = lens;
+  p.o = bfw(o);
+  p.o_st = o_sb;
+  p.o_sh = o_sh;
+  p.lse = lse;
+  p.lse_st = lse_sb;
+  p.lse_sh = 1;
+  p.B = B;
+  p.P = P;
+  p.cap = Tcap;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  const int rc = check_packed_attn(p, head_dim, scale, "attn_decode_shared");
+  if (rc) return rc;
+  if (((p_sh | p_st) & 7) || !al16(k_prefix) || !al16(v_prefix))
+    return set_error(kErrInvalidArgument,
+                     "attn_decode_shared: the prefix must be 16-byte aligned with strides % 8 == 0");
+  p.G = Hq / Hkv;
+  const size_t need = attn_decode_shared_workspace_bytes(B, Hq, Hkv, P, Tcap);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return set_error(kErrWorkspace,
+                     "attn_decode_shared: workspace too small (need " + std::to_string(need) + " bytes)");
+  if (!al16(workspace)) return set_error(kErrInvalidArgument, "attn_decode_shared: workspace must be 16-byte aligned");
+  return launch_attn_decode_shared(p, bf(k_prefix), bf(v_prefix), p_sh, p_st, workspace, as_stream(stream));
 }
 
 }  // extern "C"

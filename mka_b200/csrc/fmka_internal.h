@@ -109,6 +109,56 @@ __host__ __device__ __forceinline__ void gemm_tile_coords(int tile, int num_m, i
 int launch_gemm(const __nv_bfloat16* A, int64_t lda, const __nv_bfloat16* B, int64_t ldb, const GemmParams& p,
                 int num_sms, cudaStream_t stream);
 
+// ------------------------------------------------- packed serving operators --
+struct QkNormParams {
+  const __nv_bfloat16* x[2];   // q, k: x[b, t, h, :]
+  __nv_bfloat16* y[2];
+  int64_t x_sb[2], x_st[2], x_sh[2];
+  int64_t y_sb[2], y_st[2], y_sh[2];
+  const void* w[2];            // [128] or null (no norm)
+  int w_f32[2];                // weights are fp32 instead of bf16
+  float eps;
+  const float* cos;            // rows of 128 or null (no rotation)
+  const float* sin;
+  int64_t rope_sb, rope_st;    // row of token (b, t) without positions
+  const void* positions;       // [B * T] rows of the table, or null
+  int pos_i64;
+  int n_pos;                   // rows of the table
+  int B, T, Hq, Hk;
+  int iters;                   // groups of four heads per warp (set by the launcher)
+  uint32_t* status;
+};
+
+// Attention over packed sequences, and over a shared prefix plus own keys.
+// Rows are (token, query head of a kv head's group) pairs.
+struct PackedAttnParams {
+  const __nv_bfloat16* q;      // q[row, head, :], row = packed token or request
+  int64_t q_st, q_sh;
+  const __nv_bfloat16* k;      // packed: k[token, head, :]; own keys: k[request, head, slot, :]
+  const __nv_bfloat16* v;
+  int64_t kv_sb, kv_st, kv_sh;
+  __nv_bfloat16* o;            // o[row, head, :]
+  int64_t o_st, o_sh;
+  float* lse;                  // lse[row * lse_st + head * lse_sh], may be null
+  int64_t lse_st, lse_sh;
+  int Hq, Hkv;
+  int G;                       // query heads per kv head
+  int Gs, n_gs;                // heads per slice of the group, slices
+  float scale_log2;            // softmax scale * log2(e)
+  // packed sequences
+  const int* cu_q;
+  const int* cu_k;
+  int n_seqs, total_q, total_k, causal;
+  // shared prefix / own keys
+  int B, P, cap;
+  const int* lens;             // keys of each request, may be null (all cap)
+  int keys_per_split, n_splits;
+  int part0;                   // index of this launch's first part
+  float* part_o;               // [parts][B * Hq][128]
+  float* part_lse;             // [parts][B * Hq] log2-sum-exp
+  uint32_t* status;
+};
+
 // Device status word used by kernels to report bounded-wait timeouts; one per
 // device, allocated lazily.
 uint32_t* device_status_word();

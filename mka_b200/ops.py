@@ -488,6 +488,233 @@ def silu_mul(g: torch.Tensor, u: torch.Tensor, out: Optional[torch.Tensor] = Non
     return out
 
 
+# ------------------------------------------- packed serving operators --
+def _check_same_device(dev: torch.device, what: str, *ts: Optional[torch.Tensor]) -> None:
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{what}: all tensors must be on {dev}")
+
+
+def _strides(t: torch.Tensor) -> Tuple[int, ...]:
+    """Element strides, 0 for dimensions of one element (whose stride says nothing)."""
+    return tuple(0 if n == 1 else st for n, st in zip(t.shape, t.stride()))
+
+
+def _check_out(what: str, out: torch.Tensor, shape: Sequence[int], dev: torch.device) -> None:
+    _check_bf16(out)
+    if tuple(out.shape) != tuple(shape) or out.device != dev or out.stride(-1) != 1 or any(
+            st == 0 and n > 1 for n, st in zip(out.shape, out.stride())):
+        raise RuntimeError(f"{what} must be a bf16 tensor of shape {tuple(shape)} on {dev} with contiguous channels "
+                           "and no expanded dimension")
+
+
+def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                 positions: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """RMS norm of every query and key head and the rotate-half position rotation, in one pass.
+
+    q [T, Hq, 128] or [B, T, Hq, 128] and k likewise with Hkv heads (or None),
+    bf16, any strides with contiguous channels: slices of one packed q/k/v
+    projection, or transposed views of the head-split [B, H, T, 128] layout.
+    Per head: y = rope(x * rsqrt(mean(x^2) + eps) * weight), fp32 inside, one
+    rounding. q_weight / k_weight [128] bf16 or fp32; None leaves that norm out.
+    rope: fp32 (cos, sin), [T, 128] or [1|B, T, 128] per token, or with
+    `positions` (int32 / int64 of q's token shape) tables [P, 128] indexed by
+    position; None leaves the rotation out. A token at position -1 is padding:
+    its output rows are left as they were; any other position outside the table
+    does the same and sets STATUS_BAD_LAUNCH in the device status word.
+    q_out / k_out: any strided tensors of the inputs' shapes, q and k themselves
+    included. Returns (q_out, k_out).
+    """
+    _check_cuda(q, k, q_weight, k_weight, positions)
+    _check_bf16(q, k)
+    dev = q.device
+    _check_same_device(dev, "qk_norm_rope", k, q_weight, k_weight, positions)
+    if q.dim() not in (3, 4) or q.shape[-1] != HEAD_DIM or q.stride(-1) != 1:
+        raise RuntimeError("qk_norm_rope: q must be [T, Hq, 128] or [B, T, Hq, 128] with contiguous channels")
+    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != HEAD_DIM
+                          or k.stride(-1) != 1):
+        raise RuntimeError("qk_norm_rope: k must be q's shape with Hkv heads and contiguous channels")
+    w_f32 = 0
+    for bit, w in enumerate((q_weight, k_weight)):
+        if w is None:
+            continue
+        if w.shape != (HEAD_DIM,) or not w.is_contiguous() or w.dtype not in (torch.bfloat16, torch.float32):
+            raise RuntimeError("qk_norm_rope: the norm weights must be contiguous bf16 or fp32 [128] tensors")
+        w_f32 |= int(w.dtype == torch.float32) << bit
+    T, Hq = q.shape[-3], q.shape[-2]
+    B = q.shape[0] if q.dim() == 4 else 1
+    Hkv = 0 if k is None else k.shape[-2]
+    pos_i64 = n_pos = 0
+    if positions is not None:
+        if rope is None:
+            raise RuntimeError("qk_norm_rope: positions need the cos/sin tables")
+        if positions.shape != q.shape[:-2] or positions.dtype not in (torch.int32, torch.int64):
+            raise RuntimeError("qk_norm_rope: positions must be int32 or int64 of q's token shape")
+        positions = positions.contiguous()
+        pos_i64 = int(positions.dtype == torch.int64)
+        n_pos = rope[0].shape[0]
+        if rope[0].dim() != 2 or rope[0].shape != rope[1].shape or n_pos == 0:
+            raise RuntimeError("qk_norm_rope: with positions, cos and sin must be tables [P, 128]")
+        cos, sin, rsb, rst = _rope_args(rope, 1, n_pos)
+    else:
+        cos, sin, rsb, rst = _rope_args(rope, B, T)
+    _check_same_device(dev, "qk_norm_rope", cos, sin)
+    if q_out is None:
+        q_out = torch.empty_like(q)
+    else:
+        _check_out("qk_norm_rope: q_out", q_out, q.shape, dev)
+    if k is None:
+        k_out = None
+    elif k_out is None:
+        k_out = torch.empty_like(k)
+    else:
+        _check_out("qk_norm_rope: k_out", k_out, k.shape, dev)
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        return q_out, k_out
+    if Hq == 0:
+        raise RuntimeError("qk_norm_rope: q needs at least one head")
+
+    def st(t):
+        return (0, 0, 0) if t is None else (0,) * (4 - t.dim()) + _strides(t)[:-1]
+
+    with torch.cuda.device(dev):
+        _lib.call("fmka_qk_norm_rope_bf16", q.data_ptr(), *st(q), _ptr(k), *st(k), _ptr(q_weight), _ptr(k_weight),
+                  w_f32, float(eps), _ptr(cos), _ptr(sin), rsb, rst, _ptr(positions), pos_i64, n_pos,
+                  q_out.data_ptr(), *st(q_out), _ptr(k_out), *st(k_out), B, T, Hq, Hkv, HEAD_DIM, _stream(q))
+    return q_out, k_out
+
+
+def _check_heads(what: str, Hq: int, Hkv: int, *ts: torch.Tensor) -> None:
+    for t in ts:
+        if t.shape[-1] != HEAD_DIM or t.stride(-1) != 1:
+            raise RuntimeError(f"{what}: head_dim must be 128 with contiguous channels")
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise RuntimeError(f"{what}: query heads must be a multiple of kv heads")
+
+
+def _same_kv(what: str, k: torch.Tensor, v: torch.Tensor) -> None:
+    if k.shape != v.shape or _strides(k) != _strides(v):
+        raise RuntimeError(f"{what}: k and v must have the same shape and strides")
+
+
+def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                max_k: Optional[int] = None, causal: bool = True, scale: Optional[float] = None,
+                out: Optional[torch.Tensor] = None,
+                want_lse: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Attention over sequences packed one behind the other, without padding.
+
+    q [Tq, Hq, 128], k/v [Tk, Hkv, 128] (any strides with contiguous head dim,
+    e.g. slices of one packed projection); cu_q, cu_k: int32 [S + 1] offsets on
+    the GPU, sequence s owning rows [cu[s], cu[s+1]). With causal, query i of a
+    sequence of Lq queries and Lk keys sees keys j <= i + Lk - Lq, so prompts
+    (Lq == Lk), chunks of prompts behind a history and single tokens mix freely
+    in one call; a row that sees no key gives zeros and a log-sum-exp of -inf.
+    max_k: the longest sequence's keys if the caller knows it (a bound that
+    sizes the scratch memory; it limits nothing). The offsets must be
+    non-decreasing and within the tensors: if not, nothing is written and
+    STATUS_BAD_LAUNCH is set in the device status word. Returns o [Tq, Hq, 128]
+    (or `out`, any strides; rows outside every sequence are left as they were)
+    and lse [Hq, Tq] fp32.
+    """
+    _check_cuda(q, k, v, cu_q, cu_k)
+    _check_bf16(q, k, v)
+    dev = q.device
+    _check_same_device(dev, "attn_varlen", k, v, cu_q, cu_k)
+    if q.dim() != 3 or k.dim() != 3:
+        raise RuntimeError("attn_varlen: expected q [Tq, Hq, 128] and k/v [Tk, Hkv, 128]")
+    _same_kv("attn_varlen", k, v)
+    Tq, Hq, Dh = q.shape
+    Tk, Hkv, _ = k.shape
+    _check_heads("attn_varlen", Hq, Hkv, q, k, v)
+    for cu in (cu_q, cu_k):
+        if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 1 or not cu.is_contiguous():
+            raise RuntimeError("attn_varlen: cu_q and cu_k must be contiguous int32 [S + 1] tensors")
+    if cu_q.numel() != cu_k.numel():
+        raise RuntimeError("attn_varlen: cu_q and cu_k must describe the same sequences")
+    S = cu_q.numel() - 1
+    if max_k is None:
+        max_k = Tk
+    elif max_k < 0:
+        raise RuntimeError("attn_varlen: max_k must not be negative")
+    if out is None:
+        out = torch.empty((Tq, Hq, Dh), dtype=torch.bfloat16, device=dev)
+    else:
+        _check_out("attn_varlen: out", out, q.shape, dev)
+    lse = torch.empty((Hq, Tq), dtype=torch.float32, device=dev) if want_lse else None
+    if Tq == 0 or S == 0:
+        return out, lse
+    max_k = min(int(max_k), Tk)
+    qs, ks, os_ = _strides(q), _strides(k), _strides(out)
+    with torch.cuda.device(dev):
+        ws_bytes = _lib.load().fmka_attn_varlen_workspace_size(S, Tq, max_k, Hq, Hkv)
+        # one allocation per call: a buffer kept between calls would be shared by
+        # captured graphs that replay on different streams
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        _lib.call("fmka_attn_varlen", q.data_ptr(), qs[0], qs[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
+                  cu_q.data_ptr(), cu_k.data_ptr(), S, out.data_ptr(), os_[0], os_[1], _ptr(lse), 1, Tq, Tq, Tk,
+                  max_k, Hq, Hkv, Dh, int(causal), 1.0 / math.sqrt(Dh) if scale is None else float(scale), _ptr(ws),
+                  ws_bytes, _stream(q))
+    return out, lse
+
+
+def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor,
+                       v: torch.Tensor, lens: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                       out: Optional[torch.Tensor] = None,
+                       want_lse: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Single-token attention of a batch whose requests share a prefix.
+
+    q [B, Hq, 1, 128] or [B, Hq, 128]; k_prefix / v_prefix [Hkv, P, 128] (or
+    [1, Hkv, P, 128]), the keys and values every request sees first, read once
+    for the whole batch; k / v [B, Hkv, Tcap, 128], each request's own cache
+    behind the prefix, of which the first lens[b] slots are valid (int32 [B] on
+    the GPU, clamped to [0, Tcap]; None: all of them). Strided views are fine.
+    The result is attn_decode's over the concatenated keys. Either part may be
+    empty; a request without any key gives zeros and a log-sum-exp of -inf.
+    Returns o [B, 1, Hq, 128] and lse [B, Hq].
+    """
+    _check_cuda(q, k_prefix, v_prefix, k, v, lens)
+    _check_bf16(q, k_prefix, v_prefix, k, v)
+    dev = q.device
+    _check_same_device(dev, "attn_decode_shared", k_prefix, v_prefix, k, v, lens)
+    if q.dim() == 4 and q.shape[2] == 1:
+        q = q[:, :, 0]
+    if q.dim() != 3:
+        raise RuntimeError("attn_decode_shared: one query token per request, q [B, Hq, 1, 128] or [B, Hq, 128]")
+    if k_prefix.dim() == 4 and k_prefix.shape[0] == 1 and v_prefix.dim() == 4 and v_prefix.shape[0] == 1:
+        k_prefix, v_prefix = k_prefix[0], v_prefix[0]
+    if k_prefix.dim() != 3 or k.dim() != 4:
+        raise RuntimeError("attn_decode_shared: expected a prefix [Hkv, P, 128] and k/v [B, Hkv, Tcap, 128]")
+    _same_kv("attn_decode_shared", k_prefix, v_prefix)
+    _same_kv("attn_decode_shared", k, v)
+    B, Hq, Dh = q.shape
+    Hkv, P, _ = k_prefix.shape
+    Tcap = k.shape[2]
+    if k.shape[0] != B or k.shape[1] != Hkv:
+        raise RuntimeError("attn_decode_shared: k/v must hold q's batch and the prefix's kv heads")
+    _check_heads("attn_decode_shared", Hq, Hkv, q, k_prefix, v_prefix, k, v)
+    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous()):
+        raise RuntimeError("attn_decode_shared: lens must be a contiguous int32 [B] tensor")
+    if out is None:
+        out = torch.empty((B, 1, Hq, Dh), dtype=torch.bfloat16, device=dev)
+    else:
+        _check_out("attn_decode_shared: out", out, (B, 1, Hq, Dh), dev)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if want_lse else None
+    if B == 0:
+        return out, lse
+    qs, ps, ks, os_ = _strides(q), _strides(k_prefix), _strides(k), _strides(out)
+    with torch.cuda.device(dev):
+        ws_bytes = _lib.load().fmka_attn_decode_shared_workspace_size(B, Hq, Hkv, P, Tcap)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None  # as in attn_varlen
+        _lib.call("fmka_attn_decode_shared", q.data_ptr(), qs[0], qs[1], k_prefix.data_ptr(), v_prefix.data_ptr(),
+                  ps[0], ps[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], _ptr(lens), out.data_ptr(), os_[0],
+                  os_[2], _ptr(lse), Hq, B, Hq, Hkv, P, Tcap, Dh,
+                  1.0 / math.sqrt(Dh) if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(q))
+    return out, lse
+
+
 # ------------------------------------------------------------ L3 recall --
 def gemm_f32out(a: torch.Tensor, w: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[M, N] = a[M, K] @ w[N, K]^T in fp32 (bf16 operands, tcgen05)."""

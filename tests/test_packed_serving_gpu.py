@@ -1,0 +1,608 @@
+"""The packed serving operators (per-head q/k norm with rotation, attention over
+packed sequences, single-token attention behind a shared prefix) against plain
+implementations in 64 bits.
+
+Tolerances. bf16 rounds by at most h = 2^-8 of a value. qk_norm_rope computes in
+fp32 and rounds once: h * |y|, plus 2^-20 of the two rotated terms for the fp32
+arithmetic. Attention rounds each softmax weight to bf16 for the second product,
+which moves the output by at most h * sum_j p_j |v_j|, and rounds the output once,
+h * |o|; 2^-12 * sum_j p_j |v_j| covers the fp32 scores and exponentials (a score
+is a 128-term fp32 sum, off by about 1e-5 here). The log-sum-exp is fp32: 1e-4,
+and 2^-20 of its value: the largest score is summed in eight steps of 16 products,
+each of which may lose a step of 2^-23 of the partial sum where all products have
+one sign (8 * 2^-23 = 2^-20), which shows once the value is in the hundreds.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+H_BF16 = 2.0 ** -8
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from mka_b200 import ops as _ops
+
+    _ops.device_status()
+    return _ops
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(g, *shape, scale=1.0):
+    return (torch.randn(*shape, device=DEV, generator=g) * scale).bfloat16()
+
+
+# --------------------------------------------------------------- references --
+def _tables(pos):
+    inv = 10000.0 ** (-torch.arange(0, 128, 2, dtype=torch.float64, device=DEV) / 128)
+    a = pos.double()[..., None] * inv
+    a = torch.cat([a, a], -1)
+    return a.cos().float(), a.sin().float()
+
+
+def _ref_norm(x, w, eps, cos, sin):
+    """x [..., H, 128]; cos / sin [..., 128] or None. Returns the value and the size of its terms."""
+    x = x.double()
+    if w is not None:
+        x = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w.double()
+    if cos is None:
+        return x, x.abs()
+    c, s = cos.double().unsqueeze(-2), sin.double().unsqueeze(-2)
+    turned = torch.cat([-x[..., 64:], x[..., :64]], -1)
+    return x * c + turned * s, (x * c).abs() + (turned * s).abs()
+
+
+def _check_norm(got, x, w, eps, cos, sin):
+    ref, size = _ref_norm(x, w, eps, cos, sin)
+    err = (got.double() - ref).abs()
+    assert torch.isfinite(err).all()
+    assert (err <= H_BF16 * ref.abs() * (1 + 2.0 ** -8) + 2.0 ** -20 * size + 1e-30).all(), err.max().item()
+
+
+def _ref_rows(q, k, v, see, scale):
+    """q [R, 128], k / v [S, 128], see [R, S]: o, sum p|v|, lse in 64 bits."""
+    s = (q.double() @ k.double().t()) * scale
+    s = s.masked_fill(~see, -math.inf)
+    m = s.amax(-1, keepdim=True) if s.shape[1] else torch.full((s.shape[0], 1), -math.inf, device=DEV)
+    e = torch.exp(s - m.masked_fill(m == -math.inf, 0.0)).masked_fill(~see, 0.0)
+    z = e.sum(-1, keepdim=True)
+    p = e / z.masked_fill(z == 0, 1.0)
+    v = torch.nan_to_num(v.double()) if not see.all() else v.double()
+    return p @ v, p @ v.abs(), (z.log() + m).squeeze(-1)
+
+
+def _check_attn(o, lse, ro, size, rl, what=""):
+    err = (o.double() - ro).abs()
+    assert torch.isfinite(o.double()).all(), what
+    tol = H_BF16 * (size + ro.abs()) * (1 + 2.0 ** -8) + 2.0 ** -12 * size
+    assert (err <= tol).all(), (what, (err - tol).max().item())
+    if lse is not None:
+        empty = torch.isinf(rl)
+        assert torch.equal(torch.isinf(lse) & (lse < 0), empty), what
+        assert ((lse.double() - rl).abs()[~empty] <= 1e-4 + 2.0 ** -20 * rl.abs()[~empty]).all(), what
+
+
+def _check_varlen(o, lse, q, k, v, q_lens, k_lens, causal, scale=128 ** -0.5):
+    G = q.shape[1] // k.shape[1]
+    q0 = k0 = 0
+    for i, (lq, lk) in enumerate(zip(q_lens, k_lens)):
+        see = torch.ones(lq, lk, dtype=torch.bool, device=DEV)
+        if causal:
+            see = torch.arange(lk, device=DEV)[None] <= torch.arange(lq, device=DEV)[:, None] + lk - lq
+        for h in range(q.shape[1]):
+            kk, vv = k[k0:k0 + lk, h // G], v[k0:k0 + lk, h // G]
+            ref = _ref_rows(q[q0:q0 + lq, h], kk, vv, see, scale)
+            _check_attn(o[q0:q0 + lq, h], None if lse is None else lse[h, q0:q0 + lq], *ref, what=(i, lq, lk, h))
+        q0, k0 = q0 + lq, k0 + lk
+
+
+def _cu(lens):
+    return torch.tensor([0] + list(lens), device=DEV).cumsum(0).int()
+
+
+def _check_shared(o, lse, q, kp, vp, k, v, lens, scale=128 ** -0.5):
+    G = q.shape[1] // kp.shape[0]
+    for b, n in enumerate(lens):
+        for h in range(q.shape[1]):
+            kk = torch.cat([kp[h // G], k[b, h // G, :n]])
+            vv = torch.cat([vp[h // G], v[b, h // G, :n]])
+            see = torch.ones(1, kk.shape[0], dtype=torch.bool, device=DEV)
+            ref = _ref_rows(q[b, h][None], kk, vv, see, scale)
+            _check_attn(o[b, 0, h][None], None if lse is None else lse[b, h][None], *ref, what=(b, n, h))
+
+
+# ------------------------------------------------------------- qk_norm_rope --
+@pytest.mark.parametrize("T,Hq,Hkv", [(1, 1, 1), (1, 32, 8), (3, 28, 4), (64, 32, 8), (129, 5, 2), (1021, 7, 7),
+                                      (77, 16, 16), (2500, 28, 4)])
+@pytest.mark.parametrize("layout", ["fused", "heads"])
+def test_norm_rope(ops, T, Hq, Hkv, layout):
+    g = _gen(T + Hq)
+    if layout == "fused":
+        x = _randn(g, T, Hq + 2 * Hkv, 128, scale=3.0)
+        q, k = x[:, :Hq], x[:, Hq:Hq + Hkv]
+    else:
+        q, k = _randn(g, Hq, T, 128).transpose(0, 1), _randn(g, Hkv, T, 128).transpose(0, 1)
+    qw, kw = 1 + _randn(g, 128, scale=0.3), 1 + _randn(g, 128, scale=0.3)
+    cos, sin = _tables(torch.arange(T, device=DEV) + 5000)
+    qo, ko = ops.qk_norm_rope(q, k, qw, kw, 1e-6, rope=(cos, sin))
+    assert qo.shape == q.shape and ko.shape == k.shape
+    _check_norm(qo, q, qw, 1e-6, cos, sin)
+    _check_norm(ko, k, kw, 1e-6, cos, sin)
+
+
+@pytest.mark.parametrize("pos_dtype", [torch.int32, torch.int64])
+def test_norm_rope_batched_positions_and_padding(ops, pos_dtype):
+    g = _gen(3)
+    B, T, Hq, Hkv, P = 3, 37, 6, 2, 500
+    q, k = _randn(g, B, T, Hq, 128), _randn(g, B, T, Hkv, 128)
+    qw, kw = torch.randn(128, device=DEV, generator=g), 1 + _randn(g, 128)  # one fp32, one bf16 weight
+    cos, sin = _tables(torch.arange(P, device=DEV))
+    pos = torch.randint(0, P, (B, T), device=DEV, generator=g).to(pos_dtype)
+    pos[0, :5] = pos[2, -3:] = -1  # padding
+    qo, ko = torch.full_like(q, 7.0), torch.full_like(k, 7.0)
+    ops.qk_norm_rope(q, k, qw, kw, 1e-5, rope=(cos, sin), positions=pos, q_out=qo, k_out=ko)
+    live = pos >= 0
+    at = pos.clamp(min=0).long()
+    _check_norm(qo[live], q[live], qw, 1e-5, cos[at][live], sin[at][live])
+    _check_norm(ko[live], k[live], kw, 1e-5, cos[at][live], sin[at][live])
+    assert (qo[~live] == 7).all() and (ko[~live] == 7).all()
+    assert ops.device_status() == 0
+
+
+def test_norm_rope_position_outside_the_table_is_reported(ops):
+    g = _gen(4)
+    q = _randn(g, 4, 2, 128)
+    cos, sin = _tables(torch.arange(10, device=DEV))
+    for bad in (10, -2, 2 ** 31 - 1):
+        pos = torch.tensor([0, 9, bad, 3], device=DEV, dtype=torch.int32)
+        out = torch.full_like(q, 7.0)
+        ops.qk_norm_rope(q, None, rope=(cos, sin), positions=pos, q_out=out)
+        assert ops.device_status() == ops.STATUS_BAD_LAUNCH
+        assert (out[2] == 7).all()
+        rest = torch.tensor([0, 1, 3], device=DEV)
+        _check_norm(out[rest], q[rest], None, 0, cos[pos[rest].long()], sin[pos[rest].long()])
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("B,T,rope_batch", [(2, 50, 1), (3, 17, 3), (1, 1, 1)])
+def test_norm_rope_per_token_tables_of_a_batch(ops, B, T, rope_batch):
+    """[1|B, T, 128] angles, into views of a head-split cache [B, H, cap, 128]."""
+    g = _gen(B * T)
+    q, k = _randn(g, B, 8, T, 128).transpose(1, 2), _randn(g, B, 2, T, 128).transpose(1, 2)
+    kw = 1 + _randn(g, 128, scale=0.2)
+    cos, sin = _tables(torch.randint(0, 9000, (rope_batch, T), device=DEV, generator=g))
+    cache = torch.full((B, 2, T + 9, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+    qo, _ = ops.qk_norm_rope(q, k, None, kw, 1e-6, rope=(cos, sin), k_out=cache[:, :, 4:4 + T].transpose(1, 2))
+    _check_norm(qo, q, None, 0, cos.expand(B, T, 128), sin.expand(B, T, 128))
+    _check_norm(cache[:, :, 4:4 + T].transpose(1, 2), k, kw, 1e-6, cos.expand(B, T, 128), sin.expand(B, T, 128))
+    assert (cache[:, :, :4] == 7).all() and (cache[:, :, 4 + T:] == 7).all()
+
+
+def test_norm_rope_parts_in_place_and_values(ops):
+    g = _gen(9)
+    T = 70
+    x = _randn(g, T, 12, 128)
+    w = 1 + _randn(g, 128, scale=0.2)
+    cos, sin = _tables(torch.arange(T, device=DEV))
+    only_norm, none = ops.qk_norm_rope(x, None, w, None, 1e-6)
+    assert none is None
+    _check_norm(only_norm, x, w, 1e-6, None, None)
+    only_rope, _ = ops.qk_norm_rope(x, None, rope=(cos, sin))
+    _check_norm(only_rope, x, None, 0, cos, sin)
+    assert torch.equal(ops.qk_norm_rope(x, x[:, :3])[1], x[:, :3])  # neither: a copy
+    y = x.clone()
+    ops.qk_norm_rope(y[:, :8], y[:, 8:], w, w, 1e-6, rope=(cos, sin), q_out=y[:, :8], k_out=y[:, 8:])
+    _check_norm(y, x, w, 1e-6, cos, sin)
+    # all-zero rows, tiny rows (eps matters), one bad row that must stay alone
+    z = x.clone()
+    z[3] = 0
+    z[4] *= 1e-4
+    z[5, 2, 17] = float("nan")
+    z[6, 1, 100] = float("inf")
+    o, _ = ops.qk_norm_rope(z, None, w, None, 1e-6, rope=(cos, sin))
+    bad = torch.zeros(T, 12, dtype=torch.bool, device=DEV)
+    bad[5, 2] = bad[6, 1] = True
+    assert torch.isfinite(o[~bad].float()).all() and not torch.isfinite(o[5, 2].float()).any()
+    keep = torch.ones(T, dtype=torch.bool, device=DEV)
+    keep[5:7] = False
+    _check_norm(o[keep], z[keep], w, 1e-6, cos[keep], sin[keep])
+    e, _ = ops.qk_norm_rope(x[:0], x[:0, :2], w, w)
+    assert e.shape == (0, 12, 128)
+
+
+# -------------------------------------------------------------- attn_varlen --
+@pytest.mark.parametrize("q_lens,Hq,Hkv", [
+    ([1], 1, 1), ([1], 32, 8), ([5, 8, 30, 6, 7], 28, 4), ([64], 2, 2), ([65, 63, 1, 128, 129], 7, 7),
+    ([127, 0, 256, 0, 0, 257, 33], 10, 2), ([511, 513], 8, 1), ([300, 20], 40, 8), ([1100], 28, 4),
+    ([40] * 70, 4, 2), ([200, 90], 80, 1), ([150], 130, 1), ([33, 47], 24, 8)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_varlen_prompts(ops, q_lens, Hq, Hkv, causal):
+    g = _gen(sum(q_lens) + Hq)
+    T = sum(q_lens)
+    x = _randn(g, T, Hq + 2 * Hkv, 128, scale=1.3)
+    q, k, v = x[:, :Hq], x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:]
+    o, lse = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(q_lens), max_k=max(q_lens), causal=causal)
+    assert o.shape == (T, Hq, 128) and lse.shape == (Hq, T)
+    _check_varlen(o, lse, q, k, v, q_lens, q_lens, causal)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("q_lens,k_lens,Hq,Hkv", [
+    ([1, 1, 1, 1], [1, 64, 65, 1000], 32, 8),                # single tokens
+    ([1, 37, 1, 256], [3001, 700, 0, 4096], 28, 4),          # tokens and chunks behind a history, one without keys
+    ([40, 3, 0, 90], [17, 3, 50, 0], 6, 2),                  # more queries than keys: rows that see nothing
+    ([130, 260], [129, 1], 4, 4), ([2], [9000], 8, 1), ([1], [20000], 5, 1), ([7], [130], 16, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_varlen_histories(ops, q_lens, k_lens, Hq, Hkv, causal):
+    g = _gen(sum(k_lens))
+    q, k, v = _randn(g, sum(q_lens), Hq, 128), _randn(g, sum(k_lens), Hkv, 128), _randn(g, sum(k_lens), Hkv, 128)
+    o, lse = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(k_lens), causal=causal)
+    _check_varlen(o, lse, q, k, v, q_lens, k_lens, causal)
+    # a bound on the keys changes no result beyond the order of the sums
+    o2, lse2 = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(k_lens), max_k=max(k_lens), causal=causal)
+    _check_varlen(o2, lse2, q, k, v, q_lens, k_lens, causal)
+    assert ops.device_status() == 0
+
+
+def test_varlen_wrong_bound_on_the_keys_changes_nothing(ops):
+    g = _gen(17)
+    q_lens, k_lens = [1, 30, 1], [5000, 900, 2100]
+    q, k, v = _randn(g, 32, 8, 128), _randn(g, 8000, 2, 128), _randn(g, 8000, 2, 128)
+    for max_k in (0, 1, 100, 10 ** 9):
+        o, lse = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(k_lens), max_k=max_k)
+        _check_varlen(o, lse, q, k, v, q_lens, k_lens, True)
+
+
+def test_varlen_layouts_scale_and_rows_outside(ops):
+    """Head-split strided inputs, output into a padded view, a scale of its own; rows outside every sequence stay."""
+    g = _gen(8)
+    q_lens, k_lens, Hq, Hkv = [50, 1, 77], [90, 200, 77], 12, 4
+    cap_q, cap_k = 140, 400
+    q = _randn(g, Hq, cap_q, 128).transpose(0, 1)
+    kv = _randn(g, 2, Hkv, cap_k, 128)
+    k, v = kv[0].transpose(0, 1), kv[1].transpose(0, 1)
+    cu_q, cu_k = _cu(q_lens) + 3, _cu(k_lens) + 11  # the first sequence does not start at row 0
+    buf = torch.full((cap_q + 2, Hq, 192), 7.0, device=DEV, dtype=torch.bfloat16)
+    out = buf[1:-1, :, 32:160]
+    got, lse = ops.attn_varlen(q, k, v, cu_q, cu_k, scale=0.2, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    n = sum(q_lens)
+    _check_varlen(out[3:3 + n], lse[:, 3:3 + n], q[3:3 + n], k[11:], v[11:], q_lens, k_lens, True, 0.2)
+    left = buf.clone()
+    left[1:-1, :, 32:160][3:3 + n] = 7.0
+    assert (left == 7).all()
+    no, none = ops.attn_varlen(q, k, v, cu_q, cu_k, scale=0.2, want_lse=False)
+    assert none is None and torch.equal(no[3:3 + n], out[3:3 + n])
+
+
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
+def test_varlen_neighbours_have_no_influence(ops, poison):
+    """Bad values in other sequences, behind the last one and in keys a causal row does not see stay where they are."""
+    g = _gen(12)
+    lens, Hq, Hkv = [70, 130, 45, 300], 8, 2
+    T = sum(lens) + 60
+    q, k, v = _randn(g, T, Hq, 128), _randn(g, T, Hkv, 128), _randn(g, T, Hkv, 128)
+    cu = _cu(lens)
+    clean, clean_lse = ops.attn_varlen(q, k, v, cu, cu)
+    clean, clean_lse = clean.clone(), clean_lse.clone()
+    k2, v2, q2 = k.clone(), v.clone(), q.clone()
+    k2[70:200] = v2[70:200] = q2[70:200] = poison   # the second sequence
+    k2[sum(lens):] = v2[sum(lens):] = q2[sum(lens):] = poison
+    o, lse = ops.attn_varlen(q2, k2, v2, cu, cu)
+    rows = [i for i in range(sum(lens)) if not 70 <= i < 200]
+    assert torch.equal(o[rows], clean[rows]) and torch.equal(lse[:, rows], clean_lse[:, rows])
+    # the last keys of the fourth sequence: earlier rows do not see them
+    for first_bad in (540, 470, 373, 300):
+        k3, v3 = k.clone(), v.clone()
+        k3[first_bad:545] = v3[first_bad:545] = poison
+        o, lse = ops.attn_varlen(q, k3, v3, cu, cu)
+        assert torch.equal(o[:first_bad], clean[:first_bad]), first_bad
+        assert torch.equal(lse[:, :first_bad], clean_lse[:, :first_bad])
+        # and the rows that do see a bad value show it
+        assert not torch.isfinite(o[first_bad:545].float()).all(-1).any()
+    assert ops.device_status() == 0
+
+
+def test_varlen_extreme_scores(ops):
+    """Scores far apart: one key takes all the weight, however late it comes; the lowest finite values are values."""
+    g = _gen(13)
+    n = 700
+    q, k, v = _randn(g, 3, 4, 128), _randn(g, n, 2, 128), _randn(g, n, 2, 128)
+    k = k * 0.01
+    for at in (0, 63, 64, 127, 128, 300, 697):
+        k2 = k.clone()
+        k2[at] = q[0, :1].expand(2, 128) * 40
+        o, lse = ops.attn_varlen(q, k2, v, _cu([3]), _cu([n]))
+        _check_varlen(o, lse, q, k2, v, [3], [n], True)
+    big = torch.full_like(k, torch.finfo(torch.bfloat16).min)
+    o, lse = ops.attn_varlen(q.abs() * 1e-38, big, v, _cu([3]), _cu([n]))
+    _check_varlen(o, lse, q.abs() * 1e-38, big, v, [3], [n], True)
+
+
+@pytest.mark.parametrize("cu_q,cu_k", [([0, 10, 5], [0, 10, 20]), ([0, 10, 41], [0, 10, 20]), ([-1, 10, 20], [0, 1, 2]),
+                                       ([0, 10, 20], [0, 30, 20]), ([0, 10, 20], [0, 10, 2 ** 31 - 1])])
+def test_varlen_bad_offsets_are_reported_and_nothing_is_written(ops, cu_q, cu_k):
+    g = _gen(14)
+    q, k = _randn(g, 40, 4, 128), _randn(g, 40, 2, 128)
+    out = torch.full_like(q, 7.0)
+    i32 = lambda x: torch.tensor(x, device=DEV, dtype=torch.int32)  # noqa: E731
+    ops.attn_varlen(q, k, k, i32(cu_q), i32(cu_k), out=out)
+    assert ops.device_status() == ops.STATUS_BAD_LAUNCH
+    assert (out == 7).all()
+    assert ops.device_status() == 0
+
+
+def test_varlen_bad_offsets_late_in_a_long_list(ops):
+    g = _gen(15)
+    n = 100
+    q, k = _randn(g, n, 4, 128), _randn(g, n, 2, 128)
+    cu = torch.arange(n + 1, device=DEV, dtype=torch.int32)
+    bad = cu.clone()
+    bad[90] = 95
+    out = torch.full_like(q, 7.0)
+    ops.attn_varlen(q, k, k, cu, bad, out=out)
+    assert ops.device_status() == ops.STATUS_BAD_LAUNCH
+    assert (out == 7).all()
+
+
+def test_varlen_nothing_to_do(ops):
+    q, k = torch.zeros(4, 2, 128, device=DEV, dtype=torch.bfloat16), torch.zeros(0, 2, 128, device=DEV, dtype=torch.bfloat16)
+    zero = torch.zeros(2, device=DEV, dtype=torch.int32)
+    out = torch.full_like(q, 7.0)
+    ops.attn_varlen(q, k, k, zero[:1], zero[:1], out=out)       # no sequence
+    ops.attn_varlen(q, q, q, zero, zero, out=out)               # one empty sequence
+    assert (out == 7).all()
+    o, lse = ops.attn_varlen(q, k, k, zero + torch.tensor([0, 4], device=DEV, dtype=torch.int32), zero, out=out)
+    assert (o == 0).all() and (lse == -math.inf).all()          # rows without keys
+    assert ops.attn_varlen(q[:0], q, q, zero, zero)[0].shape == (0, 2, 128)
+
+
+# ------------------------------------------------------- attn_decode_shared --
+@pytest.mark.parametrize("B,Hq,Hkv,P,cap", [
+    (1, 1, 1, 1, 1), (1, 32, 8, 100, 3), (4, 28, 4, 1000, 64), (3, 5, 1, 129, 70), (33, 10, 2, 517, 40),
+    (64, 8, 2, 4100, 130), (2, 40, 8, 20000, 600), (5, 130, 1, 300, 20), (17, 16, 16, 64, 1), (300, 4, 4, 65, 5),
+    (7, 14, 2, 0, 300), (7, 14, 2, 300, 0), (9, 23, 1, 2, 1025), (128, 7, 1, 700, 33)])
+def test_shared(ops, B, Hq, Hkv, P, cap):
+    g = _gen(B * 7 + P)
+    q = _randn(g, B, Hq, 128, scale=1.5)
+    kp, vp = _randn(g, Hkv, P, 128), _randn(g, Hkv, P, 128)
+    k, v = _randn(g, B, Hkv, cap, 128), _randn(g, B, Hkv, cap, 128)
+    lens = torch.randint(0, cap + 1, (B,), device=DEV, generator=g, dtype=torch.int32)
+    lens[0] = cap
+    lens[-1] = 0 if P else min(1, cap)
+    o, lse = ops.attn_decode_shared(q, kp, vp, k, v, lens)
+    assert o.shape == (B, 1, Hq, 128) and lse.shape == (B, Hq)
+    _check_shared(o, lse, q, kp, vp, k, v, lens.tolist())
+    assert ops.device_status() == 0
+
+
+def test_shared_without_lens_equals_decode_of_the_whole(ops):
+    g = _gen(31)
+    B, Hq, Hkv, P, cap = 6, 28, 4, 900, 77
+    q = _randn(g, B, Hq, 1, 128)
+    kp, vp = _randn(g, 1, Hkv, P, 128), _randn(g, 1, Hkv, P, 128)
+    k, v = _randn(g, B, Hkv, cap, 128), _randn(g, B, Hkv, cap, 128)
+    o, lse = ops.attn_decode_shared(q, kp, vp, k, v)
+    _check_shared(o, lse, q[:, :, 0], kp[0], vp[0], k, v, [cap] * B)
+    whole, whole_lse = ops.attn_decode(q, torch.cat([kp.expand(B, -1, -1, -1), k], 2),
+                                       torch.cat([vp.expand(B, -1, -1, -1), v], 2))
+    assert (o.float() - whole.float()).abs().max() <= 4 * H_BF16 * whole.float().abs().max()
+    assert (lse - whole_lse).abs().max() <= 1e-4
+
+
+def test_shared_unused_slots_and_lens_out_of_range(ops):
+    g = _gen(32)
+    B, Hq, Hkv, P, cap = 5, 14, 2, 200, 150
+    q = _randn(g, B, Hq, 128)
+    kp, vp = _randn(g, Hkv, P, 128), _randn(g, Hkv, P, 128)
+    k, v = _randn(g, B, Hkv, cap, 128), _randn(g, B, Hkv, cap, 128)
+    want = [0, 1, 64, 99, cap]
+    for b, n in enumerate(want):
+        k[b, :, n:] = float("nan")
+        v[b, :, n:] = float("inf")
+    lens = torch.tensor([-5, 1, 64, 99, 10 ** 6], device=DEV, dtype=torch.int32)
+    o, lse = ops.attn_decode_shared(q, kp, vp, k, v, lens)
+    _check_shared(o, lse, q, kp, vp, k, v, want)
+    # no prefix either: the request without keys gives zeros and -inf
+    o, lse = ops.attn_decode_shared(q, kp[:, :0], vp[:, :0], k, v, lens)
+    assert (o[0] == 0).all() and (lse[0] == -math.inf).all()
+    _check_shared(o[1:], lse[1:], q[1:], kp[:, :0], vp[:, :0], k[1:], v[1:], want[1:])
+    o, lse = ops.attn_decode_shared(q, kp[:, :0], vp[:, :0], k[:, :, :0], v[:, :, :0])
+    assert (o == 0).all() and (lse == -math.inf).all()
+
+
+def test_shared_strided_views_and_out(ops):
+    g = _gen(33)
+    B, Hq, Hkv, P, cap = 9, 12, 4, 333, 50
+    q = _randn(g, Hq, B, 128).transpose(0, 1)
+    pre = _randn(g, P, 2 * Hkv, 128)            # token-major prefix, k and v side by side
+    kp, vp = pre[:, :Hkv].transpose(0, 1), pre[:, Hkv:].transpose(0, 1)
+    big = _randn(g, 2, B, Hkv, 128, 128)
+    k, v = big[0][:, :, 10:10 + cap], big[1][:, :, 10:10 + cap]
+    lens = torch.randint(0, cap + 1, (B,), device=DEV, generator=g, dtype=torch.int32)
+    buf = torch.full((B, 2, Hq, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+    o, lse = ops.attn_decode_shared(q, kp, vp, k, v, lens, scale=0.15, out=buf[:, 1:])
+    _check_shared(buf[:, 1:], lse, q, kp, vp, k, v, lens.tolist(), 0.15)
+    assert (buf[:, 0] == 7).all()
+    o2, none = ops.attn_decode_shared(q, kp, vp, k, v, lens, scale=0.15, want_lse=False)
+    assert none is None and torch.equal(o2, o)
+
+
+# ---------------------------------------------------------------- refusals --
+def test_refusals(ops):
+    bf = lambda *s: torch.zeros(*s, device=DEV, dtype=torch.bfloat16)  # noqa: E731
+    cu = torch.tensor([0, 4], device=DEV, dtype=torch.int32)
+    cos = torch.zeros(4, 128, device=DEV)
+    q, k = bf(4, 4, 128), bf(4, 2, 128)
+    bad = [
+        (ops.qk_norm_rope, (q.half(), k), {}, "bfloat16"),
+        (ops.qk_norm_rope, (bf(4, 4, 64), k), {}, "128"),
+        (ops.qk_norm_rope, (q, bf(5, 2, 128)), {}, "q's shape"),
+        (ops.qk_norm_rope, (q, k, bf(64)), {}, "weights"),
+        (ops.qk_norm_rope, (q, k, bf(128).half()), {}, "weights"),
+        (ops.qk_norm_rope, (q, k), dict(positions=cu), "tables"),
+        (ops.qk_norm_rope, (q, k), dict(rope=(cos, cos), positions=cu), "token shape"),
+        (ops.qk_norm_rope, (q, k), dict(rope=(cos[:3], cos[:3])), "rope"),
+        (ops.qk_norm_rope, (q, k), dict(q_out=bf(4, 5, 128)), "q_out"),
+        (ops.qk_norm_rope, (q, k), dict(k_out=bf(1, 2, 128).expand(4, 2, 128)), "expanded"),
+        (ops.qk_norm_rope, (bf(4, 4, 256)[:, :, ::2], k), {}, "contiguous"),
+        (ops.qk_norm_rope, (bf(4 * 4 * 128 + 4)[4:].view(4, 4, 128), None), {}, "16-byte"),
+        (ops.attn_varlen, (q, k, k, cu.long(), cu.long()), {}, "int32"),
+        (ops.attn_varlen, (q, k, k, cu, torch.cat([cu, cu])), {}, "same sequences"),
+        (ops.attn_varlen, (q, bf(4, 3, 128), bf(4, 3, 128), cu, cu), {}, "multiple"),
+        (ops.attn_varlen, (q, k, bf(4, 4, 128)[:, :2], cu, cu), {}, "strides"),
+        (ops.attn_varlen, (q, k.float(), k.float(), cu, cu), {}, "bfloat16"),
+        (ops.attn_varlen, (q, k, k, cu, cu), dict(max_k=-1), "max_k"),
+        (ops.attn_varlen, (q, k, k, cu, cu), dict(out=bf(4, 4, 64)), "out"),
+        (ops.attn_varlen, (q, k, k, cu, cu), dict(scale=float("nan")), "scale"),
+        (ops.attn_varlen, (q, k, k, cu.cpu(), cu), {}, "CUDA"),
+        (ops.attn_varlen, (bf(1, 4, 4, 128), k, k, cu, cu), {}, "expected"),
+        (ops.attn_decode_shared, (bf(4, 4, 2, 128), bf(2, 9, 128), bf(2, 9, 128), bf(4, 2, 5, 128), bf(4, 2, 5, 128)), {},
+         "one query token"),
+        (ops.attn_decode_shared, (q, bf(2, 9, 128), bf(2, 8, 128), bf(4, 2, 5, 128), bf(4, 2, 5, 128)), {}, "same shape"),
+        (ops.attn_decode_shared, (q, bf(2, 9, 128), bf(2, 9, 128), bf(3, 2, 5, 128), bf(3, 2, 5, 128)), {}, "batch"),
+        (ops.attn_decode_shared, (q, bf(2, 9, 128), bf(2, 9, 128), bf(4, 2, 5, 128), bf(4, 2, 5, 128), cu), {}, "lens"),
+        (ops.attn_decode_shared, (q, bf(3, 9, 128), bf(3, 9, 128), bf(4, 3, 5, 128), bf(4, 3, 5, 128)), {}, "multiple"),
+    ]
+    for fn, args, kw, word in bad:
+        with pytest.raises(RuntimeError, match=word):
+            fn(*args, **kw)
+
+
+# ------------------------------------------------- streams, graphs, together --
+def _calls(ops, g, B=6, Hq=8, Hkv=2):
+    """One call of each operator on inputs of its own, as closures over static buffers."""
+    lens = [3, 100, 40, 1, 260, 17]
+    T = sum(lens)
+    x = _randn(g, T, Hq + 2 * Hkv, 128)
+    w = 1 + _randn(g, 128, scale=0.1)
+    cos, sin = _tables(torch.arange(300, device=DEV))
+    pos = torch.cat([torch.arange(n, device=DEV) for n in lens]).int()
+    cu, cu_k = _cu(lens), _cu([n + 2000 for n in lens])
+    kv = _randn(g, 2, T + 2000 * len(lens), Hkv, 128)
+    kp, k = _randn(g, 2, Hkv, 1500, 128), _randn(g, 2, B, Hkv, 90, 128)
+    n_own = torch.randint(0, 91, (B,), device=DEV, generator=g, dtype=torch.int32)
+    qd = _randn(g, B, Hq, 128)
+
+    def run():
+        a = ops.qk_norm_rope(x[:, :Hq], x[:, Hq:Hq + Hkv], w, w, 1e-6, rope=(cos, sin), positions=pos)
+        b = ops.attn_varlen(a[0], a[1], x[:, Hq + Hkv:].contiguous(), cu, cu, max_k=260)
+        c = ops.attn_varlen(a[0], kv[0], kv[1], cu, cu_k)
+        d = ops.attn_decode_shared(qd, kp[0], kp[1], k[0], k[1], n_own)
+        return [*a, *b, *c, *d]
+
+    return run, (x, kv, kp, k, qd)
+
+
+def test_repeated_calls_give_the_same_bits(ops):
+    run, _ = _calls(ops, _gen(50))
+    first = [t.clone() for t in run()]
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, run()))
+
+
+def test_other_streams(ops):
+    """Two streams at once, each with its own inputs, give what one stream gives."""
+    runs = [_calls(ops, _gen(60 + i))[0] for i in range(2)]
+    want = [[t.clone() for t in r()] for r in runs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in runs]
+    got = [None, None]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = runs[i]()
+    torch.cuda.synchronize()
+    for w, o in zip(want, got):
+        assert all(torch.equal(a, b) for a, b in zip(w, o))
+    assert ops.device_status() == 0
+
+
+def test_captured_graphs_replay_with_new_inputs_and_side_by_side(ops):
+    made = [_calls(ops, _gen(70 + i)) for i in range(2)]
+    graphs, outs = [], []
+    for run, _ in made:
+        run()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            run()
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(run())
+        graphs.append(gr)
+    for step in range(3):
+        for i, (_, bufs) in enumerate(made):
+            g = _gen(100 * step + i)
+            for b in bufs:
+                b.copy_(_randn(g, *b.shape))
+        want = [[t.clone() for t in run()] for run, _ in made]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for s, gr in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                gr.replay()
+                gr.replay()
+        torch.cuda.synchronize()
+        for w, o in zip(want, outs):
+            assert all(torch.equal(a, b) for a, b in zip(w, o))
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (7, 1)])
+def test_a_packed_serving_step(ops, Hq, Hkv):
+    """The three together, as a server uses them: a shared prompt is computed once and kept, three questions follow it
+    as packed sequences, then every request decodes two tokens behind prompt and question. Each token's output has to
+    be the plain causal attention over its whole sequence (roped, normed keys in bf16, as the caches hold them)."""
+    g = _gen(80)
+    P, q_lens, steps = 150, [5, 64, 33], 2
+    B = len(q_lens)
+    cap = max(q_lens) + steps
+    seqs = [_randn(g, P, Hq + 2 * Hkv, 128)]                                  # the prompt's projections
+    tails = [_randn(g, n + steps, Hq + 2 * Hkv, 128) for n in q_lens]         # the requests' own
+    qw, kw = 1 + _randn(g, 128, scale=0.2), 1 + _randn(g, 128, scale=0.2)
+    rope = _tables(torch.arange(P + cap, device=DEV))
+
+    def norm(x, pos):
+        return ops.qk_norm_rope(x[:, :Hq], x[:, Hq:Hq + Hkv], qw, kw, 1e-6, rope=rope, positions=pos)
+
+    # the prompt: its keys and values become the shared prefix
+    pq, pk = norm(seqs[0], torch.arange(P, device=DEV))
+    pv = seqs[0][:, Hq + Hkv:]
+    ops.attn_varlen(pq, pk.contiguous(), pv.contiguous(), _cu([P]), _cu([P]))
+    k_prefix, v_prefix = pk.transpose(0, 1).contiguous(), pv.transpose(0, 1).contiguous()
+    # the questions, packed, each behind the prompt
+    x = torch.cat([t[:n] for t, n in zip(tails, q_lens)])
+    pos = torch.cat([torch.arange(P, P + n, device=DEV) for n in q_lens])
+    q, k = norm(x, pos)
+    v = x[:, Hq + Hkv:]
+    parts_q, parts_k, parts_v = q.split(q_lens), k.split(q_lens), v.split(q_lens)
+    k_all = torch.cat([torch.cat([pk, t]) for t in parts_k])
+    v_all = torch.cat([torch.cat([pv, t]) for t in parts_v])
+    k_lens = [P + n for n in q_lens]
+    o, lse = ops.attn_varlen(q, k_all, v_all, _cu(q_lens), _cu(k_lens), max_k=max(k_lens))
+    _check_varlen(o, lse, q, k_all, v_all, q_lens, k_lens, True)
+    # decode: own caches behind the shared prefix
+    kc = torch.full((B, Hkv, cap, 128), float("nan"), device=DEV, dtype=torch.bfloat16)
+    vc = torch.full_like(kc, float("nan"))
+    for b, n in enumerate(q_lens):
+        kc[b, :, :n], vc[b, :, :n] = parts_k[b].transpose(0, 1), parts_v[b].transpose(0, 1)
+    lens = torch.tensor(q_lens, device=DEV, dtype=torch.int32)
+    for t in range(steps):
+        x1 = torch.stack([s[n + t] for s, n in zip(tails, q_lens)])
+        q1, k1 = norm(x1, P + lens)
+        _check_norm(k1, x1[:, Hq:Hq + Hkv], kw, 1e-6, rope[0][(P + lens).long()], rope[1][(P + lens).long()])
+        at = lens.long()
+        kc[torch.arange(B), :, at], vc[torch.arange(B), :, at] = k1, x1[:, Hq + Hkv:]
+        lens += 1
+        od, ld = ops.attn_decode_shared(q1, k_prefix, v_prefix, kc, vc, lens)
+        _check_shared(od, ld, q1, k_prefix, v_prefix, kc, vc, lens.tolist())
+    assert ops.device_status() == 0
