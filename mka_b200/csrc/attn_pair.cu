@@ -1,0 +1,1036 @@
+// Attention for many rows on tcgen05, by pairs of CTAs: packed sequences of
+// different lengths, and the shared prefix of a decode batch.
+//
+//   o_r = sum_{j <= lim(r)} softmax_j(scale * q_r k_j) v_j,  lse_r = log sum_j exp(scale * q_r k_j)
+//
+// Work is cut into items: a tile of rows ((token, query head of one kv head's
+// group) pairs, 128 per CTA, 256 per pair) against a range of keys. A persistent
+// grid of CTA pairs takes the items in a fixed order, heavy ones first. Items
+// that cover only a part of a row's keys leave a normalised fp32 partial output
+// and a log2-sum-exp, joined by a second kernel.
+//
+// Each pair multiplies with the 2-SM MMA (M = 256, cta_group::2): every CTA
+// holds its own 128 rows of Q, S, P and O and only half of each K tile (64
+// keys) and V tile (64 channels), which halves the operand traffic per SM.
+// TMEM of each CTA (512 columns): O | S0 | S1 | S2. P (bf16) is written over its
+// S and read from there by the second product. With one row tile per CTA and
+// three S buffers, the two softmax warpgroups take the key tiles of the same
+// rows in turn: while one is in its exponentials, the other finds its row
+// maxima, and the next S is already there, so the chain S -> softmax -> P V ->
+// next S of one tile no longer bounds the step.
+//
+// Warp roles (12 warps per CTA):
+//   warp 0      producer: Q, K, V tiles by TMA (128-byte swizzle)
+//   warp 1      MMA issuer (the even CTA's, for both): S runs up to three tiles
+//               ahead of P V, across item borders
+//   warp 2      TMEM allocation
+//   warp 3      V gate: hands each V tile to the MMA; on tiles with masked keys
+//               it first puts zeros over the rows past the last key and over
+//               infinities and NaNs in rows that only some queries see, because
+//               a zero weight times such a value would not be zero
+//   warps 4-7, 8-11  softmax of the even / odd key tiles, thread = row. The
+//               running maximum passes from one warpgroup to the other through
+//               shared memory; it moves only when a row outgrows it by 2^8, and
+//               then O is rescaled in TMEM (exact: the sums use the same
+//               maximum). Each warpgroup keeps its own sum; the one with an
+//               item's last tile joins them and writes the output.
+#include <algorithm>
+#include <utility>
+
+#include "fmka_internal.h"
+#include "ptx.cuh"
+
+namespace fmka {
+
+namespace {
+
+constexpr int kBN = 128;        // keys per tile
+constexpr int kHeadDim = 128;
+constexpr int kThreads = 384;
+constexpr int kSBufs = 3;
+constexpr int kKStages = 5;
+constexpr int kVStages = 5;
+constexpr int kQBytes = 32768;   // 128 rows x 128 channels
+constexpr int kQHalf = 16384;    // 64 channels
+constexpr int kKBytes = 16384;   // 64 keys x 128 channels
+constexpr int kVBytes = 16384;   // 128 keys x 64 channels
+constexpr int kTileSmem = 2 * kQBytes + kKStages * kKBytes + kVStages * kVBytes;
+constexpr int kSmemBytes = kTileSmem + 3072;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+constexpr uint32_t kTmemO = 0, kTmemS = 128;
+// Register split between the control warps and the softmax warps (setmaxnreg);
+// the sum has to fit in what the block is launched with.
+constexpr int kRegsControl = 64;
+constexpr int kRegsSoftmax = 216;
+constexpr int kMinLaunchRegs = (128 * kRegsControl + 256 * kRegsSoftmax + kThreads - 1) / kThreads;
+
+struct PairItem {
+  int q0, nq;      // first row token, tokens (over both CTAs)
+  int k0;          // packed row of the sequence's key 0
+  int kb, ke;      // keys [kb, ke)
+  int lim0;        // last key token 0 sees (token i sees lim0 + i)
+  int hkv, g0, gn;
+  int n;           // key tiles
+  int64_t part;    // first partial row, or -1
+  int part_ts;     // partial rows per token
+};
+
+struct PairParams {
+  __nv_bfloat16* o;
+  int64_t o_st, o_sh;
+  float* lse;
+  int64_t lse_st, lse_sh;
+  const __nv_bfloat16* v;
+  int64_t kv_st, kv_sh;
+  int Hq, G, Gs, n_gs, nh;   // nh = kv heads x group slices
+  int tpt;                   // tokens per CTA
+  float scale_log2;
+  const int* header;         // [0] list entries; null: uniform items
+  const int4* list;          // {q0, nq, k0, kb}, {ke, lim0, part, 0}
+  int B, P, n_rt, n_splits, keys_per_split;  // uniform items
+  float* part_o;
+  float* part_lse;
+  uint32_t* status;
+};
+
+__device__ __forceinline__ int pair_item_count(const PairParams& p) {
+  return (p.header != nullptr ? __ldcg(p.header) : p.n_rt * p.n_splits) * p.nh;
+}
+
+// The items of one pair: a snake over the list, which is sorted by falling work.
+__device__ __forceinline__ int pair_item_index(int r, int pair, int pairs) {
+  return r * pairs + ((r & 1) ? pairs - 1 - pair : pair);
+}
+
+__device__ __forceinline__ void load_item(const PairParams& p, int idx, PairItem& it) {
+  const int li = idx / p.nh, h = idx - li * p.nh;
+  it.hkv = h / p.n_gs;
+  it.g0 = (h - it.hkv * p.n_gs) * p.Gs;
+  it.gn = min(p.Gs, p.G - it.g0);
+  if (p.header != nullptr) {
+    const int4 a = __ldcg(p.list + 2 * li), b = __ldcg(p.list + 2 * li + 1);
+    it.q0 = a.x;
+    it.nq = a.y;
+    it.k0 = a.z;
+    it.kb = a.w;
+    it.ke = b.x;
+    it.lim0 = b.y;
+    it.part = b.z < 0 ? -1 : (int64_t)b.z + (int64_t)h * a.y * p.Gs;
+    it.part_ts = p.Gs;
+  } else {
+    const int split = li / p.n_rt, rt = li - split * p.n_rt;
+    it.q0 = rt * 2 * p.tpt;
+    it.nq = min(2 * p.tpt, p.B - it.q0);
+    it.k0 = 0;
+    it.kb = split * p.keys_per_split;
+    it.ke = min(p.P, it.kb + p.keys_per_split);
+    it.lim0 = p.P;
+    it.part = ((int64_t)split * p.B + it.q0) * p.Hq + it.hkv * p.G + it.g0;
+    it.part_ts = p.Hq;
+  }
+  it.n = it.ke > it.kb ? (it.ke - it.kb + kBN - 1) / kBN : 0;
+}
+
+// A walk over the key tiles of a pair's items.
+struct Cursor {
+  int r = -1, j = 0, items = 0;
+  bool end = false;
+  PairItem it;
+  __device__ __forceinline__ void next_item(const PairParams& p, int n_items, int pair, int pairs) {
+    do {
+      const int idx = pair_item_index(++r, pair, pairs);
+      // the snake's odd rounds run backwards: the last round can be short at either end
+      if (r * pairs >= n_items) {
+        end = true;
+        return;
+      }
+      it.n = 0;
+      if (idx < n_items) load_item(p, idx, it);
+    } while (it.n == 0);
+    j = 0;
+  }
+  __device__ __forceinline__ void step(const PairParams& p, int n_items, int pair, int pairs) {
+    if (++j == it.n) {
+      ++items;
+      next_item(p, n_items, pair, pairs);
+    }
+  }
+};
+
+__device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    attn_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PairParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + 2 * kQBytes;
+  uint8_t* sV = sK + kKStages * kKBytes;
+  float* s_m = reinterpret_cast<float*>(sV + kVStages * kVBytes);  // [2][128] running maximum after even / odd tiles
+  float* s_l = s_m + 256;                                           // [2][128] sums handed on at an item's end
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + 256);
+  uint64_t* q_full = bars;                 // [2] even CTA
+  uint64_t* q_empty = q_full + 2;          // [2] both
+  uint64_t* k_full = q_empty + 2;          // [kKStages] even CTA
+  uint64_t* k_empty = k_full + kKStages;   // [kKStages] both
+  uint64_t* v_land = k_empty + kKStages;   // [kVStages] own loads have landed
+  uint64_t* v_ready = v_land + kVStages;   // [kVStages] even CTA: both gates passed
+  uint64_t* v_empty = v_ready + kVStages;  // [kVStages] both
+  uint64_t* s_full = v_empty + kVStages;   // [kSBufs] both
+  uint64_t* p_full = s_full + kSBufs;      // [kSBufs] even CTA, 8 warps
+  uint64_t* pv_done = p_full + kSBufs;     // [kSBufs] both
+  uint64_t* o_free = pv_done + kSBufs;     // even CTA, 8 warps
+  uint64_t* m_bar = o_free + 1;            // [2][4] maximum handed on, per quarter
+  uint64_t* l_bar = m_bar + 8;             // [2][2][4] sum handed on: warpgroup, its count's parity, quarter
+  uint64_t* mma_done = l_bar + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* bad_v = abort_flag + 1;    // [8] by item number: 1 + the last item with taken-out values
+  static_assert(1024 * 2 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 3 * kSBufs + 1 + 24 + 1) + 40 <= 3072,
+                "control block fits behind the tiles");
+
+  const int warp = warp_id();
+  const int lane = lane_id();
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1;
+  const int pairs = gridDim.x >> 1;
+  if (smem_u32(smem) & 1023u) {  // the swizzled tiles need it; the same in every CTA
+    if (threadIdx.x == 0) atomicOr(p.status, kStatusBadLaunch);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < kKStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < kVStages; ++i) {
+      mbar_init(&v_land[i], 1);
+      mbar_init(&v_ready[i], 2);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < kSBufs; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(o_free, 8);
+    for (int i = 0; i < 8; ++i) mbar_init(&m_bar[i], 1);
+    for (int i = 0; i < 16; ++i) mbar_init(&l_bar[i], 1);
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    for (int i = 0; i < 8; ++i) bad_v[i] = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 2) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();  // the item list (or the previous kernel's outputs) is complete
+  grid_launch_dependents();
+  const int n_items = pair_item_count(p);
+
+  if (warp == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    // ------------------------------------------------------------ producer --
+    if (lane == 0) {
+      const uint32_t q_full_even = cluster_addr(&q_full[0], 0);
+      const uint32_t k_full_even = cluster_addr(&k_full[0], 0);
+      const int q_box = p.Gs * p.tpt * 128;  // bytes of one 64-channel box
+      Cursor kc, vc;
+      kc.next_item(p, n_items, pair, pairs);
+      vc = kc;
+      int gk = 0, gv = 0;
+      bool ok = true;
+      while (ok && !vc.end) {
+        while (!kc.end && gk - gv < kSBufs) {
+          if (kc.j == 0) {
+            const int qs = kc.items & 1;
+            if (!(ok = mbar_wait(&q_empty[qs], ((kc.items >> 1) & 1) ^ 1u, p.status))) break;
+            if (rank == 0) mbar_arrive_expect_tx(&q_full[qs], 4 * q_box);
+            const int tok = kc.it.q0 + (int)rank * p.tpt;
+            const int head = kc.it.hkv * p.G + kc.it.g0;
+            tma_load_3d_pair(sQ + qs * kQBytes, &tmQ, q_full_even + qs * 8, 0, head, tok);
+            tma_load_3d_pair(sQ + qs * kQBytes + kQHalf, &tmQ, q_full_even + qs * 8, 64, head, tok);
+          }
+          const int ks = gk % kKStages;
+          if (!(ok = mbar_wait(&k_empty[ks], ((gk / kKStages) & 1) ^ 1u, p.status))) break;
+          if (rank == 0) mbar_arrive_expect_tx(&k_full[ks], 2 * kKBytes);
+          const int key = kc.it.k0 + kc.it.kb + kc.j * kBN + (int)rank * 64;
+          tma_load_3d_pair(sK + ks * kKBytes, &tmK, k_full_even + ks * 8, 0, key, kc.it.hkv);
+          tma_load_3d_pair(sK + ks * kKBytes + kKBytes / 2, &tmK, k_full_even + ks * 8, 64, key, kc.it.hkv);
+          ++gk;
+          kc.step(p, n_items, pair, pairs);
+        }
+        if (!ok) break;
+        const int vs = gv % kVStages;
+        if (!(ok = mbar_wait(&v_empty[vs], ((gv / kVStages) & 1) ^ 1u, p.status))) break;
+        mbar_arrive_expect_tx(&v_land[vs], kVBytes);
+        tma_load_3d(sV + vs * kVBytes, &tmV, &v_land[vs], 64 * (int)rank, vc.it.k0 + vc.it.kb + vc.j * kBN, vc.it.hkv);
+        ++gv;
+        vc.step(p, n_items, pair, pairs);
+        if (*abort_flag) ok = false;
+      }
+      if (!ok) *abort_flag = 1;
+      // Drain: every load has landed, and its tile has been consumed, before the CTA goes.
+      for (int g = gv - 1; g >= 0 && g >= gv - kVStages; --g)
+        mbar_wait(&v_land[g % kVStages], (g / kVStages) & 1, p.status);
+      for (int g = gk - 1; g >= 0 && g >= gk - kKStages; --g)
+        mbar_wait(&k_empty[g % kKStages], (g / kKStages) & 1, p.status);
+    }
+  } else if (warp == 1) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    // ------------------------------------------- MMA (the even CTA issues) --
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t id_s = make_idesc_bf16(256, kBN, false, false);
+      constexpr uint32_t id_pv = make_idesc_bf16(256, kHeadDim, false, true);
+      Cursor sc, vc;
+      sc.next_item(p, n_items, pair, pairs);
+      vc = sc;
+      int gs = 0, gv = 0;
+      bool ok = true;
+      while (ok && !vc.end) {
+        while (!sc.end && gs - gv < kSBufs) {
+          const int qs = sc.items & 1;
+          if (sc.j == 0 && !(ok = mbar_wait(&q_full[qs], (sc.items >> 1) & 1, p.status))) break;
+          const int ks = gs % kKStages;
+          if (!(ok = mbar_wait(&k_full[ks], (gs / kKStages) & 1, p.status))) break;
+          tc_fence_after();
+          const uint32_t q_addr = smem_u32(sQ + qs * kQBytes);
+          const uint32_t k_addr = smem_u32(sK + ks * kKBytes);
+          const int sb = gs % kSBufs;
+          const uint32_t d = tmem + kTmemS + sb * 128;
+#pragma unroll
+          for (int k = 0; k < kHeadDim / 16; ++k)
+            umma_ss_pair(d, desc_kmajor_sw128(q_addr + (k >> 2) * kQHalf + (k & 3) * 32),
+                         desc_kmajor_sw128(k_addr + (k >> 2) * (kKBytes / 2) + (k & 3) * 32), id_s, k > 0 ? 1u : 0u);
+          tc_commit_pair(&s_full[sb], 0x3);
+          tc_commit_pair(&k_empty[ks], 0x3);
+          if (sc.j == sc.it.n - 1) tc_commit_pair(&q_empty[qs], 0x3);
+          ++gs;
+          sc.step(p, n_items, pair, pairs);
+        }
+        if (!ok) break;
+        const int vs = gv % kVStages, sb = gv % kSBufs;
+        if (vc.j == 0 && vc.items > 0 && !(ok = mbar_wait_cluster(o_free, (vc.items - 1) & 1, p.status))) break;
+        if (!(ok = mbar_wait_cluster(&v_ready[vs], (gv / kVStages) & 1, p.status))) break;
+        if (!(ok = mbar_wait_cluster(&p_full[sb], (gv / kSBufs) & 1, p.status))) break;
+        tc_fence_after();
+        const uint32_t v_addr = smem_u32(sV + vs * kVBytes);
+#pragma unroll
+        for (int k = 0; k < kBN / 16; ++k)
+          umma_ts_pair(tmem + kTmemO, tmem + kTmemS + sb * 128 + k * 8,
+                       desc_mnmajor_sw128(v_addr + k * 2048, kVBytes), id_pv, (vc.j > 0 || k > 0) ? 1u : 0u);
+        tc_commit_pair(&pv_done[sb], 0x3);
+        tc_commit_pair(&v_empty[vs], 0x3);
+        ++gv;
+        vc.step(p, n_items, pair, pairs);
+        if (*abort_flag) ok = false;
+      }
+      if (!ok) *abort_flag = 1;
+      tc_commit_pair(mma_done, 0x1);
+      mbar_wait(mma_done, 0, p.status);
+    }
+  } else if (warp == 3) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    // -------------------------------------------------------------- V gate --
+    const uint32_t ready_even = cluster_addr(&v_ready[0], 0);
+    const uint32_t bad_peer = cluster_addr(const_cast<int*>(bad_v), rank ^ 1u);
+    Cursor c;
+    c.next_item(p, n_items, pair, pairs);
+    int g = 0;
+    while (!c.end) {
+      const int vs = g % kVStages;
+      if (!__all_sync(0xffffffffu, mbar_wait(&v_land[vs], (g / kVStages) & 1, p.status))) {
+        *abort_flag = 1;
+        break;
+      }
+      const int kt = c.it.kb + c.j * kBN;
+      const int live = min(kBN, c.it.ke - kt);                                        // rows that hold keys
+      const int some = c.it.nq > 1 ? min(live, max(0, c.it.lim0 + 1 - kt)) : live;    // rows that every query sees
+      if (some < kBN) {
+        // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes four rows at a time
+        bool bad = false;
+        for (int row = some + (lane >> 3); row < kBN; row += 4) {
+          uint4* at = reinterpret_cast<uint4*>(sV + vs * kVBytes + row * 128 + (lane & 7) * 16);
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (row < live) {
+            x = *at;
+            if (!zero_nonfinite(x)) continue;
+            bad = true;
+          }
+          *at = x;
+        }
+        if (__any_sync(0xffffffffu, bad) && lane == 0) {
+          // the gate is at most five tiles ahead of the products, so eight slots never meet
+          bad_v[c.items & 7] = c.items + 1;
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(bad_peer + 4 * (c.items & 7)), "r"(c.items + 1)
+                       : "memory");
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(ready_even + vs * 8);
+      ++g;
+      c.step(p, n_items, pair, pairs);
+    }
+  } else if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    // ------------------------------------------------------------- softmax --
+    const int wg = (warp - 4) >> 2;
+    const int quarter = warp & 3;  // the TMEM lanes this warp may touch
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t p_full_even = cluster_addr(&p_full[0], 0);
+    const uint32_t o_free_even = cluster_addr(o_free, 0);
+    const int ri = r / p.Gs, rg = r - ri * p.Gs;  // token of the CTA's tile, head of the slice
+    const int ti = (int)rank * p.tpt + ri;         // token of the pair's tile
+    int g0 = 0;                                    // tiles before this item
+    int items = 0;                                 // items with tiles before this one
+    int gave = 0, took = 0;                        // sums handed to / by the other warpgroup so far
+    bool ok = true;
+    PairItem it;
+    for (int rr = 0; ok && rr * pairs < n_items; ++rr) {
+      const int idx = pair_item_index(rr, pair, pairs);
+      if (idx >= n_items) continue;
+      load_item(p, idx, it);
+      const bool row_ok = ri < p.tpt && ti < it.nq && rg < it.gn;
+      const int n = it.n;
+      if (n == 0) {
+        // no row of the tile sees a key
+        if (wg == 0 && row_ok) {
+          uint4* dst = reinterpret_cast<uint4*>(p.o + (it.q0 + ti) * p.o_st + (it.hkv * p.G + it.g0 + rg) * p.o_sh);
+          for (int c = 0; c < 16; ++c) dst[c] = make_uint4(0, 0, 0, 0);
+          if (p.lse != nullptr)
+            p.lse[(it.q0 + ti) * p.lse_st + (it.hkv * p.G + it.g0 + rg) * p.lse_sh] = -INFINITY;
+        }
+        continue;
+      }
+      const int lim = row_ok ? min(it.ke - 1, it.lim0 + ti) : -1;  // last visible key
+      const int last_wg = (g0 + n - 1) & 1;
+      float m_own = -INFINITY, m_prev = -INFINITY, l = 0.f;
+      for (int j = (g0 & 1) == wg ? 0 : 1; j < n; j += 2) {
+        const int g = g0 + j;
+        const int sb = g % kSBufs;
+        const uint32_t s_col = kTmemS + sb * 128;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[sb], (g / kSBufs) & 1, p.status))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const int kbase = it.kb + j * kBN;
+        uint32_t s[128];
+        tmem_ld32(lane_addr + s_col + 0, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        tmem_ld32(lane_addr + s_col + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+        tmem_ld32(lane_addr + s_col + 64, *reinterpret_cast<uint32_t(*)[32]>(&s[64]));
+        tmem_ld32(lane_addr + s_col + 96, *reinterpret_cast<uint32_t(*)[32]>(&s[96]));
+        tmem_wait_ld();
+        if (kbase + kBN - 1 > lim) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (kbase + c > lim) s[c] = 0xFF800000u;  // -inf
+        }
+        float mxa[8];
+#pragma unroll
+        for (int a = 0; a < 8; ++a) mxa[a] = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 128; c += 16) {
+#pragma unroll
+          for (int a = 0; a < 8; ++a) mxa[a] = fmax3(mxa[a], __uint_as_float(s[c + a]), __uint_as_float(s[c + 8 + a]));
+        }
+        const float mx = p.scale_log2 * fmax3(fmax3(mxa[0], mxa[1], mxa[2]), fmax3(mxa[3], mxa[4], mxa[5]),
+                                              fmaxf(mxa[6], mxa[7]));
+        // the maximum after the tile before (the other warpgroup's, same rows)
+        if (g > 0 && !__all_sync(0xffffffffu, mbar_wait(&m_bar[((g - 1) & 1) * 4 + quarter], ((g - 1) >> 1) & 1,
+                                                         p.status))) {
+          ok = false;
+          break;
+        }
+        float m_ref = j > 0 ? s_m[((g - 1) & 1) * 128 + r] : -INFINITY;
+        m_prev = m_ref;
+        float alpha = 1.f;
+        const bool grow = __any_sync(0xffffffffu, mx > m_ref + kRescaleThreshold);
+        if (grow) {
+          const float m_new = fmaxf(m_ref, mx);
+          alpha = m_new == m_ref ? 1.f : fast_exp2(m_ref - m_new);
+          m_ref = m_new;
+        }
+        s_m[(g & 1) * 128 + r] = m_ref;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m_bar[(g & 1) * 4 + quarter]);
+        if (grow && j > 0) {
+          // O holds the tiles before this one: wait for the last product, then move O to the new maximum. (One
+          // barrier per S buffer: S(g) is there, so the product of tile g - 3 is complete and no phase is skipped.)
+          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[(g - 1) % kSBufs], ((g - 1) / kSBufs) & 1, p.status))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c4 = 0; c4 < 8; ++c4) {
+            uint32_t o[16];
+            tmem_ld16(lane_addr + kTmemO + c4 * 16, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+            tmem_st16(lane_addr + kTmemO + c4 * 16, o);
+          }
+        }
+        l *= m_own == m_ref ? 1.f : fast_exp2(m_own - m_ref);
+        m_own = m_ref;
+        const float msub = m_ref == -INFINITY ? 0.f : m_ref;
+        const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+        const float2 nm2 = make_float2(-msub, -msub);
+        float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          const uint32_t* sc = s + 32 * ch;
+          uint32_t pk[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float2 xx =
+                ffma2(make_float2(__uint_as_float(sc[2 * c]), __uint_as_float(sc[2 * c + 1])), sl2, nm2);
+            const float2 pp = exp2_pair(xx);
+            acc[c & 3] = fadd2(acc[c & 3], pp);
+            pk[c] = pack_bf16x2(pp.x, pp.y);
+          }
+          tmem_st16(lane_addr + s_col + 16 * ch, pk);
+        }
+        const float2 asum = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
+        l += asum.x + asum.y;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(p_full_even + sb * 8);
+      }
+      if (!ok) break;
+      if (wg != last_wg) {
+        if (n >= 2) {
+          // the sum so far, at this warpgroup's maximum, for the warpgroup that ends the item
+          // Two slots and barriers: the next item's sum can be ready before this one is read, the one after cannot,
+          // because its tiles wait for a maximum that the reader passes on after reading.
+          s_l[(gave & 1) * 128 + r] = l;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&l_bar[(wg * 2 + (gave & 1)) * 4 + quarter]);
+          ++gave;
+        }
+      } else {
+        // ---- epilogue: O of all tiles, both sums ----
+        const int gl = g0 + n - 1;
+        bool e_ok = true;
+        float l_other = 0.f;  // at m_prev, the maximum after the tile before the last
+        if (n >= 2) {
+          e_ok = mbar_wait(&l_bar[((wg ^ 1) * 2 + (took & 1)) * 4 + quarter], (took >> 1) & 1, p.status);
+          l_other = s_l[(took & 1) * 128 + r];
+          ++took;
+        }
+        if (!__all_sync(0xffffffffu, e_ok && mbar_wait(&pv_done[gl % kSBufs], (gl / kSBufs) & 1, p.status))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const bool bad = bad_v[items & 7] == items + 1;
+        uint32_t o[128];
+        tmem_ld32(lane_addr + kTmemO + 0, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+        tmem_ld32(lane_addr + kTmemO + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+        tmem_ld32(lane_addr + kTmemO + 64, *reinterpret_cast<uint32_t(*)[32]>(&o[64]));
+        tmem_ld32(lane_addr + kTmemO + 96, *reinterpret_cast<uint32_t(*)[32]>(&o[96]));
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(o_free_even);
+        const float L = l + l_other * (m_prev == m_own ? 1.f : fast_exp2(m_prev - m_own));
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float lse2 = L == 0.f ? -INFINITY : m_own + __log2f(L);
+        if (row_ok) {
+          const int tok = it.q0 + ti, head = it.hkv * p.G + it.g0 + rg;
+          const int j0 = max(it.kb, it.lim0 + 1);  // keys before this one are seen by every row
+          const __nv_bfloat16* vrow = p.v + (int64_t)it.k0 * p.kv_st + it.hkv * p.kv_sh;
+          if (it.part < 0) {
+            __nv_bfloat16* dst = p.o + tok * p.o_st + head * p.o_sh;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              uint4 w;
+              w.x = pack_bf16x2(__uint_as_float(o[c * 8 + 0]) * inv, __uint_as_float(o[c * 8 + 1]) * inv);
+              w.y = pack_bf16x2(__uint_as_float(o[c * 8 + 2]) * inv, __uint_as_float(o[c * 8 + 3]) * inv);
+              w.z = pack_bf16x2(__uint_as_float(o[c * 8 + 4]) * inv, __uint_as_float(o[c * 8 + 5]) * inv);
+              w.w = pack_bf16x2(__uint_as_float(o[c * 8 + 6]) * inv, __uint_as_float(o[c * 8 + 7]) * inv);
+              reinterpret_cast<uint4*>(dst)[c] = w;
+            }
+            if (p.lse != nullptr) p.lse[tok * p.lse_st + head * p.lse_sh] = lse2 * 0.69314718055994531f;
+            if (bad) {
+              // rare: values that the V gate took out go to the rows that see them
+              for (int key = j0; key <= lim; ++key)
+                for (int d = 0; d < kHeadDim; ++d) {
+                  const float x = __bfloat162float(vrow[key * p.kv_st + d]);
+                  if (!(fabsf(x) <= 3.4e38f)) dst[d] = __float2bfloat16(__bfloat162float(dst[d]) + x);
+                }
+            }
+          } else {
+            const int64_t rec = it.part + (int64_t)ti * it.part_ts + rg;
+            if (L != 0.f) {
+              float* dst = p.part_o + rec * kHeadDim;
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                reinterpret_cast<float4*>(dst)[c] =
+                    make_float4(__uint_as_float(o[c * 4]) * inv, __uint_as_float(o[c * 4 + 1]) * inv,
+                                __uint_as_float(o[c * 4 + 2]) * inv, __uint_as_float(o[c * 4 + 3]) * inv);
+              if (bad) {
+                for (int key = j0; key <= lim; ++key)
+                  for (int d = 0; d < kHeadDim; ++d) {
+                    const float x = __bfloat162float(vrow[key * p.kv_st + d]);
+                    if (!(fabsf(x) <= 3.4e38f)) dst[d] += x;
+                  }
+              }
+            }
+            p.part_lse[rec] = lse2;
+          }
+        }
+      }
+      g0 += n;
+      ++items;
+    }
+    if (!ok) *abort_flag = 1;
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));  // warp 2
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // nothing aimed at either CTA is still under way
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------- plan --
+// (List, header and parts are read past L1: the reading kernels start before their writers end.)
+// One CTA turns the sequences' offsets into the item list: row tiles of 2 * tpt
+// tokens, each against the keys its rows see, sorted by falling work (a counting
+// sort over kBins classes of tile counts), so that the snake of the main kernel
+// gives every pair about the same. A tile with more work than a pair's fair
+// share is cut along its keys into parts that are joined afterwards.
+constexpr int kPlanThreads = 512;
+constexpr int kBins = 512;
+constexpr int kMinPartTiles = 4;  // a part is worth its partial output from 512 keys on
+
+struct PlanParams {
+  const int* cu_q;
+  const int* cu_k;
+  int n_seqs, total_q, total_k, causal;
+  int tok_tile;    // tokens per item
+  int nh, Gs, pairs;
+  int split;       // parts are allowed
+  int max_parts;   // list entries set aside for parts
+  int* header;     // [0] list entries, [1] groups of parts
+  int* seq_tiles;  // [n_seqs + 1] tiles before each sequence
+  int4* list;
+  int4* groups;    // {q0, nq, parts, first partial row}
+  uint32_t* status;
+};
+
+struct TileOf {
+  int q0, nq, k0, ke, lim0, tiles;
+};
+
+__device__ __forceinline__ TileOf tile_of(const PlanParams& p, int f) {
+  int lo = 0, hi = p.n_seqs - 1;  // the last sequence whose first tile is at or before f
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (p.seq_tiles[mid] <= f) lo = mid;
+    else hi = mid - 1;
+  }
+  const int q0 = p.cu_q[lo], lq = p.cu_q[lo + 1] - q0;
+  const int k0 = p.cu_k[lo], lk = p.cu_k[lo + 1] - k0;
+  const int t0 = (f - p.seq_tiles[lo]) * p.tok_tile;
+  TileOf t;
+  t.q0 = q0 + t0;
+  t.nq = min(p.tok_tile, lq - t0);
+  t.k0 = k0;
+  t.lim0 = p.causal ? t0 + lk - lq : lk;
+  t.ke = p.causal ? max(0, min(lk, t.lim0 + t.nq)) : lk;
+  t.tiles = (t.ke + kBN - 1) / kBN;
+  return t;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const __grid_constant__ PlanParams p) {
+  __shared__ int s_warp[kPlanThreads / 32];
+  __shared__ int s_hist[kBins];
+  __shared__ unsigned long long s_total;
+  __shared__ int s_groups, s_rows, s_max;
+  const int tid = threadIdx.x, lane = lane_id(), warp = warp_id();
+  grid_launch_dependents();
+  for (int i = tid; i < kBins; i += kPlanThreads) s_hist[i] = 0;
+  if (tid == 0) {
+    s_total = 0;
+    s_groups = s_rows = s_max = 0;
+  }
+  // tiles before each sequence
+  int base = 0;
+  bool bad = false;
+  for (int s0 = 0; s0 < p.n_seqs; s0 += kPlanThreads) {
+    const int s = s0 + tid;
+    int nt = 0;
+    if (s < p.n_seqs) {
+      const int q0 = p.cu_q[s], q1 = p.cu_q[s + 1], k0 = p.cu_k[s], k1 = p.cu_k[s + 1];
+      bad |= q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k;
+      nt = bad ? 0 : (q1 - q0 + p.tok_tile - 1) / p.tok_tile;
+    }
+    int incl = nt;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += x;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      before += w < warp ? s_warp[w] : 0;
+      all += s_warp[w];
+    }
+    if (s < p.n_seqs) p.seq_tiles[s] = base + before + incl - nt;
+    base += all;
+    __syncthreads();
+  }
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) {
+      atomicOr(p.status, kStatusBadLaunch);
+      p.header[0] = p.header[1] = 0;
+    }
+    return;
+  }
+  const int n_tiles = base;
+  // all work, and the largest tile
+  unsigned long long sum = 0;
+  int most = 1;
+  for (int f = tid; f < n_tiles; f += kPlanThreads) {
+    const int c = tile_of(p, f).tiles;
+    sum += c;
+    most = max(most, c);
+  }
+  atomicAdd(&s_total, sum);
+  atomicMax(&s_max, most);
+  __syncthreads();
+  const unsigned long long work = s_total * p.nh;
+  const int share = (int)max((unsigned long long)kMinPartTiles, (work + p.pairs - 1) / p.pairs);
+  auto parts_of = [&](int tiles) { return p.split && tiles > share ? (tiles + share - 1) / share : 1; };
+  const int top = min(s_max, p.split ? max(share, 1) : s_max);
+  auto bin_of = [&](int tiles) {
+    return kBins - 1 - (int)min((long long)kBins - 1, (long long)tiles * kBins / (top + 1));
+  };
+  for (int f = tid; f < n_tiles; f += kPlanThreads) {
+    const int c = tile_of(p, f).tiles, np = parts_of(c);
+    atomicAdd(&s_hist[bin_of((c + np - 1) / np)], np);
+  }
+  __syncthreads();
+  // exclusive sums over the bins, heavy bins first
+  {
+    static_assert(kBins == kPlanThreads, "one bin per thread");
+    const int n = s_hist[tid];
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += x;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      before += w < warp ? s_warp[w] : 0;
+      all += s_warp[w];
+    }
+    s_hist[tid] = before + incl - n;
+    if (tid == 0) p.header[0] = all;
+  }
+  __syncthreads();
+  for (int f = tid; f < n_tiles; f += kPlanThreads) {
+    const TileOf t = tile_of(p, f);
+    const int np = parts_of(t.tiles);
+    const int per = (t.tiles + np - 1) / np;
+    const int at = atomicAdd(&s_hist[bin_of(per)], np);
+    int row0 = -1;
+    if (np > 1) {
+      const int rows = t.nq * p.Gs * p.nh;
+      row0 = atomicAdd(&s_rows, np * rows);
+      p.groups[atomicAdd(&s_groups, 1)] = make_int4(t.q0, t.nq, np, row0);
+      for (int i = 0; i < np; ++i) {
+        p.list[2 * (at + i)] = make_int4(t.q0, t.nq, t.k0, i * per * kBN);
+        p.list[2 * (at + i) + 1] = make_int4(min(t.ke, (i + 1) * per * kBN), t.lim0, row0 + i * rows, 0);
+      }
+    } else {
+      p.list[2 * at] = make_int4(t.q0, t.nq, t.k0, 0);
+      p.list[2 * at + 1] = make_int4(t.ke, t.lim0, -1, 0);
+    }
+  }
+  __syncthreads();
+  if (tid == 0) p.header[1] = s_groups;
+}
+
+// Joins the parts of the rows whose keys were cut: a block per group of parts (x) and slice of its rows (y), a warp
+// per row.
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ PairParams p, const int* header,
+                                                        const int4* groups) {
+  grid_dependency_wait();
+  if ((int)blockIdx.x >= __ldcg(header + 1)) return;
+  const int4 gr = __ldcg(groups + blockIdx.x);
+  const int lane = lane_id();
+  const int item_rows = gr.y * p.Gs, rows = item_rows * p.nh;
+  for (int row = blockIdx.y * 8 + warp_id(); row < rows; row += gridDim.y * 8) {
+    const int h = row / item_rows, ti = (row - h * item_rows) / p.Gs, g = row % p.Gs;
+    const int hkv = h / p.n_gs, hg = (h - hkv * p.n_gs) * p.Gs + g;
+    if (hg >= p.G) continue;
+    float M = -INFINITY;
+    for (int s = 0; s < gr.z; ++s) M = fmaxf(M, __ldcg(p.part_lse + gr.w + (int64_t)s * rows + row));
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < gr.z; ++s) {
+      const int64_t rec = (int64_t)gr.w + (int64_t)s * rows + row;
+      const float x = __ldcg(p.part_lse + rec);
+      if (x == -INFINITY) continue;  // this part saw no key of the row: nothing was written
+      const float w = fast_exp2(x - Ms);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + rec * kHeadDim) + lane);
+      L += w;
+      acc.x += w * v.x;
+      acc.y += w * v.y;
+      acc.z += w * v.z;
+      acc.w += w * v.w;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int64_t tok = gr.x + ti;
+    const int head = hkv * p.G + hg;
+    reinterpret_cast<uint2*>(p.o + tok * p.o_st + head * p.o_sh)[lane] =
+        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[tok * p.lse_st + head * p.lse_sh] = L == 0.f ? -INFINITY : (Ms + __log2f(L)) * 0.69314718055994531f;
+  }
+}
+
+template <class... Params, class... Args>
+cudaError_t launch_after(void (*kern)(Params...), dim3 grid, int threads, size_t smem, bool dependent,
+                         cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// Tensor map over [rows][heads][128] with a box of box_h heads x box_r rows x 64 channels. The stride of a dimension
+// of one element says nothing.
+int rows_map(CUtensorMap* out, const __nv_bfloat16* base, int64_t rows, int64_t st, int heads, int64_t sh, int box_h,
+             int box_r, bool head_inner) {
+  if (rows == 1 || st == 0) st = 128;
+  if (heads == 1 || sh == 0) sh = 128;
+  if (head_inner) {
+    const uint64_t dims[3] = {128, (uint64_t)heads, (uint64_t)rows};
+    const uint64_t strides[2] = {(uint64_t)sh * 2, (uint64_t)st * 2};
+    const uint32_t box[3] = {64, (uint32_t)box_h, (uint32_t)box_r};
+    return make_tmap_bf16(out, base, 3, dims, strides, box, true);
+  }
+  const uint64_t dims[3] = {128, (uint64_t)rows, (uint64_t)heads};
+  const uint64_t strides[2] = {(uint64_t)st * 2, (uint64_t)sh * 2};
+  const uint32_t box[3] = {64, (uint32_t)box_r, 1};
+  return make_tmap_bf16(out, base, 3, dims, strides, box, true);
+}
+
+void pair_tile(PairParams& p) {
+  p.n_gs = (p.G + 127) / 128;
+  p.Gs = (p.G + p.n_gs - 1) / p.n_gs;
+  p.tpt = 128 / p.Gs;
+  p.nh = (p.Hq / p.G) * p.n_gs;
+}
+
+int launch_pair(const PairParams& p, const __nv_bfloat16* q, int64_t q_rows, int64_t q_st, int64_t q_sh,
+                const __nv_bfloat16* k, const __nv_bfloat16* v, int64_t kv_rows, int64_t kv_st, int64_t kv_sh,
+                int pairs, bool dependent, cudaStream_t stream, const char* what) {
+  CUtensorMap tmQ, tmK, tmV;
+  int rc = rows_map(&tmQ, q, q_rows, q_st, p.Hq, q_sh, p.Gs, p.tpt, true);
+  if (rc) return rc;
+  rc = rows_map(&tmK, k, kv_rows, kv_st, p.Hq / p.G, kv_sh, 1, 64, false);
+  if (rc) return rc;
+  rc = rows_map(&tmV, v, kv_rows, kv_st, p.Hq / p.G, kv_sh, 1, 128, false);
+  if (rc) return rc;
+  static int launch_regs = 0;
+  if (launch_regs == 0) {
+    cudaFuncAttributes fa;
+    rc = check_cuda(cudaFuncGetAttributes(&fa, attn_pair_kernel), what);
+    if (rc) return rc;
+    launch_regs = fa.numRegs;
+  }
+  if (launch_regs < kMinLaunchRegs)
+    return set_error(kErrUnsupported, std::string(what) + ": compiled register count too small for the warpgroup split");
+  rc = check_cuda(cudaFuncSetAttribute(attn_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes), what);
+  if (rc) return rc;
+  return check_cuda(launch_after(attn_pair_kernel, dim3(2 * pairs), kThreads, kSmemBytes, dependent, stream, tmQ, tmK,
+                                 tmV, p),
+                    what);
+}
+
+// Scratch of the packed form, in bytes from its start.
+struct VarlenLayout {
+  int max_list, max_parts, split;
+  int64_t part_rows;
+  size_t seq_tiles, list, groups, part_o, part_lse, total;
+};
+
+size_t up16(size_t x) { return (x + 15) & ~size_t(15); }
+
+VarlenLayout varlen_layout(int n_seqs, int total_q, int max_k, const PairParams& p, int pairs) {
+  VarlenLayout w;
+  const int tok_tile = 2 * p.tpt;
+  // a tile with more than a pair's share of the work is cut into at most twice work / share parts, so all parts of
+  // all heads number at most twice the pairs
+  w.split = max_k > kMinPartTiles * kBN;
+  w.max_parts = w.split ? 2 * pairs : 0;
+  w.max_list = total_q / tok_tile + n_seqs + w.max_parts;
+  w.part_rows = (int64_t)w.max_parts * tok_tile * p.Gs;
+  size_t at = 16;
+  w.seq_tiles = at;
+  at = up16(at + sizeof(int) * (size_t)(n_seqs + 1));
+  w.list = at;
+  at += sizeof(int4) * 2 * (size_t)w.max_list;
+  w.groups = at;
+  at += sizeof(int4) * (size_t)w.max_parts;
+  w.part_o = at;
+  at += sizeof(float) * kHeadDim * (size_t)w.part_rows;
+  w.part_lse = at;
+  at += sizeof(float) * (size_t)w.part_rows;
+  w.total = up16(at);
+  return w;
+}
+
+}  // namespace
+
+size_t attn_pair_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv) {
+  PairParams p = {};
+  p.Hq = Hq;
+  p.G = Hq / Hkv;
+  pair_tile(p);
+  return varlen_layout(n_seqs, total_q, max_k, p, num_sms_current_device() / 2).total;
+}
+
+int launch_attn_pair_varlen(const PackedAttnParams& a, int max_k, void* workspace, cudaStream_t stream) {
+  const int pairs = num_sms_current_device() / 2;
+  PairParams p = {};
+  p.o = a.o;
+  p.o_st = a.o_st;
+  p.o_sh = a.o_sh;
+  p.lse = a.lse;
+  p.lse_st = a.lse_st;
+  p.lse_sh = a.lse_sh;
+  p.v = a.v;
+  p.kv_st = a.kv_st;
+  p.kv_sh = a.kv_sh;
+  p.Hq = a.Hq;
+  p.G = a.G;
+  pair_tile(p);
+  p.scale_log2 = a.scale_log2;
+  p.status = a.status;
+  const VarlenLayout w = varlen_layout(a.n_seqs, a.total_q, max_k, p, pairs);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.header = reinterpret_cast<const int*>(ws);
+  p.list = reinterpret_cast<const int4*>(ws + w.list);
+  p.part_o = reinterpret_cast<float*>(ws + w.part_o);
+  p.part_lse = reinterpret_cast<float*>(ws + w.part_lse);
+  PlanParams pl = {};
+  pl.cu_q = a.cu_q;
+  pl.cu_k = a.cu_k;
+  pl.n_seqs = a.n_seqs;
+  pl.total_q = a.total_q;
+  pl.total_k = a.total_k;
+  pl.causal = a.causal;
+  pl.tok_tile = 2 * p.tpt;
+  pl.nh = p.nh;
+  pl.Gs = p.Gs;
+  pl.pairs = pairs;
+  pl.split = w.split;
+  pl.max_parts = w.max_parts;
+  pl.header = reinterpret_cast<int*>(ws);
+  pl.seq_tiles = reinterpret_cast<int*>(ws + w.seq_tiles);
+  pl.list = reinterpret_cast<int4*>(ws + w.list);
+  pl.groups = reinterpret_cast<int4*>(ws + w.groups);
+  pl.status = a.status;
+  attn_plan_kernel<<<1, kPlanThreads, 0, stream>>>(pl);
+  int rc = check_cuda(cudaGetLastError(), "attn_varlen plan launch");
+  if (rc) return rc;
+  rc = launch_pair(p, a.q, a.total_q, a.q_st, a.q_sh, a.k, a.v, a.total_k, a.kv_st, a.kv_sh, pairs, true, stream,
+                   "attn_varlen launch");
+  if (rc || !w.split) return rc;
+  return check_cuda(launch_after(attn_join_kernel, dim3(w.max_parts, 8), 256, 0, true, stream, p, p.header,
+                                 reinterpret_cast<const int4*>(ws + w.groups)),
+                    "attn_varlen join launch");
+}
+
+// Parts of the shared prefix: cut along the keys so that all pairs have work, in about equal rounds.
+int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int* keys_per_split) {
+  PairParams p = {};
+  p.Hq = Hq;
+  p.G = Hq / Hkv;
+  pair_tile(p);
+  const int pairs = num_sms_current_device() / 2;
+  const int64_t units = (int64_t)((B + 2 * p.tpt - 1) / (2 * p.tpt)) * p.nh;
+  const int tiles = (P + kBN - 1) / kBN;
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const int per = (tiles + s - 1) / s;
+    const int64_t rounds = (units * ((tiles + per - 1) / per) + pairs - 1) / pairs;
+    const int64_t cost = rounds * (per + 2) + s / 8;  // two tiles' time per item for its start and end
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  const int per = (tiles + best - 1) / best;
+  *keys_per_split = per * kBN;
+  return (tiles + per - 1) / per;
+}
+
+int launch_attn_pair_prefix(const PackedAttnParams& a, cudaStream_t stream) {
+  PairParams p = {};
+  p.v = a.v;
+  p.kv_st = a.kv_st;
+  p.kv_sh = a.kv_sh;
+  p.Hq = a.Hq;
+  p.G = a.G;
+  pair_tile(p);
+  p.scale_log2 = a.scale_log2;
+  p.status = a.status;
+  p.B = a.B;
+  p.P = a.P;
+  p.n_rt = (a.B + 2 * p.tpt - 1) / (2 * p.tpt);
+  p.n_splits = a.n_splits;
+  p.keys_per_split = a.keys_per_split;
+  p.part_o = a.part_o;
+  p.part_lse = a.part_lse;
+  const int64_t items = (int64_t)p.n_rt * p.n_splits * p.nh;
+  if (items > 0x3FFFFFFF) return set_error(kErrUnsupported, "attn_decode_shared: problem too large");
+  const int pairs = (int)std::min<int64_t>(num_sms_current_device() / 2, items);
+  return launch_pair(p, a.q, a.B, a.q_st, a.q_sh, a.k, a.v, a.P, a.kv_st, a.kv_sh, pairs, false, stream,
+                     "attn_decode_shared prefix launch");
+}
+
+}  // namespace fmka

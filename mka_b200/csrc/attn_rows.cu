@@ -68,20 +68,6 @@ __device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
   return row * 256 + ((chunk ^ (row & 7)) << 4);
 }
 
-// Infinities and NaNs among the eight bf16 of a 16-byte chunk are replaced by zeros; true if there were any.
-__device__ __forceinline__ bool zero_nonfinite(uint4& c) {
-  uint32_t* w = reinterpret_cast<uint32_t*>(&c);
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool lo = (w[i] & 0x7F80u) == 0x7F80u;
-    const bool hi = (w[i] & 0x7F800000u) == 0x7F800000u;
-    any |= lo | hi;
-    w[i] &= (lo ? 0xFFFF0000u : 0xFFFFFFFFu) & (hi ? 0x0000FFFFu : 0xFFFFFFFFu);
-  }
-  return any;
-}
-
 struct RowsItem {
   int row0, n_tok;   // first packed token (request), tokens of this tile
   int64_t kv_off;    // element offset of key 0 of the kv head
@@ -471,16 +457,23 @@ void slice_group(PackedAttnParams& p, int rows) {
   p.Gs = (p.G + p.n_gs - 1) / p.n_gs;
 }
 
+// Which kernel takes a packed batch. Macro for now.
+#ifndef FMKA_VARLEN_ROWS_MAX
+#define FMKA_VARLEN_ROWS_MAX 0
+#endif
+bool varlen_by_rows(int total_q, int max_k) { return (int64_t)total_q * max_k < FMKA_VARLEN_ROWS_MAX || max_k == 0; }
+
 struct SharedPlan {
   int prefix_splits, prefix_keys;  // parts over the prefix, keys per part
   int own_splits, own_keys;
+  bool pair;                       // the prefix goes to the pair kernel
 };
 
-SharedPlan plan_shared(int P, int cap) {
-  SharedPlan s{0, kTileKeys, 0, kTileKeys};
+SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
+  SharedPlan s{0, kTileKeys, 0, kTileKeys, false};
   if (P > 0) {
-    s.prefix_keys = 512;
-    s.prefix_splits = (P + s.prefix_keys - 1) / s.prefix_keys;
+    s.pair = true;
+    s.prefix_splits = attn_pair_prefix_splits(B, Hq, Hkv, P, &s.prefix_keys);
   }
   if (cap > 0) {
     s.own_keys = 512;
@@ -491,11 +484,14 @@ SharedPlan plan_shared(int P, int cap) {
 
 }  // namespace
 
-size_t attn_varlen_workspace_bytes(int, int, int, int, int) { return 0; }
+size_t attn_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv) {
+  return varlen_by_rows(total_q, max_k) ? 0 : attn_pair_varlen_workspace_bytes(n_seqs, total_q, max_k, Hq, Hkv);
+}
 
-int launch_attn_varlen(PackedAttnParams p, int, void*, cudaStream_t stream) {
+int launch_attn_varlen(PackedAttnParams p, int max_k, void* workspace, cudaStream_t stream) {
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_varlen: device status word unavailable");
+  if (!varlen_by_rows(p.total_q, max_k) && p.total_k > 0) return launch_attn_pair_varlen(p, max_k, workspace, stream);
   slice_group(p, 64);
   const int tpt = 64 / p.Gs;
   const int64_t tiles = (int64_t)p.total_q / tpt + p.n_seqs;  // at least one tile ends in every sequence
@@ -503,7 +499,7 @@ int launch_attn_varlen(PackedAttnParams p, int, void*, cudaStream_t stream) {
 }
 
 size_t attn_decode_shared_workspace_bytes(int B, int Hq, int Hkv, int P, int cap) {
-  const SharedPlan s = plan_shared(P, cap);
+  const SharedPlan s = plan_shared(B, Hq, Hkv, P, cap);
   return (size_t)(s.prefix_splits + s.own_splits) * B * Hq * (kHeadDim + 1) * sizeof(float);
 }
 
@@ -511,7 +507,7 @@ int launch_attn_decode_shared(PackedAttnParams p, const __nv_bfloat16* kp, const
                               int64_t kp_st, void* workspace, cudaStream_t stream) {
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_decode_shared: device status word unavailable");
-  const SharedPlan s = plan_shared(p.P, p.cap);
+  const SharedPlan s = plan_shared(p.B, p.Hq, p.Hkv, p.P, p.cap);
   const int parts = s.prefix_splits + s.own_splits;
   p.part_o = static_cast<float*>(workspace);
   p.part_lse = p.part_o + (int64_t)parts * p.B * p.Hq * kHeadDim;
@@ -524,10 +520,15 @@ int launch_attn_decode_shared(PackedAttnParams p, const __nv_bfloat16* kp, const
     a.n_splits = s.prefix_splits;
     a.keys_per_split = s.prefix_keys;
     a.part0 = 0;
-    slice_group(a, 64);
-    const int tpt = 64 / a.Gs;
-    int rc = launch_rows<4, kModePrefix>(a, (int64_t)((a.B + tpt - 1) / tpt) * a.n_splits, stream,
-                                         "attn_decode_shared prefix launch");
+    int rc;
+    if (s.pair) {
+      rc = launch_attn_pair_prefix(a, stream);
+    } else {
+      slice_group(a, 64);
+      const int tpt = 64 / a.Gs;
+      rc = launch_rows<4, kModePrefix>(a, (int64_t)((a.B + tpt - 1) / tpt) * a.n_splits, stream,
+                                       "attn_decode_shared prefix launch");
+    }
     if (rc) return rc;
   }
   if (s.own_splits > 0) {

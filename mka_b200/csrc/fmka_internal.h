@@ -159,6 +159,12 @@ struct PackedAttnParams {
   uint32_t* status;
 };
 
+// attn_pair.cu: the tcgen05 form for many rows.
+size_t attn_pair_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv);
+int launch_attn_pair_varlen(const PackedAttnParams& a, int max_k, void* workspace, cudaStream_t stream);
+int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int* keys_per_split);
+int launch_attn_pair_prefix(const PackedAttnParams& a, cudaStream_t stream);
+
 // Device status word used by kernels to report bounded-wait timeouts; one per
 // device, allocated lazily.
 uint32_t* device_status_word();
