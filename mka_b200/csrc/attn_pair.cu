@@ -94,7 +94,8 @@ struct PairParams {
 };
 
 __device__ __forceinline__ int pair_item_count(const PairParams& p) {
-  return (p.header != nullptr ? __ldcg(p.header) : p.n_rt * p.n_splits) * p.nh;
+  const int n = p.header != nullptr ? __ldcg(p.header) : p.n_rt * p.n_splits;
+  return __shfl_sync(0xffffffffu, n, 0) * p.nh;
 }
 
 // The items of one pair: a snake over the list, which is sorted by falling work.
@@ -109,13 +110,15 @@ __device__ __forceinline__ void load_item(const PairParams& p, int idx, PairItem
   it.gn = min(p.Gs, p.G - it.g0);
   if (p.header != nullptr) {
     const int4 a = __ldcg(p.list + 2 * li), b = __ldcg(p.list + 2 * li + 1);
-    it.q0 = a.x;
-    it.nq = a.y;
-    it.k0 = a.z;
-    it.kb = a.w;
-    it.ke = b.x;
-    it.lim0 = b.y;
-    it.part = b.z < 0 ? -1 : (int64_t)b.z + (int64_t)h * a.y * p.Gs;
+    // the shuffles tell the compiler that the whole warp holds the same values
+    it.q0 = __shfl_sync(0xffffffffu, a.x, 0);
+    it.nq = __shfl_sync(0xffffffffu, a.y, 0);
+    it.k0 = __shfl_sync(0xffffffffu, a.z, 0);
+    it.kb = __shfl_sync(0xffffffffu, a.w, 0);
+    it.ke = __shfl_sync(0xffffffffu, b.x, 0);
+    it.lim0 = __shfl_sync(0xffffffffu, b.y, 0);
+    const int part = __shfl_sync(0xffffffffu, b.z, 0);
+    it.part = part < 0 ? -1 : (int64_t)part + (int64_t)h * it.nq * p.Gs;
     it.part_ts = p.Gs;
   } else {
     const int split = li / p.n_rt, rt = li - split * p.n_rt;
@@ -129,6 +132,13 @@ __device__ __forceinline__ void load_item(const PairParams& p, int idx, PairItem
     it.part_ts = p.Hq;
   }
   it.n = it.ke > it.kb ? (it.ke - it.kb + kBN - 1) / kBN : 0;
+}
+
+// Keys of tile j that hold a key which every row of the item sees.
+__device__ __forceinline__ int rows_all_see(const PairItem& it, int j) {
+  const int kt = it.kb + j * kBN;
+  const int live = min(kBN, it.ke - kt);
+  return it.nq > 1 ? min(live, max(0, it.lim0 + 1 - kt)) : live;
 }
 
 // A walk over the key tiles of a pair's items.
@@ -153,6 +163,19 @@ struct Cursor {
     if (++j == it.n) {
       ++items;
       next_item(p, n_items, pair, pairs);
+    }
+  }
+};
+
+// Position in a ring of N stages and the parity of its current round.
+template <int N>
+struct Ring {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void step() {
+    if (++s == N) {
+      s = 0;
+      ph ^= 1u;
     }
   }
 };
@@ -189,7 +212,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   static_assert(1024 * 2 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 3 * kSBufs + 1 + 24 + 1) + 40 <= 3072,
                 "control block fits behind the tiles");
 
-  const int warp = warp_id();
+  const int warp = __shfl_sync(0xffffffffu, warp_id(), 0);
   const int lane = lane_id();
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1;
@@ -246,102 +269,131 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     // ------------------------------------------------------------ producer --
-    if (lane == 0) {
-      const uint32_t q_full_even = cluster_addr(&q_full[0], 0);
-      const uint32_t k_full_even = cluster_addr(&k_full[0], 0);
-      const int q_box = p.Gs * p.tpt * 128;  // bytes of one 64-channel box
-      Cursor kc, vc;
-      kc.next_item(p, n_items, pair, pairs);
-      vc = kc;
-      int gk = 0, gv = 0;
-      bool ok = true;
-      while (ok && !vc.end) {
-        while (!kc.end && gk - gv < kSBufs) {
-          if (kc.j == 0) {
-            const int qs = kc.items & 1;
-            if (!(ok = mbar_wait(&q_empty[qs], ((kc.items >> 1) & 1) ^ 1u, p.status))) break;
+    const uint32_t q_full_even = cluster_addr(&q_full[0], 0);
+    const uint32_t k_full_even = cluster_addr(&k_full[0], 0);
+    const int q_box = p.Gs * p.tpt * 128;  // bytes of one 64-channel box
+    Cursor kc, vc;
+    kc.next_item(p, n_items, pair, pairs);
+    vc = kc;
+    int gk = 0, gv = 0;
+    Ring<kKStages> kr;
+    Ring<kVStages> vr;
+    bool ok = true;
+    while (ok && !vc.end) {
+      while (!kc.end && gk - gv < kSBufs) {
+        if (kc.j == 0) {
+          const int qs = kc.items & 1;
+          if (!(ok = warp_wait(&q_empty[qs], ((kc.items >> 1) & 1) ^ 1u, p.status))) break;
+          if (elect_one()) {
             if (rank == 0) mbar_arrive_expect_tx(&q_full[qs], 4 * q_box);
             const int tok = kc.it.q0 + (int)rank * p.tpt;
             const int head = kc.it.hkv * p.G + kc.it.g0;
             tma_load_3d_pair(sQ + qs * kQBytes, &tmQ, q_full_even + qs * 8, 0, head, tok);
             tma_load_3d_pair(sQ + qs * kQBytes + kQHalf, &tmQ, q_full_even + qs * 8, 64, head, tok);
           }
-          const int ks = gk % kKStages;
-          if (!(ok = mbar_wait(&k_empty[ks], ((gk / kKStages) & 1) ^ 1u, p.status))) break;
-          if (rank == 0) mbar_arrive_expect_tx(&k_full[ks], 2 * kKBytes);
-          const int key = kc.it.k0 + kc.it.kb + kc.j * kBN + (int)rank * 64;
-          tma_load_3d_pair(sK + ks * kKBytes, &tmK, k_full_even + ks * 8, 0, key, kc.it.hkv);
-          tma_load_3d_pair(sK + ks * kKBytes + kKBytes / 2, &tmK, k_full_even + ks * 8, 64, key, kc.it.hkv);
-          ++gk;
-          kc.step(p, n_items, pair, pairs);
+          __syncwarp();
         }
-        if (!ok) break;
-        const int vs = gv % kVStages;
-        if (!(ok = mbar_wait(&v_empty[vs], ((gv / kVStages) & 1) ^ 1u, p.status))) break;
-        mbar_arrive_expect_tx(&v_land[vs], kVBytes);
-        tma_load_3d(sV + vs * kVBytes, &tmV, &v_land[vs], 64 * (int)rank, vc.it.k0 + vc.it.kb + vc.j * kBN, vc.it.hkv);
-        ++gv;
-        vc.step(p, n_items, pair, pairs);
-        if (*abort_flag) ok = false;
+        if (!(ok = warp_wait(&k_empty[kr.s], kr.ph ^ 1u, p.status))) break;
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(&k_full[kr.s], 2 * kKBytes);
+          const int key = kc.it.k0 + kc.it.kb + kc.j * kBN + (int)rank * 64;
+          tma_load_3d_pair(sK + kr.s * kKBytes, &tmK, k_full_even + kr.s * 8, 0, key, kc.it.hkv);
+          tma_load_3d_pair(sK + kr.s * kKBytes + kKBytes / 2, &tmK, k_full_even + kr.s * 8, 64, key, kc.it.hkv);
+        }
+        __syncwarp();
+        ++gk;
+        kr.step();
+        kc.step(p, n_items, pair, pairs);
       }
-      if (!ok) *abort_flag = 1;
-      // Drain: every load has landed, and its tile has been consumed, before the CTA goes.
-      for (int g = gv - 1; g >= 0 && g >= gv - kVStages; --g)
-        mbar_wait(&v_land[g % kVStages], (g / kVStages) & 1, p.status);
-      for (int g = gk - 1; g >= 0 && g >= gk - kKStages; --g)
-        mbar_wait(&k_empty[g % kKStages], (g / kKStages) & 1, p.status);
+      if (!ok || !(ok = warp_wait(&v_empty[vr.s], vr.ph ^ 1u, p.status))) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&v_land[vr.s], kVBytes);
+        tma_load_3d(sV + vr.s * kVBytes, &tmV, &v_land[vr.s], 64 * (int)rank, vc.it.k0 + vc.it.kb + vc.j * kBN,
+                    vc.it.hkv);
+      }
+      __syncwarp();
+      ++gv;
+      vr.step();
+      vc.step(p, n_items, pair, pairs);
+      ok = !__any_sync(0xffffffffu, *abort_flag);
     }
+    if (!ok) *abort_flag = 1;
+    // Drain: every load has landed, and its tile has been consumed, before the CTA goes.
+    for (int g = gv - 1; g >= 0 && g >= gv - kVStages; --g)
+      mbar_wait(&v_land[g % kVStages], (g / kVStages) & 1, p.status);
+    for (int g = gk - 1; g >= 0 && g >= gk - kKStages; --g)
+      mbar_wait(&k_empty[g % kKStages], (g / kKStages) & 1, p.status);
   } else if (warp == 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     // ------------------------------------------- MMA (the even CTA issues) --
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t id_s = make_idesc_bf16(256, kBN, false, false);
       constexpr uint32_t id_pv = make_idesc_bf16(256, kHeadDim, false, true);
+      const uint64_t q_desc = desc_kmajor_sw128(smem_u32(sQ));
+      const uint64_t k_desc = desc_kmajor_sw128(smem_u32(sK));
+      const uint64_t v_desc = desc_mnmajor_sw128(smem_u32(sV), kVBytes);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       Cursor sc, vc;
       sc.next_item(p, n_items, pair, pairs);
       vc = sc;
       int gs = 0, gv = 0;
+      Ring<kKStages> kr;
+      Ring<kVStages> vr;
+      Ring<kSBufs> sr, pr;
       bool ok = true;
       while (ok && !vc.end) {
         while (!sc.end && gs - gv < kSBufs) {
           const int qs = sc.items & 1;
-          if (sc.j == 0 && !(ok = mbar_wait(&q_full[qs], (sc.items >> 1) & 1, p.status))) break;
-          const int ks = gs % kKStages;
-          if (!(ok = mbar_wait(&k_full[ks], (gs / kKStages) & 1, p.status))) break;
+          if (sc.j == 0 && !(ok = warp_wait(&q_full[qs], (sc.items >> 1) & 1, p.status))) break;
+          if (!(ok = warp_wait(&k_full[kr.s], kr.ph, p.status))) break;
           tc_fence_after();
-          const uint32_t q_addr = smem_u32(sQ + qs * kQBytes);
-          const uint32_t k_addr = smem_u32(sK + ks * kKBytes);
-          const int sb = gs % kSBufs;
-          const uint32_t d = tmem + kTmemS + sb * 128;
+          const uint64_t qd = q_desc + (uint64_t)(qs * (kQBytes >> 4));
+          const uint64_t kd = k_desc + (uint64_t)(kr.s * (kKBytes >> 4));
+          const uint32_t d = tm + kTmemS + sr.s * 128;
+          const bool last = sc.j == sc.it.n - 1;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kHeadDim / 16; ++k)
-            umma_ss_pair(d, desc_kmajor_sw128(q_addr + (k >> 2) * kQHalf + (k & 3) * 32),
-                         desc_kmajor_sw128(k_addr + (k >> 2) * (kKBytes / 2) + (k & 3) * 32), id_s, k > 0 ? 1u : 0u);
-          tc_commit_pair(&s_full[sb], 0x3);
-          tc_commit_pair(&k_empty[ks], 0x3);
-          if (sc.j == sc.it.n - 1) tc_commit_pair(&q_empty[qs], 0x3);
+            for (int k = 0; k < kHeadDim / 16; ++k)
+              umma_ss_pair(d, qd + (k >> 2) * (kQHalf >> 4) + (k & 3) * 2, kd + (k >> 2) * (kKBytes >> 5) + (k & 3) * 2,
+                           id_s, k > 0 ? 1u : 0u);
+            tc_commit_pair(&s_full[sr.s], 0x3);
+            tc_commit_pair(&k_empty[kr.s], 0x3);
+            if (last) tc_commit_pair(&q_empty[qs], 0x3);
+          }
+          __syncwarp();
           ++gs;
+          kr.step();
+          sr.step();
           sc.step(p, n_items, pair, pairs);
         }
         if (!ok) break;
-        const int vs = gv % kVStages, sb = gv % kSBufs;
-        if (vc.j == 0 && vc.items > 0 && !(ok = mbar_wait_cluster(o_free, (vc.items - 1) & 1, p.status))) break;
-        if (!(ok = mbar_wait_cluster(&v_ready[vs], (gv / kVStages) & 1, p.status))) break;
-        if (!(ok = mbar_wait_cluster(&p_full[sb], (gv / kSBufs) & 1, p.status))) break;
+        if (vc.j == 0 && vc.items > 0 && !(ok = warp_wait(o_free, (vc.items - 1) & 1, p.status))) break;
+        // a tile that the gates may have written to is acquired from the other CTA as well
+        ok = rows_all_see(vc.it, vc.j) < kBN
+                 ? __all_sync(0xffffffffu, mbar_wait_cluster(&v_ready[vr.s], vr.ph, p.status))
+                 : warp_wait(&v_ready[vr.s], vr.ph, p.status);
+        if (!ok || !(ok = warp_wait(&p_full[pr.s], pr.ph, p.status))) break;
         tc_fence_after();
-        const uint32_t v_addr = smem_u32(sV + vs * kVBytes);
+        const uint64_t vd = v_desc + (uint64_t)(vr.s * (kVBytes >> 4));
+        const uint32_t a = tm + kTmemS + pr.s * 128;
+        const uint32_t add = vc.j > 0 ? 1u : 0u;
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kBN / 16; ++k)
-          umma_ts_pair(tmem + kTmemO, tmem + kTmemS + sb * 128 + k * 8,
-                       desc_mnmajor_sw128(v_addr + k * 2048, kVBytes), id_pv, (vc.j > 0 || k > 0) ? 1u : 0u);
-        tc_commit_pair(&pv_done[sb], 0x3);
-        tc_commit_pair(&v_empty[vs], 0x3);
+          for (int k = 0; k < kBN / 16; ++k)
+            umma_ts_pair(tm + kTmemO, a + k * 8, vd + k * (2048 >> 4), id_pv, k > 0 ? 1u : add);
+          tc_commit_pair(&pv_done[pr.s], 0x3);
+          tc_commit_pair(&v_empty[vr.s], 0x3);
+        }
+        __syncwarp();
         ++gv;
+        vr.step();
+        pr.step();
         vc.step(p, n_items, pair, pairs);
-        if (*abort_flag) ok = false;
+        ok = !__any_sync(0xffffffffu, *abort_flag);
       }
       if (!ok) *abort_flag = 1;
-      tc_commit_pair(mma_done, 0x1);
+      if (elect_one()) tc_commit_pair(mma_done, 0x1);
+      __syncwarp();
       mbar_wait(mma_done, 0, p.status);
     }
   } else if (warp == 3) {
@@ -351,16 +403,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t bad_peer = cluster_addr(const_cast<int*>(bad_v), rank ^ 1u);
     Cursor c;
     c.next_item(p, n_items, pair, pairs);
-    int g = 0;
+    Ring<kVStages> vr;
     while (!c.end) {
-      const int vs = g % kVStages;
-      if (!__all_sync(0xffffffffu, mbar_wait(&v_land[vs], (g / kVStages) & 1, p.status))) {
+      const int vs = vr.s;
+      if (!warp_wait(&v_land[vs], vr.ph, p.status)) {
         *abort_flag = 1;
         break;
       }
       const int kt = c.it.kb + c.j * kBN;
-      const int live = min(kBN, c.it.ke - kt);                                        // rows that hold keys
-      const int some = c.it.nq > 1 ? min(live, max(0, c.it.lim0 + 1 - kt)) : live;    // rows that every query sees
+      const int live = min(kBN, c.it.ke - kt);  // rows that hold keys
+      const int some = rows_all_see(c.it, c.j);
       if (some < kBN) {
         // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes four rows at a time
         bool bad = false;
@@ -381,10 +433,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                        : "memory");
         }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(ready_even + vs * 8);
-      ++g;
+      if (some < kBN) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(ready_even + vs * 8);
+      } else if (lane == 0) {
+        mbar_arrive_cluster_cta(ready_even + vs * 8);
+      }
+      vr.step();
       c.step(p, n_items, pair, pairs);
     }
   } else if (warp >= 4) {
@@ -514,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(p_full_even + sb * 8);
+        if (lane == 0) mbar_arrive_cluster_cta(p_full_even + sb * 8);
       }
       if (!ok) break;
       if (wg != last_wg) {
@@ -551,7 +607,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(o_free_even);
+        if (lane == 0) mbar_arrive_cluster_cta(o_free_even);
         const float L = l + l_other * (m_prev == m_own ? 1.f : fast_exp2(m_prev - m_own));
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const float lse2 = L == 0.f ? -INFINITY : m_own + __log2f(L);

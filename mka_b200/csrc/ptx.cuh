@@ -307,6 +307,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 
+// The same with the default (CTA-scope) release: for hand-overs whose data is in
+// TMEM (ordered by the tcgen05 fences), where a cluster-scope release would wait
+// for every earlier store of the thread (about 500 cycles).
+__device__ __forceinline__ void mbar_arrive_cluster_cta(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+
 // TMA tile loads into this CTA's shared memory whose completion is counted on
 // an mbarrier of the pair's even CTA (bar_cluster_addr from cluster_addr).
 __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* tmap, uint32_t bar_cluster_addr,
@@ -365,8 +372,8 @@ __device__ __forceinline__ void umma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, u
       : "memory");
 }
 
-// Bounded wait like mbar_wait on a barrier that the pair's other CTA arrives on
-// (acquire at cluster scope).
+// Bounded wait like mbar_wait with acquire at cluster scope, for shared memory
+// that the pair's other CTA has written (about 400 cycles more than mbar_wait).
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* status) {
   const uint32_t a = smem_u32(bar);
   uint64_t t0 = 0;
@@ -390,6 +397,25 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
       }
     }
   }
+}
+
+// One lane of the (converged) warp. Code around it stays warp-uniform, so that
+// descriptors and addresses live in uniform registers: a loop of pair MMAs with
+// its waits and commits then issues at the tensor pipe's rate (1022 cycles for
+// 16 MMAs of 256 x 128 x 16; 1237 inside a branch on the lane number).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+
+// Bounded wait of a whole warp, with a warp-uniform result.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
 }
 
 // Programmatic dependent launch: waits until the kernels before this one in the
