@@ -21,9 +21,11 @@
 //
 // Warp roles (12 warps per CTA):
 //   warp 0      producer: Q, K, V tiles by TMA (128-byte swizzle)
-//   warp 1      MMA issuer (the even CTA's, for both): S runs up to three tiles
-//               ahead of P V, across item borders
-//   warp 2      TMEM allocation
+//   warp 1      issues S = Q K^T (the even CTA's, for both), up to three tiles
+//               ahead of P V and across item borders
+//   warp 2      TMEM allocation; issues O += P V (the even CTA's). Two issuers,
+//               because one warp's waits, commits and bookkeeping for both
+//               products took longer (2050 cycles a tile) than the MMAs (1024)
 //   warp 3      V gate: hands each V tile to the MMA; on tiles with masked keys
 //               it first puts zeros over the rows past the last key and over
 //               infinities and NaNs in rows that only some queries see, because
@@ -48,6 +50,7 @@ constexpr int kBN = 128;        // keys per tile
 constexpr int kHeadDim = 128;
 constexpr int kThreads = 384;
 constexpr int kSBufs = 3;
+constexpr int kAhead = 3;       // key tiles that K is loaded ahead of V
 constexpr int kKStages = 5;
 constexpr int kVStages = 5;
 constexpr int kQBytes = 32768;   // 128 rows x 128 channels
@@ -60,7 +63,7 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr uint32_t kTmemO = 0, kTmemS = 128;
 // Register split between the control warps and the softmax warps (setmaxnreg);
 // the sum has to fit in what the block is launched with.
-constexpr int kRegsControl = 64;
+constexpr int kRegsControl = 72;
 constexpr int kRegsSoftmax = 216;
 constexpr int kMinLaunchRegs = (128 * kRegsControl + 256 * kRegsSoftmax + kThreads - 1) / kThreads;
 
@@ -103,36 +106,66 @@ __device__ __forceinline__ int pair_item_index(int r, int pair, int pairs) {
   return r * pairs + ((r & 1) ? pairs - 1 - pair : pair);
 }
 
-__device__ __forceinline__ void load_item(const PairParams& p, int idx, PairItem& it) {
-  const int li = idx / p.nh, h = idx - li * p.nh;
-  it.hkv = h / p.n_gs;
-  it.g0 = (h - it.hkv * p.n_gs) * p.Gs;
-  it.gn = min(p.Gs, p.G - it.g0);
-  if (p.header != nullptr) {
-    const int4 a = __ldcg(p.list + 2 * li), b = __ldcg(p.list + 2 * li + 1);
-    // the shuffles tell the compiler that the whole warp holds the same values
-    it.q0 = __shfl_sync(0xffffffffu, a.x, 0);
-    it.nq = __shfl_sync(0xffffffffu, a.y, 0);
-    it.k0 = __shfl_sync(0xffffffffu, a.z, 0);
-    it.kb = __shfl_sync(0xffffffffu, a.w, 0);
-    it.ke = __shfl_sync(0xffffffffu, b.x, 0);
-    it.lim0 = __shfl_sync(0xffffffffu, b.y, 0);
-    const int part = __shfl_sync(0xffffffffu, b.z, 0);
-    it.part = part < 0 ? -1 : (int64_t)part + (int64_t)h * it.nq * p.Gs;
-    it.part_ts = p.Gs;
-  } else {
-    const int split = li / p.n_rt, rt = li - split * p.n_rt;
-    it.q0 = rt * 2 * p.tpt;
-    it.nq = min(2 * p.tpt, p.B - it.q0);
-    it.k0 = 0;
-    it.kb = split * p.keys_per_split;
-    it.ke = min(p.P, it.kb + p.keys_per_split);
-    it.lim0 = p.P;
-    it.part = ((int64_t)split * p.B + it.q0) * p.Hq + it.hkv * p.G + it.g0;
-    it.part_ts = p.Hq;
+// The items of one pair, one after the other. The list entry of the next item is
+// loaded while the current one runs; all lanes of a warp walk together.
+struct ItemWalk {
+  int r, idx, n_items;  // round of the entry held in (a, b), its item, all items
+  int4 a, b;
+  __device__ __forceinline__ void fetch(const PairParams& p, int pair, int pairs) {
+    // the snake's odd rounds run backwards, so only some pairs have an item in the last round
+    idx = pair_item_index(r, pair, pairs);
+    if (idx >= n_items) idx = r * pairs >= n_items ? -1 : -2;  // -1: past the end, -2: none in this round
+    if (idx >= 0 && p.header != nullptr) {
+      const int li = idx / p.nh;
+      a = __ldcg(p.list + 2 * li);
+      b = __ldcg(p.list + 2 * li + 1);
+    }
   }
-  it.n = it.ke > it.kb ? (it.ke - it.kb + kBN - 1) / kBN : 0;
-}
+  __device__ __forceinline__ void start(const PairParams& p, int n, int pair, int pairs) {
+    r = 0;
+    n_items = n;
+    fetch(p, pair, pairs);
+  }
+  // The next item, or false after the last. Items without key tiles (n == 0) are only given where `empty` asks.
+  __device__ __forceinline__ bool next(const PairParams& p, int pair, int pairs, PairItem& it, bool empty) {
+    while (true) {
+      const int i = idx;
+      if (i == -1) return false;
+      if (i >= 0) {
+        const int li = i / p.nh, h = i - li * p.nh;
+        it.hkv = h / p.n_gs;
+        it.g0 = (h - it.hkv * p.n_gs) * p.Gs;
+        it.gn = min(p.Gs, p.G - it.g0);
+        if (p.header != nullptr) {
+          // the shuffles tell the compiler that the whole warp holds the same values
+          it.q0 = __shfl_sync(0xffffffffu, a.x, 0);
+          it.nq = __shfl_sync(0xffffffffu, a.y, 0);
+          it.k0 = __shfl_sync(0xffffffffu, a.z, 0);
+          it.kb = __shfl_sync(0xffffffffu, a.w, 0);
+          it.ke = __shfl_sync(0xffffffffu, b.x, 0);
+          it.lim0 = __shfl_sync(0xffffffffu, b.y, 0);
+          const int part = __shfl_sync(0xffffffffu, b.z, 0);
+          it.part = part < 0 ? -1 : (int64_t)part + (int64_t)h * it.nq * p.Gs;
+          it.part_ts = p.Gs;
+        } else {
+          const int split = li / p.n_rt, rt = li - split * p.n_rt;
+          it.q0 = rt * 2 * p.tpt;
+          it.nq = min(2 * p.tpt, p.B - it.q0);
+          it.k0 = 0;
+          it.kb = split * p.keys_per_split;
+          it.ke = min(p.P, it.kb + p.keys_per_split);
+          it.lim0 = p.P;
+          it.part = ((int64_t)split * p.B + it.q0) * p.Hq + it.hkv * p.G + it.g0;
+          it.part_ts = p.Hq;
+        }
+        it.n = it.ke > it.kb ? (it.ke - it.kb + kBN - 1) / kBN : 0;
+      }
+      ++r;
+      fetch(p, pair, pairs);
+      if (i >= 0 && (it.n > 0 || empty)) return true;
+    }
+  }
+};
 
 // Keys of tile j that hold a key which every row of the item sees.
 __device__ __forceinline__ int rows_all_see(const PairItem& it, int j) {
@@ -140,32 +173,6 @@ __device__ __forceinline__ int rows_all_see(const PairItem& it, int j) {
   const int live = min(kBN, it.ke - kt);
   return it.nq > 1 ? min(live, max(0, it.lim0 + 1 - kt)) : live;
 }
-
-// A walk over the key tiles of a pair's items.
-struct Cursor {
-  int r = -1, j = 0, items = 0;
-  bool end = false;
-  PairItem it;
-  __device__ __forceinline__ void next_item(const PairParams& p, int n_items, int pair, int pairs) {
-    do {
-      const int idx = pair_item_index(++r, pair, pairs);
-      // the snake's odd rounds run backwards: the last round can be short at either end
-      if (r * pairs >= n_items) {
-        end = true;
-        return;
-      }
-      it.n = 0;
-      if (idx < n_items) load_item(p, idx, it);
-    } while (it.n == 0);
-    j = 0;
-  }
-  __device__ __forceinline__ void step(const PairParams& p, int n_items, int pair, int pairs) {
-    if (++j == it.n) {
-      ++items;
-      next_item(p, n_items, pair, pairs);
-    }
-  }
-};
 
 // Position in a ring of N stages and the parity of its current round.
 template <int N>
@@ -205,11 +212,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t* o_free = pv_done + kSBufs;     // even CTA, 8 warps
   uint64_t* m_bar = o_free + 1;            // [2][4] maximum handed on, per quarter
   uint64_t* l_bar = m_bar + 8;             // [2][2][4] sum handed on: warpgroup, its count's parity, quarter
-  uint64_t* mma_done = l_bar + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  uint64_t* mma_done = l_bar + 16;         // [2] S, P V
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* bad_v = abort_flag + 1;    // [8] by item number: 1 + the last item with taken-out values
-  static_assert(1024 * 2 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 3 * kSBufs + 1 + 24 + 1) + 40 <= 3072,
+  static_assert(1024 * 2 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 3 * kSBufs + 1 + 24 + 2) + 40 <= 3072,
                 "control block fits behind the tiles");
 
   const int warp = __shfl_sync(0xffffffffu, warp_id(), 0);
@@ -244,7 +251,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     mbar_init(o_free, 8);
     for (int i = 0; i < 8; ++i) mbar_init(&m_bar[i], 1);
     for (int i = 0; i < 16; ++i) mbar_init(&l_bar[i], 1);
-    mbar_init(mma_done, 1);
+    mbar_init(&mma_done[0], 1);
+    mbar_init(&mma_done[1], 1);
     *abort_flag = 0;
     for (int i = 0; i < 8; ++i) bad_v[i] = 0;
     fence_barrier_init();
@@ -269,25 +277,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     // ------------------------------------------------------------ producer --
+    // K runs kAhead tiles ahead of V, as S runs ahead of P V.
     const uint32_t q_full_even = cluster_addr(&q_full[0], 0);
     const uint32_t k_full_even = cluster_addr(&k_full[0], 0);
     const int q_box = p.Gs * p.tpt * 128;  // bytes of one 64-channel box
-    Cursor kc, vc;
-    kc.next_item(p, n_items, pair, pairs);
-    vc = kc;
-    int gk = 0, gv = 0;
+    ItemWalk kw, vw;
+    PairItem ki, vi;
+    kw.start(p, n_items, pair, pairs);
+    vw = kw;
+    bool k_more = kw.next(p, pair, pairs, ki, false), v_more = vw.next(p, pair, pairs, vi, false);
+    int kj = 0, vj = 0, ahead = 0, gk = 0, gv = 0, k_items = 0;
     Ring<kKStages> kr;
     Ring<kVStages> vr;
     bool ok = true;
-    while (ok && !vc.end) {
-      while (!kc.end && gk - gv < kSBufs) {
-        if (kc.j == 0) {
-          const int qs = kc.items & 1;
-          if (!(ok = warp_wait(&q_empty[qs], ((kc.items >> 1) & 1) ^ 1u, p.status))) break;
+    while (ok && v_more) {
+      while (k_more && ahead < kAhead) {
+        if (kj == 0) {
+          const int qs = k_items & 1;
+          if (!(ok = warp_wait(&q_empty[qs], ((k_items >> 1) & 1) ^ 1u, p.status))) break;
           if (elect_one()) {
             if (rank == 0) mbar_arrive_expect_tx(&q_full[qs], 4 * q_box);
-            const int tok = kc.it.q0 + (int)rank * p.tpt;
-            const int head = kc.it.hkv * p.G + kc.it.g0;
+            const int tok = ki.q0 + (int)rank * p.tpt;
+            const int head = ki.hkv * p.G + ki.g0;
             tma_load_3d_pair(sQ + qs * kQBytes, &tmQ, q_full_even + qs * 8, 0, head, tok);
             tma_load_3d_pair(sQ + qs * kQBytes + kQHalf, &tmQ, q_full_even + qs * 8, 64, head, tok);
           }
@@ -296,26 +307,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (!(ok = warp_wait(&k_empty[kr.s], kr.ph ^ 1u, p.status))) break;
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&k_full[kr.s], 2 * kKBytes);
-          const int key = kc.it.k0 + kc.it.kb + kc.j * kBN + (int)rank * 64;
-          tma_load_3d_pair(sK + kr.s * kKBytes, &tmK, k_full_even + kr.s * 8, 0, key, kc.it.hkv);
-          tma_load_3d_pair(sK + kr.s * kKBytes + kKBytes / 2, &tmK, k_full_even + kr.s * 8, 64, key, kc.it.hkv);
+          const int key = ki.k0 + ki.kb + kj * kBN + (int)rank * 64;
+          tma_load_3d_pair(sK + kr.s * kKBytes, &tmK, k_full_even + kr.s * 8, 0, key, ki.hkv);
+          tma_load_3d_pair(sK + kr.s * kKBytes + kKBytes / 2, &tmK, k_full_even + kr.s * 8, 64, key, ki.hkv);
         }
         __syncwarp();
         ++gk;
+        ++ahead;
         kr.step();
-        kc.step(p, n_items, pair, pairs);
+        if (++kj == ki.n) {
+          kj = 0;
+          ++k_items;
+          k_more = kw.next(p, pair, pairs, ki, false);
+          if (__any_sync(0xffffffffu, *abort_flag)) ok = false;
+        }
       }
       if (!ok || !(ok = warp_wait(&v_empty[vr.s], vr.ph ^ 1u, p.status))) break;
       if (elect_one()) {
         mbar_arrive_expect_tx(&v_land[vr.s], kVBytes);
-        tma_load_3d(sV + vr.s * kVBytes, &tmV, &v_land[vr.s], 64 * (int)rank, vc.it.k0 + vc.it.kb + vc.j * kBN,
-                    vc.it.hkv);
+        tma_load_3d(sV + vr.s * kVBytes, &tmV, &v_land[vr.s], 64 * (int)rank, vi.k0 + vi.kb + vj * kBN, vi.hkv);
       }
       __syncwarp();
       ++gv;
+      --ahead;
       vr.step();
-      vc.step(p, n_items, pair, pairs);
-      ok = !__any_sync(0xffffffffu, *abort_flag);
+      if (++vj == vi.n) {
+        vj = 0;
+        v_more = vw.next(p, pair, pairs, vi, false);
+      }
     }
     if (!ok) *abort_flag = 1;
     // Drain: every load has landed, and its tile has been consumed, before the CTA goes.
@@ -325,32 +344,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_wait(&k_empty[g % kKStages], (g / kKStages) & 1, p.status);
   } else if (warp == 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
-    // ------------------------------------------- MMA (the even CTA issues) --
+    // ----------------------------------- S = Q K^T (the even CTA issues) --
     if (rank == 0) {
       constexpr uint32_t id_s = make_idesc_bf16(256, kBN, false, false);
-      constexpr uint32_t id_pv = make_idesc_bf16(256, kHeadDim, false, true);
       const uint64_t q_desc = desc_kmajor_sw128(smem_u32(sQ));
       const uint64_t k_desc = desc_kmajor_sw128(smem_u32(sK));
-      const uint64_t v_desc = desc_mnmajor_sw128(smem_u32(sV), kVBytes);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      Cursor sc, vc;
-      sc.next_item(p, n_items, pair, pairs);
-      vc = sc;
-      int gs = 0, gv = 0;
+      ItemWalk w;
+      PairItem it;
+      w.start(p, n_items, pair, pairs);
       Ring<kKStages> kr;
-      Ring<kVStages> vr;
-      Ring<kSBufs> sr, pr;
+      Ring<kSBufs> sr;
+      Ring<2> qr;
       bool ok = true;
-      while (ok && !vc.end) {
-        while (!sc.end && gs - gv < kSBufs) {
-          const int qs = sc.items & 1;
-          if (sc.j == 0 && !(ok = warp_wait(&q_full[qs], (sc.items >> 1) & 1, p.status))) break;
-          if (!(ok = warp_wait(&k_full[kr.s], kr.ph, p.status))) break;
+      while (ok && w.next(p, pair, pairs, it, false)) {
+        if (!(ok = warp_wait(&q_full[qr.s], qr.ph, p.status))) break;
+        const uint64_t qd = q_desc + (uint64_t)(qr.s * (kQBytes >> 4));
+        for (int j = 0; j < it.n; ++j) {
+          // the K tile, and the S buffer (its last P has been multiplied)
+          if (!(ok = warp_wait(&k_full[kr.s], kr.ph, p.status) && warp_wait(&pv_done[sr.s], sr.ph ^ 1u, p.status))) break;
           tc_fence_after();
-          const uint64_t qd = q_desc + (uint64_t)(qs * (kQBytes >> 4));
           const uint64_t kd = k_desc + (uint64_t)(kr.s * (kKBytes >> 4));
           const uint32_t d = tm + kTmemS + sr.s * 128;
-          const bool last = sc.j == sc.it.n - 1;
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kHeadDim / 16; ++k)
@@ -358,91 +373,108 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                            id_s, k > 0 ? 1u : 0u);
             tc_commit_pair(&s_full[sr.s], 0x3);
             tc_commit_pair(&k_empty[kr.s], 0x3);
-            if (last) tc_commit_pair(&q_empty[qs], 0x3);
           }
           __syncwarp();
-          ++gs;
           kr.step();
           sr.step();
-          sc.step(p, n_items, pair, pairs);
         }
-        if (!ok) break;
-        if (vc.j == 0 && vc.items > 0 && !(ok = warp_wait(o_free, (vc.items - 1) & 1, p.status))) break;
-        // a tile that the gates may have written to is acquired from the other CTA as well
-        ok = rows_all_see(vc.it, vc.j) < kBN
-                 ? __all_sync(0xffffffffu, mbar_wait_cluster(&v_ready[vr.s], vr.ph, p.status))
-                 : warp_wait(&v_ready[vr.s], vr.ph, p.status);
-        if (!ok || !(ok = warp_wait(&p_full[pr.s], pr.ph, p.status))) break;
-        tc_fence_after();
-        const uint64_t vd = v_desc + (uint64_t)(vr.s * (kVBytes >> 4));
-        const uint32_t a = tm + kTmemS + pr.s * 128;
-        const uint32_t add = vc.j > 0 ? 1u : 0u;
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kBN / 16; ++k)
-            umma_ts_pair(tm + kTmemO, a + k * 8, vd + k * (2048 >> 4), id_pv, k > 0 ? 1u : add);
-          tc_commit_pair(&pv_done[pr.s], 0x3);
-          tc_commit_pair(&v_empty[vr.s], 0x3);
-        }
+        if (ok && elect_one()) tc_commit_pair(&q_empty[qr.s], 0x3);
         __syncwarp();
-        ++gv;
-        vr.step();
-        pr.step();
-        vc.step(p, n_items, pair, pairs);
-        ok = !__any_sync(0xffffffffu, *abort_flag);
+        qr.step();
+        if (__any_sync(0xffffffffu, *abort_flag)) ok = false;
       }
       if (!ok) *abort_flag = 1;
-      if (elect_one()) tc_commit_pair(mma_done, 0x1);
+      if (elect_one()) tc_commit_pair(&mma_done[0], 0x1);
       __syncwarp();
-      mbar_wait(mma_done, 0, p.status);
+      mbar_wait(&mma_done[0], 0, p.status);
+    }
+  } else if (warp == 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    // ------------------------------------ O += P V (the even CTA issues) --
+    if (rank == 0) {
+      constexpr uint32_t id_pv = make_idesc_bf16(256, kHeadDim, false, true);
+      const uint64_t v_desc = desc_mnmajor_sw128(smem_u32(sV), kVBytes);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      ItemWalk w;
+      PairItem it;
+      w.start(p, n_items, pair, pairs);
+      Ring<kVStages> vr;
+      Ring<kSBufs> pr;
+      uint32_t o_phase = 1;  // nothing to wait for before the first item
+      bool ok = true;
+      while (ok && w.next(p, pair, pairs, it, false)) {
+        if (!(ok = warp_wait(o_free, o_phase, p.status))) break;
+        o_phase ^= 1u;
+        for (int j = 0; j < it.n; ++j) {
+          // a tile that the gates may have written to is acquired from the other CTA as well
+          ok = rows_all_see(it, j) < kBN ? __all_sync(0xffffffffu, mbar_wait_cluster(&v_ready[vr.s], vr.ph, p.status))
+                                         : warp_wait(&v_ready[vr.s], vr.ph, p.status);
+          if (!ok || !(ok = warp_wait(&p_full[pr.s], pr.ph, p.status))) break;
+          tc_fence_after();
+          const uint64_t vd = v_desc + (uint64_t)(vr.s * (kVBytes >> 4));
+          const uint32_t a = tm + kTmemS + pr.s * 128;
+          const uint32_t add = j > 0 ? 1u : 0u;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kBN / 16; ++k)
+              umma_ts_pair(tm + kTmemO, a + k * 8, vd + k * (2048 >> 4), id_pv, k > 0 ? 1u : add);
+            tc_commit_pair(&pv_done[pr.s], 0x3);
+            tc_commit_pair(&v_empty[vr.s], 0x3);
+          }
+          __syncwarp();
+          vr.step();
+          pr.step();
+        }
+        if (__any_sync(0xffffffffu, *abort_flag)) ok = false;
+      }
+      if (!ok) *abort_flag = 1;
+      if (elect_one()) tc_commit_pair(&mma_done[1], 0x1);
+      __syncwarp();
+      mbar_wait(&mma_done[1], 0, p.status);
     }
   } else if (warp == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     // -------------------------------------------------------------- V gate --
     const uint32_t ready_even = cluster_addr(&v_ready[0], 0);
     const uint32_t bad_peer = cluster_addr(const_cast<int*>(bad_v), rank ^ 1u);
-    Cursor c;
-    c.next_item(p, n_items, pair, pairs);
+    ItemWalk w;
+    PairItem it;
+    w.start(p, n_items, pair, pairs);
     Ring<kVStages> vr;
-    while (!c.end) {
-      const int vs = vr.s;
-      if (!warp_wait(&v_land[vs], vr.ph, p.status)) {
-        *abort_flag = 1;
-        break;
-      }
-      const int kt = c.it.kb + c.j * kBN;
-      const int live = min(kBN, c.it.ke - kt);  // rows that hold keys
-      const int some = rows_all_see(c.it, c.j);
-      if (some < kBN) {
-        // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes four rows at a time
-        bool bad = false;
-        for (int row = some + (lane >> 3); row < kBN; row += 4) {
-          uint4* at = reinterpret_cast<uint4*>(sV + vs * kVBytes + row * 128 + (lane & 7) * 16);
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (row < live) {
-            x = *at;
-            if (!zero_nonfinite(x)) continue;
-            bad = true;
+    bool ok = true;
+    for (int item = 1; ok && w.next(p, pair, pairs, it, false); ++item) {
+      for (int j = 0; j < it.n; ++j) {
+        if (!(ok = warp_wait(&v_land[vr.s], vr.ph, p.status))) break;
+        const int live = min(kBN, it.ke - it.kb - j * kBN);  // rows that hold keys
+        const int some = rows_all_see(it, j);
+        if (some < kBN) {
+          // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes four rows at a time
+          bool bad = false;
+          for (int row = some + (lane >> 3); row < kBN; row += 4) {
+            uint4* at = reinterpret_cast<uint4*>(sV + vr.s * kVBytes + row * 128 + (lane & 7) * 16);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row < live) {
+              x = *at;
+              if (!zero_nonfinite(x)) continue;
+              bad = true;
+            }
+            *at = x;
           }
-          *at = x;
+          if (__any_sync(0xffffffffu, bad) && lane == 0) {
+            // the gate is at most five tiles ahead of the products, so eight slots never meet
+            bad_v[item & 7] = item;
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(bad_peer + 4 * (item & 7)), "r"(item) : "memory");
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(ready_even + vr.s * 8);
+        } else if (lane == 0) {
+          mbar_arrive_cluster_cta(ready_even + vr.s * 8);
         }
-        if (__any_sync(0xffffffffu, bad) && lane == 0) {
-          // the gate is at most five tiles ahead of the products, so eight slots never meet
-          bad_v[c.items & 7] = c.items + 1;
-          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(bad_peer + 4 * (c.items & 7)), "r"(c.items + 1)
-                       : "memory");
-        }
+        vr.step();
       }
-      if (some < kBN) {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(ready_even + vs * 8);
-      } else if (lane == 0) {
-        mbar_arrive_cluster_cta(ready_even + vs * 8);
-      }
-      vr.step();
-      c.step(p, n_items, pair, pairs);
     }
+    if (!ok) *abort_flag = 1;
   } else if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ------------------------------------------------------------- softmax --
@@ -459,10 +491,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int gave = 0, took = 0;                        // sums handed to / by the other warpgroup so far
     bool ok = true;
     PairItem it;
-    for (int rr = 0; ok && rr * pairs < n_items; ++rr) {
-      const int idx = pair_item_index(rr, pair, pairs);
-      if (idx >= n_items) continue;
-      load_item(p, idx, it);
+    ItemWalk w;
+    w.start(p, n_items, pair, pairs);
+    while (ok && w.next(p, pair, pairs, it, true)) {
       const bool row_ok = ri < p.tpt && ti < it.nq && rg < it.gn;
       const int n = it.n;
       if (n == 0) {
@@ -598,7 +629,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           break;
         }
         tc_fence_after();
-        const bool bad = bad_v[items & 7] == items + 1;
+        const bool bad = bad_v[(items + 1) & 7] == items + 1;
         uint32_t o[128];
         tmem_ld32(lane_addr + kTmemO + 0, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
         tmem_ld32(lane_addr + kTmemO + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
@@ -660,8 +691,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       ++items;
     }
     if (!ok) *abort_flag = 1;
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));  // warp 2
   }
 
   __syncwarp();
