@@ -12,17 +12,17 @@
 // Each pair multiplies with the 2-SM MMA (M = 256, cta_group::2): every CTA
 // holds its own 128 rows of Q, S, P and O and only half of each K tile (64
 // keys) and V tile (64 channels), which halves the operand traffic per SM.
-// TMEM of each CTA (512 columns): O | S0 | S1 | S2. P (bf16) is written over its
-// S and read from there by the second product. With one row tile per CTA and
-// three S buffers, the two softmax warpgroups take the key tiles of the same
-// rows in turn: while one is in its exponentials, the other finds its row
-// maxima, and the next S is already there, so the chain S -> softmax -> P V ->
-// next S of one tile no longer bounds the step.
+// TMEM of each CTA (512 columns): O | S0 | S1 | P0 | P1. With one row tile per CTA,
+// two softmax warpgroups take the key tiles of the same rows in turn, each with
+// its own S and P (bf16) buffer: an S buffer is free again once its scores are in
+// registers, so S of the next tiles is made during the exponentials and nothing
+// waits for the chain S -> softmax -> P V -> next S of a tile. (With P written
+// over S, three S buffers and that chain, a tile took 1700 cycles.)
 //
 // Warp roles (12 warps per CTA):
 //   warp 0      producer: Q, K, V tiles by TMA (128-byte swizzle)
-//   warp 1      issues S = Q K^T (the even CTA's, for both), up to three tiles
-//               ahead of P V and across item borders
+//   warp 1      issues S = Q K^T (the even CTA's, for both), ahead of P V and
+//               across item borders
 //   warp 2      TMEM allocation; issues O += P V (the even CTA's). Two issuers,
 //               because one warp's waits, commits and bookkeeping for both
 //               products took longer (2050 cycles a tile) than the MMAs (1024)
@@ -49,7 +49,6 @@ namespace {
 constexpr int kBN = 128;        // keys per tile
 constexpr int kHeadDim = 128;
 constexpr int kThreads = 384;
-constexpr int kSBufs = 3;
 constexpr int kAhead = 3;       // key tiles that K is loaded ahead of V
 constexpr int kKStages = 5;
 constexpr int kVStages = 5;
@@ -60,7 +59,7 @@ constexpr int kVBytes = 16384;   // 128 keys x 64 channels
 constexpr int kTileSmem = 2 * kQBytes + kKStages * kKBytes + kVStages * kVBytes;
 constexpr int kSmemBytes = kTileSmem + 3072;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
-constexpr uint32_t kTmemO = 0, kTmemS = 128;
+constexpr uint32_t kTmemO = 0, kTmemS = 128, kTmemP = 384;  // S: 2 x 128 columns, P: 2 x 64
 // Register split between the control warps and the softmax warps (setmaxnreg);
 // the sum has to fit in what the block is launched with.
 constexpr int kRegsControl = 72;
@@ -206,17 +205,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint64_t* v_land = k_empty + kKStages;   // [kVStages] own loads have landed
   uint64_t* v_ready = v_land + kVStages;   // [kVStages] even CTA: both gates passed
   uint64_t* v_empty = v_ready + kVStages;  // [kVStages] both
-  uint64_t* s_full = v_empty + kVStages;   // [kSBufs] both
-  uint64_t* p_full = s_full + kSBufs;      // [kSBufs] even CTA, 8 warps
-  uint64_t* pv_done = p_full + kSBufs;     // [kSBufs] both
-  uint64_t* o_free = pv_done + kSBufs;     // even CTA, 8 warps
+  uint64_t* s_full = v_empty + kVStages;   // [2] both
+  uint64_t* s_free = s_full + 2;           // [2] even CTA, 8 warps
+  uint64_t* p_full = s_free + 2;           // [2] even CTA, 8 warps
+  uint64_t* pv_done = p_full + 2;          // [4] both, by tile number
+  uint64_t* o_free = pv_done + 4;          // even CTA, 8 warps
   uint64_t* m_bar = o_free + 1;            // [2][4] maximum handed on, per quarter
   uint64_t* l_bar = m_bar + 8;             // [2][2][4] sum handed on: warpgroup, its count's parity, quarter
   uint64_t* mma_done = l_bar + 16;         // [2] S, P V
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* bad_v = abort_flag + 1;    // [8] by item number: 1 + the last item with taken-out values
-  static_assert(1024 * 2 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 3 * kSBufs + 1 + 24 + 2) + 40 <= 3072,
+  static_assert(1024 * 2 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 6 + 4 + 1 + 24 + 2) + 40 <= 3072,
                 "control block fits behind the tiles");
 
   const int warp = __shfl_sync(0xffffffffu, warp_id(), 0);
@@ -243,11 +243,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&v_ready[i], 2);
       mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < kSBufs; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 8);
       mbar_init(&p_full[i], 8);
-      mbar_init(&pv_done[i], 1);
     }
+    for (int i = 0; i < 4; ++i) mbar_init(&pv_done[i], 1);
     mbar_init(o_free, 8);
     for (int i = 0; i < 8; ++i) mbar_init(&m_bar[i], 1);
     for (int i = 0; i < 16; ++i) mbar_init(&l_bar[i], 1);
@@ -266,6 +267,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tmem_alloc_pair(tmem_slot, 512);
     tmem_relinquish_pair();
   }
+  // rows that no Q box reaches
+  for (int i = threadIdx.x; i < 4 * (128 - p.Gs * p.tpt) * 8; i += kThreads) {
+    const int per = (128 - p.Gs * p.tpt) * 8, half = i / per;
+    reinterpret_cast<uint4*>(sQ + half * kQHalf + p.Gs * p.tpt * 128)[i - half * per] = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
@@ -354,15 +361,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       PairItem it;
       w.start(p, n_items, pair, pairs);
       Ring<kKStages> kr;
-      Ring<kSBufs> sr;
-      Ring<2> qr;
+      Ring<2> sr, qr;
       bool ok = true;
       while (ok && w.next(p, pair, pairs, it, false)) {
         if (!(ok = warp_wait(&q_full[qr.s], qr.ph, p.status))) break;
         const uint64_t qd = q_desc + (uint64_t)(qr.s * (kQBytes >> 4));
         for (int j = 0; j < it.n; ++j) {
-          // the K tile, and the S buffer (its last P has been multiplied)
-          if (!(ok = warp_wait(&k_full[kr.s], kr.ph, p.status) && warp_wait(&pv_done[sr.s], sr.ph ^ 1u, p.status))) break;
+          // the K tile, and the S buffer (its last scores are in registers)
+          if (!(ok = warp_wait(&k_full[kr.s], kr.ph, p.status) && warp_wait(&s_free[sr.s], sr.ph ^ 1u, p.status))) break;
           tc_fence_after();
           const uint64_t kd = k_desc + (uint64_t)(kr.s * (kKBytes >> 4));
           const uint32_t d = tm + kTmemS + sr.s * 128;
@@ -399,7 +405,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       PairItem it;
       w.start(p, n_items, pair, pairs);
       Ring<kVStages> vr;
-      Ring<kSBufs> pr;
+      Ring<2> pr;
+      Ring<4> dr;
       uint32_t o_phase = 1;  // nothing to wait for before the first item
       bool ok = true;
       while (ok && w.next(p, pair, pairs, it, false)) {
@@ -412,18 +419,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (!ok || !(ok = warp_wait(&p_full[pr.s], pr.ph, p.status))) break;
           tc_fence_after();
           const uint64_t vd = v_desc + (uint64_t)(vr.s * (kVBytes >> 4));
-          const uint32_t a = tm + kTmemS + pr.s * 128;
+          const uint32_t a = tm + kTmemP + pr.s * 64;
           const uint32_t add = j > 0 ? 1u : 0u;
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kBN / 16; ++k)
               umma_ts_pair(tm + kTmemO, a + k * 8, vd + k * (2048 >> 4), id_pv, k > 0 ? 1u : add);
-            tc_commit_pair(&pv_done[pr.s], 0x3);
+            tc_commit_pair(&pv_done[dr.s], 0x3);
             tc_commit_pair(&v_empty[vr.s], 0x3);
           }
           __syncwarp();
           vr.step();
           pr.step();
+          dr.step();
         }
         if (__any_sync(0xffffffffu, *abort_flag)) ok = false;
       }
@@ -482,7 +490,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int quarter = warp & 3;  // the TMEM lanes this warp may touch
     const int r = quarter * 32 + lane;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t p_full_even = cluster_addr(&p_full[0], 0);
+    const uint32_t p_full_even = cluster_addr(&p_full[wg], 0);
+    const uint32_t s_free_even = cluster_addr(&s_free[wg], 0);
     const uint32_t o_free_even = cluster_addr(o_free, 0);
     const int ri = r / p.Gs, rg = r - ri * p.Gs;  // token of the CTA's tile, head of the slice
     const int ti = (int)rank * p.tpt + ri;         // token of the pair's tile
@@ -506,17 +515,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         continue;
       }
-      const int lim = row_ok ? min(it.ke - 1, it.lim0 + ti) : -1;  // last visible key
+      // Last visible key. Rows that are not there (behind the last token, or the last rows where the group does not
+      // divide 128) multiply whatever their Q holds; nothing of theirs is stored or has a say in the rescaling.
+      const int lim = row_ok ? min(it.ke - 1, it.lim0 + ti) : 0x3FFFFFFF;
       const int last_wg = (g0 + n - 1) & 1;
       float m_own = -INFINITY, m_prev = -INFINITY, l = 0.f;
       for (int j = (g0 & 1) == wg ? 0 : 1; j < n; j += 2) {
-        const int g = g0 + j;
-        const int sb = g % kSBufs;
-        const uint32_t s_col = kTmemS + sb * 128;
-        if (!__all_sync(0xffffffffu, mbar_wait(&s_full[sb], (g / kSBufs) & 1, p.status))) {
-          ok = false;
-          break;
-        }
+        const int g = g0 + j;  // g & 1 == wg
+        const uint32_t s_col = kTmemS + wg * 128, p_col = kTmemP + wg * 64;
+        if (!(ok = warp_wait(&s_full[wg], (g >> 1) & 1, p.status))) break;
         tc_fence_after();
         const int kbase = it.kb + j * kBN;
         uint32_t s[128];
@@ -525,10 +532,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tmem_ld32(lane_addr + s_col + 64, *reinterpret_cast<uint32_t(*)[32]>(&s[64]));
         tmem_ld32(lane_addr + s_col + 96, *reinterpret_cast<uint32_t(*)[32]>(&s[96]));
         tmem_wait_ld();
-        if (kbase + kBN - 1 > lim) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_cta(s_free_even);
+        const int seen = lim - kbase;  // last visible column of the tile
+        if (__any_sync(0xffffffffu, seen < kBN - 1)) {
+          const int all_see = __reduce_min_sync(0xffffffffu, seen);
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (kbase + c > lim) s[c] = 0xFF800000u;  // -inf
+          for (int c0 = 0; c0 < 128; c0 += 16) {
+            if (all_see < c0 + 15) {
+#pragma unroll
+              for (int c = c0; c < c0 + 16; ++c)
+                if (c > seen) s[c] = 0xFF800000u;  // -inf
+            }
+          }
         }
         float mxa[8];
 #pragma unroll
@@ -541,30 +558,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const float mx = p.scale_log2 * fmax3(fmax3(mxa[0], mxa[1], mxa[2]), fmax3(mxa[3], mxa[4], mxa[5]),
                                               fmaxf(mxa[6], mxa[7]));
         // the maximum after the tile before (the other warpgroup's, same rows)
-        if (g > 0 && !__all_sync(0xffffffffu, mbar_wait(&m_bar[((g - 1) & 1) * 4 + quarter], ((g - 1) >> 1) & 1,
-                                                         p.status))) {
-          ok = false;
-          break;
-        }
-        float m_ref = j > 0 ? s_m[((g - 1) & 1) * 128 + r] : -INFINITY;
+        if (g > 0 && !(ok = warp_wait(&m_bar[(wg ^ 1) * 4 + quarter], ((g - 1) >> 1) & 1, p.status))) break;
+        float m_ref = j > 0 ? s_m[(wg ^ 1) * 128 + r] : -INFINITY;
         m_prev = m_ref;
         float alpha = 1.f;
-        const bool grow = __any_sync(0xffffffffu, mx > m_ref + kRescaleThreshold);
+        const bool grow = __any_sync(0xffffffffu, row_ok && mx > m_ref + kRescaleThreshold);
         if (grow) {
           const float m_new = fmaxf(m_ref, mx);
           alpha = m_new == m_ref ? 1.f : fast_exp2(m_ref - m_new);
           m_ref = m_new;
         }
-        s_m[(g & 1) * 128 + r] = m_ref;
+        s_m[wg * 128 + r] = m_ref;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&m_bar[(g & 1) * 4 + quarter]);
+        if (lane == 0) mbar_arrive(&m_bar[wg * 4 + quarter]);
+        // this warpgroup's last P has been multiplied, so its buffer is free
+        if (g > 1 && !(ok = warp_wait(&pv_done[(g - 2) & 3], ((g - 2) >> 2) & 1, p.status))) break;
         if (grow && j > 0) {
-          // O holds the tiles before this one: wait for the last product, then move O to the new maximum. (One
-          // barrier per S buffer: S(g) is there, so the product of tile g - 3 is complete and no phase is skipped.)
-          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[(g - 1) % kSBufs], ((g - 1) / kSBufs) & 1, p.status))) {
-            ok = false;
-            break;
-          }
+          // O holds the tiles before this one: wait for the last product, then move O to the new maximum. (No phase
+          // of the barrier is skipped: the other warpgroup has waited for tile g - 5 before it wrote P of tile g - 3,
+          // whose product comes before that of tile g - 2.)
+          if (!(ok = warp_wait(&pv_done[(g - 1) & 3], ((g - 1) >> 2) & 1, p.status))) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c4 = 0; c4 < 8; ++c4) {
@@ -594,14 +607,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             acc[c & 3] = fadd2(acc[c & 3], pp);
             pk[c] = pack_bf16x2(pp.x, pp.y);
           }
-          tmem_st16(lane_addr + s_col + 16 * ch, pk);
+          tmem_st16(lane_addr + p_col + 16 * ch, pk);
         }
         const float2 asum = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
         l += asum.x + asum.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_cta(p_full_even + sb * 8);
+        if (lane == 0) mbar_arrive_cluster_cta(p_full_even);
       }
       if (!ok) break;
       if (wg != last_wg) {
@@ -624,7 +637,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           l_other = s_l[(took & 1) * 128 + r];
           ++took;
         }
-        if (!__all_sync(0xffffffffu, e_ok && mbar_wait(&pv_done[gl % kSBufs], (gl / kSBufs) & 1, p.status))) {
+        if (!__all_sync(0xffffffffu, e_ok && mbar_wait(&pv_done[gl & 3], (gl >> 2) & 1, p.status))) {
           ok = false;
           break;
         }
