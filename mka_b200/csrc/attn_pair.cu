@@ -50,20 +50,29 @@ constexpr int kBN = 128;        // keys per tile
 constexpr int kHeadDim = 128;
 constexpr int kThreads = 384;
 constexpr int kAhead = 3;       // key tiles that K is loaded ahead of V
-constexpr int kKStages = 5;
-constexpr int kVStages = 5;
+constexpr int kKStages = 4;
+constexpr int kVStages = 4;
 constexpr int kQBytes = 32768;   // 128 rows x 128 channels
 constexpr int kQHalf = 16384;    // 64 channels
 constexpr int kKBytes = 16384;   // 64 keys x 128 channels
 constexpr int kVBytes = 16384;   // 128 keys x 64 channels
-constexpr int kTileSmem = 2 * kQBytes + kKStages * kKBytes + kVStages * kVBytes;
+constexpr int kStageBytes = 8 * 4096;  // 4 KB per softmax warp
+constexpr int kTileSmem = 2 * kQBytes + kKStages * kKBytes + kVStages * kVBytes + kStageBytes;
 constexpr int kSmemBytes = kTileSmem + 3072;
+#ifndef FMKA_PE
+#define FMKA_PE 100
+#endif
+constexpr int kPolyEvery = FMKA_PE;   // one pair of exponentials in so many runs on the FMA pipe
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr uint32_t kTmemO = 0, kTmemS = 128, kTmemP = 384;  // S: 2 x 128 columns, P: 2 x 64
 // Register split between the control warps and the softmax warps (setmaxnreg);
 // the sum has to fit in what the block is launched with.
-constexpr int kRegsControl = 72;
-constexpr int kRegsSoftmax = 216;
+#ifndef FMKA_RC
+#define FMKA_RC 72
+#define FMKA_RS 216
+#endif
+constexpr int kRegsControl = FMKA_RC;
+constexpr int kRegsSoftmax = FMKA_RS;
 constexpr int kMinLaunchRegs = (128 * kRegsControl + 256 * kRegsSoftmax + kThreads - 1) / kThreads;
 
 struct PairItem {
@@ -186,7 +195,23 @@ struct Ring {
   }
 };
 
-__device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
+// 2^x for a pair on the FMA pipe: x = n + f with n = round(x), 2^f on [-1/2, 1/2] from a degree-5 polynomial fitted
+// here by Remez exchange on the relative error (7.5e-8 in exact arithmetic, 2.1e-7 in fp32, about what ex2.approx
+// has), times 2^n built from the exponent bits. Below -126.5 that factor is zero; NaN stays NaN.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float2 c = make_float2(fmax_nan(x.x, -127.0f), fmax_nan(x.y, -127.0f));
+  const float2 t = fadd2(c, make_float2(12582912.0f, 12582912.0f));
+  const float2 n = fadd2(t, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), c);
+  float2 p = ffma2(make_float2(1.3276472e-3f, 1.3276472e-3f), f, make_float2(9.675541e-3f, 9.675541e-3f));
+  p = ffma2(p, f, make_float2(5.5507133e-2f, 5.5507133e-2f));
+  p = ffma2(p, f, make_float2(0.24022120f, 0.24022120f));
+  p = ffma2(p, f, make_float2(0.69314697f, 0.69314697f));
+  p = ffma2(p, f, make_float2(1.0000001f, 1.0000001f));
+  const float2 e = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3F800000),
+                               __int_as_float((__float_as_int(t.y) << 23) + 0x3F800000));
+  return fmul2(p, e);
+}
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     attn_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -195,8 +220,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + 2 * kQBytes;
   uint8_t* sV = sK + kKStages * kKBytes;
-  float* s_m = reinterpret_cast<float*>(sV + kVStages * kVBytes);  // [2][128] running maximum after even / odd tiles
-  float* s_l = s_m + 256;                                           // [2][128] sums handed on at an item's end
+  uint8_t* sStage = sV + kVStages * kVBytes;
+  float* s_m = reinterpret_cast<float*>(sStage + kStageBytes);  // [128] running maximum
+  float* s_l = s_m + 128;                                           // [2][128] sums handed on at an item's end
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + 256);
   uint64_t* q_full = bars;                 // [2] even CTA
   uint64_t* q_empty = q_full + 2;          // [2] both
@@ -216,7 +242,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* bad_v = abort_flag + 1;    // [8] by item number: 1 + the last item with taken-out values
-  static_assert(1024 * 2 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 6 + 4 + 1 + 24 + 2) + 40 <= 3072,
+  static_assert(512 * 3 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 6 + 4 + 1 + 24 + 2) + 40 <= 3072,
                 "control block fits behind the tiles");
 
   const int warp = __shfl_sync(0xffffffffu, warp_id(), 0);
@@ -469,7 +495,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             *at = x;
           }
           if (__any_sync(0xffffffffu, bad) && lane == 0) {
-            // the gate is at most five tiles ahead of the products, so eight slots never meet
+            // the gate is at most four tiles ahead of the products, so eight slots never meet
             bad_v[item & 7] = item;
             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(bad_peer + 4 * (item & 7)), "r"(item) : "memory");
           }
@@ -495,6 +521,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t o_free_even = cluster_addr(o_free, 0);
     const int ri = r / p.Gs, rg = r - ri * p.Gs;  // token of the CTA's tile, head of the slice
     const int ti = (int)rank * p.tpt + ri;         // token of the pair's tile
+    const uint32_t s_col = kTmemS + wg * 128, p_col = kTmemP + wg * 64;
     int g0 = 0;                                    // tiles before this item
     int items = 0;                                 // items with tiles before this one
     int gave = 0, took = 0;                        // sums handed to / by the other warpgroup so far
@@ -518,14 +545,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // Last visible key. Rows that are not there (behind the last token, or the last rows where the group does not
       // divide 128) multiply whatever their Q holds; nothing of theirs is stored or has a say in the rescaling.
       const int lim = row_ok ? min(it.ke - 1, it.lim0 + ti) : 0x3FFFFFFF;
+      // keys that every row of this CTA sees (from the first one on)
+      const int rows_see = min(it.ke, max(it.kb, it.lim0 + 1 + (int)rank * p.tpt));
       const int last_wg = (g0 + n - 1) & 1;
       float m_own = -INFINITY, m_prev = -INFINITY, l = 0.f;
+      // from this tile on, some row of this CTA does not see every key
+      const int first_masked = (rows_see - it.kb) / kBN;
       for (int j = (g0 & 1) == wg ? 0 : 1; j < n; j += 2) {
         const int g = g0 + j;  // g & 1 == wg
-        const uint32_t s_col = kTmemS + wg * 128, p_col = kTmemP + wg * 64;
-        if (!(ok = warp_wait(&s_full[wg], (g >> 1) & 1, p.status))) break;
+        if (!(ok = warp_ready(&s_full[wg], (g >> 1) & 1) || warp_wait(&s_full[wg], (g >> 1) & 1, p.status))) break;
         tc_fence_after();
-        const int kbase = it.kb + j * kBN;
         uint32_t s[128];
         tmem_ld32(lane_addr + s_col + 0, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
         tmem_ld32(lane_addr + s_col + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
@@ -535,8 +564,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_cta(s_free_even);
-        const int seen = lim - kbase;  // last visible column of the tile
-        if (__any_sync(0xffffffffu, seen < kBN - 1)) {
+        if (j >= first_masked) {
+          const int seen = lim - it.kb - j * kBN;  // last visible column of the tile
           const int all_see = __reduce_min_sync(0xffffffffu, seen);
 #pragma unroll
           for (int c0 = 0; c0 < 128; c0 += 16) {
@@ -557,9 +586,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         const float mx = p.scale_log2 * fmax3(fmax3(mxa[0], mxa[1], mxa[2]), fmax3(mxa[3], mxa[4], mxa[5]),
                                               fmaxf(mxa[6], mxa[7]));
-        // the maximum after the tile before (the other warpgroup's, same rows)
-        if (g > 0 && !(ok = warp_wait(&m_bar[(wg ^ 1) * 4 + quarter], ((g - 1) >> 1) & 1, p.status))) break;
-        float m_ref = j > 0 ? s_m[(wg ^ 1) * 128 + r] : -INFINITY;
+        // The maximum after the tile before (the other warpgroup's, same rows), and this warpgroup's P buffer (its
+        // last P has been multiplied): one poll for both, which are there in the long run.
+        if (g > 0) {
+          uint64_t* mb = &m_bar[(wg ^ 1) * 4 + quarter];
+          uint64_t* pb = &pv_done[(g - 2) & 3];
+          const uint32_t m_ph = ((g - 1) >> 1) & 1, p_ph = ((g - 2) >> 2) & 1;
+          if (!__all_sync(0xffffffffu, mbar_try_wait(mb, m_ph) && (g == 1 || mbar_try_wait(pb, p_ph)))) {
+            if (!(ok = warp_wait(mb, m_ph, p.status) && (g == 1 || warp_wait(pb, p_ph, p.status)))) break;
+          }
+        }
+        float m_ref = j > 0 ? s_m[r] : -INFINITY;
         m_prev = m_ref;
         float alpha = 1.f;
         const bool grow = __any_sync(0xffffffffu, row_ok && mx > m_ref + kRescaleThreshold);
@@ -568,11 +605,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           alpha = m_new == m_ref ? 1.f : fast_exp2(m_ref - m_new);
           m_ref = m_new;
         }
-        s_m[wg * 128 + r] = m_ref;
+        if (grow || j == 0) s_m[r] = m_ref;
         __syncwarp();
         if (lane == 0) mbar_arrive(&m_bar[wg * 4 + quarter]);
-        // this warpgroup's last P has been multiplied, so its buffer is free
-        if (g > 1 && !(ok = warp_wait(&pv_done[(g - 2) & 3], ((g - 2) >> 2) & 1, p.status))) break;
         if (grow && j > 0) {
           // O holds the tiles before this one: wait for the last product, then move O to the new maximum. (No phase
           // of the barrier is skipped: the other warpgroup has waited for tile g - 5 before it wrote P of tile g - 3,
@@ -603,7 +638,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int c = 0; c < 16; ++c) {
             const float2 xx =
                 ffma2(make_float2(__uint_as_float(sc[2 * c]), __uint_as_float(sc[2 * c + 1])), sl2, nm2);
-            const float2 pp = exp2_pair(xx);
+            const float2 pp =
+                (c % kPolyEvery) == kPolyEvery - 1 ? exp2_poly(xx) : make_float2(fast_exp2(xx.x), fast_exp2(xx.y));
             acc[c & 3] = fadd2(acc[c & 3], pp);
             pk[c] = pack_bf16x2(pp.x, pp.y);
           }
@@ -655,48 +691,77 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const float L = l + l_other * (m_prev == m_own ? 1.f : fast_exp2(m_prev - m_own));
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const float lse2 = L == 0.f ? -INFINITY : m_own + __log2f(L);
-        if (row_ok) {
-          const int tok = it.q0 + ti, head = it.hkv * p.G + it.g0 + rg;
-          const int j0 = max(it.kb, it.lim0 + 1);  // keys before this one are seen by every row
+        // Rows go out through 4 KB of staging per warp, so that a store instruction writes whole 128-byte lines (a
+        // thread storing its own row touches 32 lines with 16 bytes each: 6000 cycles an item).
+        const bool direct = it.part < 0;
+        const bool live = row_ok && (direct || L != 0.f);  // a part without a visible key leaves only its -inf
+        const int tok = it.q0 + ti, head = it.hkv * p.G + it.g0 + rg;
+        const int64_t rec = it.part + (int64_t)ti * it.part_ts + rg;
+        const int64_t row_off = direct ? tok * p.o_st + head * p.o_sh : rec * kHeadDim;  // elements
+        const unsigned rows_live = __ballot_sync(0xffffffffu, live);
+        uint8_t* stage = sStage + (wg * 4 + quarter) * 4096;
+        uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
+        const int sub = lane >> 3, ch = lane & 7;
+        uint8_t* base = direct ? reinterpret_cast<uint8_t*>(p.o) : reinterpret_cast<uint8_t*>(p.part_o);
+        auto flush = [&](int pass) {  // 128 bytes of every row, `pass` x 128 bytes into it
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int rr = k * 4 + sub;
+            const int64_t off = __shfl_sync(0xffffffffu, row_off, rr);
+            if (rows_live >> rr & 1)
+              *reinterpret_cast<uint4*>(base + off * (direct ? 2 : 4) + pass * 128 + ch * 16) =
+                  *reinterpret_cast<const uint4*>(stage + rr * 128 + ((ch ^ (rr & 7)) << 4));
+          }
+          __syncwarp();
+        };
+        if (direct) {
+#pragma unroll
+          for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint32_t* x = o + pass * 64 + c * 8;
+              uint4 w4;
+              w4.x = pack_bf16x2(__uint_as_float(x[0]) * inv, __uint_as_float(x[1]) * inv);
+              w4.y = pack_bf16x2(__uint_as_float(x[2]) * inv, __uint_as_float(x[3]) * inv);
+              w4.z = pack_bf16x2(__uint_as_float(x[4]) * inv, __uint_as_float(x[5]) * inv);
+              w4.w = pack_bf16x2(__uint_as_float(x[6]) * inv, __uint_as_float(x[7]) * inv);
+              mine[c ^ (lane & 7)] = w4;
+            }
+            flush(pass);
+          }
+          if (row_ok && p.lse != nullptr) p.lse[tok * p.lse_st + head * p.lse_sh] = lse2 * 0.69314718055994531f;
+        } else {
+#pragma unroll
+          for (int pass = 0; pass < 4; ++pass) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint32_t* x = o + pass * 32 + c * 4;
+              mine[c ^ (lane & 7)] = make_uint4(__float_as_uint(__uint_as_float(x[0]) * inv),
+                                                __float_as_uint(__uint_as_float(x[1]) * inv),
+                                                __float_as_uint(__uint_as_float(x[2]) * inv),
+                                                __float_as_uint(__uint_as_float(x[3]) * inv));
+            }
+            flush(pass);
+          }
+          if (row_ok) p.part_lse[rec] = lse2;
+        }
+        if (bad && live) {
+          // rare: values that the V gate took out go to the rows that see them (the row's stores by other lanes come
+          // first: they are ordered by the barrier after them)
           const __nv_bfloat16* vrow = p.v + (int64_t)it.k0 * p.kv_st + it.hkv * p.kv_sh;
-          if (it.part < 0) {
-            __nv_bfloat16* dst = p.o + tok * p.o_st + head * p.o_sh;
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              uint4 w;
-              w.x = pack_bf16x2(__uint_as_float(o[c * 8 + 0]) * inv, __uint_as_float(o[c * 8 + 1]) * inv);
-              w.y = pack_bf16x2(__uint_as_float(o[c * 8 + 2]) * inv, __uint_as_float(o[c * 8 + 3]) * inv);
-              w.z = pack_bf16x2(__uint_as_float(o[c * 8 + 4]) * inv, __uint_as_float(o[c * 8 + 5]) * inv);
-              w.w = pack_bf16x2(__uint_as_float(o[c * 8 + 6]) * inv, __uint_as_float(o[c * 8 + 7]) * inv);
-              reinterpret_cast<uint4*>(dst)[c] = w;
-            }
-            if (p.lse != nullptr) p.lse[tok * p.lse_st + head * p.lse_sh] = lse2 * 0.69314718055994531f;
-            if (bad) {
-              // rare: values that the V gate took out go to the rows that see them
-              for (int key = j0; key <= lim; ++key)
-                for (int d = 0; d < kHeadDim; ++d) {
-                  const float x = __bfloat162float(vrow[key * p.kv_st + d]);
-                  if (!(fabsf(x) <= 3.4e38f)) dst[d] = __float2bfloat16(__bfloat162float(dst[d]) + x);
-                }
-            }
-          } else {
-            const int64_t rec = it.part + (int64_t)ti * it.part_ts + rg;
-            if (L != 0.f) {
-              float* dst = p.part_o + rec * kHeadDim;
-#pragma unroll
-              for (int c = 0; c < 32; ++c)
-                reinterpret_cast<float4*>(dst)[c] =
-                    make_float4(__uint_as_float(o[c * 4]) * inv, __uint_as_float(o[c * 4 + 1]) * inv,
-                                __uint_as_float(o[c * 4 + 2]) * inv, __uint_as_float(o[c * 4 + 3]) * inv);
-              if (bad) {
-                for (int key = j0; key <= lim; ++key)
-                  for (int d = 0; d < kHeadDim; ++d) {
-                    const float x = __bfloat162float(vrow[key * p.kv_st + d]);
-                    if (!(fabsf(x) <= 3.4e38f)) dst[d] += x;
-                  }
+          for (int key = max(it.kb, it.lim0 + 1); key <= lim; ++key) {
+#pragma unroll 1
+            for (int d = 0; d < kHeadDim; ++d) {
+              const float x = __bfloat162float(vrow[key * p.kv_st + d]);
+              if (fabsf(x) <= 3.4e38f) continue;
+              if (direct) {
+                __nv_bfloat16* y = p.o + row_off + d;
+                *y = __float2bfloat16(__bfloat162float(*y) + x);
+              } else {
+                p.part_o[row_off + d] += x;
               }
             }
-            p.part_lse[rec] = lse2;
           }
         }
       }

@@ -413,9 +413,39 @@ __device__ __forceinline__ bool elect_one() {
   return ok != 0;
 }
 
-// Bounded wait of a whole warp, with a warp-uniform result.
+// Bounded wait like mbar_wait that lets the warp sleep in the barrier (up to 1 ms
+// a try) instead of polling: polling warps take issue slots from the others of
+// their scheduler.
+__device__ __forceinline__ bool mbar_sleep(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  const uint32_t a = smem_u32(bar);
+  uint64_t t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (ok) return true;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      if (status) atomicOr(status, kStatusWaitTimeout);
+      return false;
+    }
+  }
+}
+
+// The same for a whole warp, with a warp-uniform result.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+  return __all_sync(0xffffffffu, mbar_sleep(bar, parity, status));
+}
+
+// Whether the phase is complete, for a whole warp, without waiting long.
+__device__ __forceinline__ bool warp_ready(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
 }
 
 // Programmatic dependent launch: waits until the kernels before this one in the
@@ -508,6 +538,14 @@ __device__ __forceinline__ bool zero_nonfinite(uint4& c) {
 // Packed fp32 pair arithmetic (sm_100a): one instruction for two lanes of work.
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+
+// Maximum that passes NaN on (fmaxf drops it).
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 
 // Three-input maximum (one instruction on sm_100a).
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
