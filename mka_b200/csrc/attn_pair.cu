@@ -86,6 +86,21 @@ struct PairItem {
   int part_ts;     // partial rows per token
 };
 
+// Division by a number known on the host: q = (umulhi(n, m) + n) >> s for 0 <= n < 2^31.
+struct FastDiv {
+  uint32_t m, s;
+  int d;
+  static FastDiv of(int d) {
+    FastDiv f;
+    f.d = d;
+    f.s = 0;
+    while ((1ll << f.s) < d) ++f.s;
+    f.m = (uint32_t)(((1ull << 32) * ((1ull << f.s) - (uint64_t)d)) / (uint64_t)d + 1);
+    return f;
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)((__umulhi((uint32_t)n, m) + (uint32_t)n) >> s); }
+};
+
 struct PairParams {
   __nv_bfloat16* o;
   int64_t o_st, o_sh;
@@ -95,6 +110,7 @@ struct PairParams {
   int64_t kv_st, kv_sh;
   int Hq, G, Gs, n_gs, nh;   // nh = kv heads x group slices
   int tpt;                   // tokens per CTA
+  FastDiv by_nh, by_ngs, by_nrt;
   float scale_log2;
   const int* header;         // [0] list entries; null: uniform items
   const int4* list;          // {q0, nq, k0, kb}, {ke, lim0, part, 0}
@@ -124,7 +140,7 @@ struct ItemWalk {
     idx = pair_item_index(r, pair, pairs);
     if (idx >= n_items) idx = r * pairs >= n_items ? -1 : -2;  // -1: past the end, -2: none in this round
     if (idx >= 0 && p.header != nullptr) {
-      const int li = idx / p.nh;
+      const int li = p.by_nh.div(idx);
       a = __ldcg(p.list + 2 * li);
       b = __ldcg(p.list + 2 * li + 1);
     }
@@ -140,8 +156,8 @@ struct ItemWalk {
       const int i = idx;
       if (i == -1) return false;
       if (i >= 0) {
-        const int li = i / p.nh, h = i - li * p.nh;
-        it.hkv = h / p.n_gs;
+        const int li = p.by_nh.div(i), h = i - li * p.nh;
+        it.hkv = p.by_ngs.div(h);
         it.g0 = (h - it.hkv * p.n_gs) * p.Gs;
         it.gn = min(p.Gs, p.G - it.g0);
         if (p.header != nullptr) {
@@ -156,7 +172,7 @@ struct ItemWalk {
           it.part = part < 0 ? -1 : (int64_t)part + (int64_t)h * it.nq * p.Gs;
           it.part_ts = p.Gs;
         } else {
-          const int split = li / p.n_rt, rt = li - split * p.n_rt;
+          const int split = p.by_nrt.div(li), rt = li - split * p.n_rt;
           it.q0 = rt * 2 * p.tpt;
           it.nq = min(2 * p.tpt, p.B - it.q0);
           it.k0 = 0;
@@ -318,16 +334,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     PairItem ki, vi;
     kw.start(p, n_items, pair, pairs);
     vw = kw;
-    bool k_more = kw.next(p, pair, pairs, ki, false), v_more = vw.next(p, pair, pairs, vi, false);
-    int kj = 0, vj = 0, ahead = 0, gk = 0, gv = 0, k_items = 0;
+    int kj = 0, vj = 0, ahead = 0, gk = 0, gv = 0, k_items = -1;
+    ki.n = vi.n = 0;
+    bool k_more = true;
     Ring<kKStages> kr;
     Ring<kVStages> vr;
     bool ok = true;
-    while (ok && v_more) {
+    while (ok) {
       while (k_more && ahead < kAhead) {
-        if (kj == 0) {
+        if (kj == ki.n) {
+          if (!(k_more = kw.next(p, pair, pairs, ki, false))) break;
+          kj = 0;
+          ++k_items;
           const int qs = k_items & 1;
-          if (!(ok = warp_wait(&q_empty[qs], ((k_items >> 1) & 1) ^ 1u, p.status))) break;
+          if (!(ok = !__any_sync(0xffffffffu, *abort_flag) &&
+                     warp_wait(&q_empty[qs], ((k_items >> 1) & 1) ^ 1u, p.status))) break;
           if (elect_one()) {
             if (rank == 0) mbar_arrive_expect_tx(&q_full[qs], 4 * q_box);
             const int tok = ki.q0 + (int)rank * p.tpt;
@@ -347,15 +368,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         ++gk;
         ++ahead;
+        ++kj;
         kr.step();
-        if (++kj == ki.n) {
-          kj = 0;
-          ++k_items;
-          k_more = kw.next(p, pair, pairs, ki, false);
-          if (__any_sync(0xffffffffu, *abort_flag)) ok = false;
-        }
       }
-      if (!ok || !(ok = warp_wait(&v_empty[vr.s], vr.ph ^ 1u, p.status))) break;
+      if (!ok) break;
+      if (vj == vi.n) {
+        if (!vw.next(p, pair, pairs, vi, false)) break;
+        vj = 0;
+      }
+      if (!(ok = warp_wait(&v_empty[vr.s], vr.ph ^ 1u, p.status))) break;
       if (elect_one()) {
         mbar_arrive_expect_tx(&v_land[vr.s], kVBytes);
         tma_load_3d(sV + vr.s * kVBytes, &tmV, &v_land[vr.s], 64 * (int)rank, vi.k0 + vi.kb + vj * kBN, vi.hkv);
@@ -363,18 +384,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       __syncwarp();
       ++gv;
       --ahead;
+      ++vj;
       vr.step();
-      if (++vj == vi.n) {
-        vj = 0;
-        v_more = vw.next(p, pair, pairs, vi, false);
-      }
     }
     if (!ok) *abort_flag = 1;
     // Drain: every load has landed, and its tile has been consumed, before the CTA goes.
+#pragma unroll 1
     for (int g = gv - 1; g >= 0 && g >= gv - kVStages; --g)
-      mbar_wait(&v_land[g % kVStages], (g / kVStages) & 1, p.status);
+      mbar_sleep(&v_land[g % kVStages], (g / kVStages) & 1, p.status);
+#pragma unroll 1
     for (int g = gk - 1; g >= 0 && g >= gk - kKStages; --g)
-      mbar_wait(&k_empty[g % kKStages], (g / kKStages) & 1, p.status);
+      mbar_sleep(&k_empty[g % kKStages], (g / kKStages) & 1, p.status);
   } else if (warp == 1) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
     // ----------------------------------- S = Q K^T (the even CTA issues) --
@@ -392,6 +412,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       while (ok && w.next(p, pair, pairs, it, false)) {
         if (!(ok = warp_wait(&q_full[qr.s], qr.ph, p.status))) break;
         const uint64_t qd = q_desc + (uint64_t)(qr.s * (kQBytes >> 4));
+#pragma unroll 1
         for (int j = 0; j < it.n; ++j) {
           // the K tile, and the S buffer (its last scores are in registers)
           if (!(ok = warp_wait(&k_full[kr.s], kr.ph, p.status) && warp_wait(&s_free[sr.s], sr.ph ^ 1u, p.status))) break;
@@ -418,7 +439,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok) *abort_flag = 1;
       if (elect_one()) tc_commit_pair(&mma_done[0], 0x1);
       __syncwarp();
-      mbar_wait(&mma_done[0], 0, p.status);
+      mbar_sleep(&mma_done[0], 0, p.status);
     }
   } else if (warp == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
@@ -438,6 +459,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       while (ok && w.next(p, pair, pairs, it, false)) {
         if (!(ok = warp_wait(o_free, o_phase, p.status))) break;
         o_phase ^= 1u;
+#pragma unroll 1
         for (int j = 0; j < it.n; ++j) {
           // a tile that the gates may have written to is acquired from the other CTA as well
           ok = rows_all_see(it, j) < kBN ? __all_sync(0xffffffffu, mbar_wait_cluster(&v_ready[vr.s], vr.ph, p.status))
@@ -464,7 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!ok) *abort_flag = 1;
       if (elect_one()) tc_commit_pair(&mma_done[1], 0x1);
       __syncwarp();
-      mbar_wait(&mma_done[1], 0, p.status);
+      mbar_sleep(&mma_done[1], 0, p.status);
     }
   } else if (warp == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
@@ -477,6 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Ring<kVStages> vr;
     bool ok = true;
     for (int item = 1; ok && w.next(p, pair, pairs, it, false); ++item) {
+#pragma unroll 1
       for (int j = 0; j < it.n; ++j) {
         if (!(ok = warp_wait(&v_land[vr.s], vr.ph, p.status))) break;
         const int live = min(kBN, it.ke - it.kb - j * kBN);  // rows that hold keys
@@ -484,6 +507,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (some < kBN) {
           // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes four rows at a time
           bool bad = false;
+#pragma unroll 1
           for (int row = some + (lane >> 3); row < kBN; row += 4) {
             uint4* at = reinterpret_cast<uint4*>(sV + vr.s * kVBytes + row * 128 + (lane & 7) * 16);
             uint4 x = make_uint4(0, 0, 0, 0);
@@ -551,9 +575,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       float m_own = -INFINITY, m_prev = -INFINITY, l = 0.f;
       // from this tile on, some row of this CTA does not see every key
       const int first_masked = (rows_see - it.kb) / kBN;
+#pragma unroll 1
       for (int j = (g0 & 1) == wg ? 0 : 1; j < n; j += 2) {
         const int g = g0 + j;  // g & 1 == wg
-        if (!(ok = warp_ready(&s_full[wg], (g >> 1) & 1) || warp_wait(&s_full[wg], (g >> 1) & 1, p.status))) break;
+        if (!(ok = warp_wait(&s_full[wg], (g >> 1) & 1, p.status))) break;
         tc_fence_after();
         uint32_t s[128];
         tmem_ld32(lane_addr + s_col + 0, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
@@ -666,90 +691,82 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       } else {
         // ---- epilogue: O of all tiles, both sums ----
         const int gl = g0 + n - 1;
-        bool e_ok = true;
         float l_other = 0.f;  // at m_prev, the maximum after the tile before the last
         if (n >= 2) {
-          e_ok = mbar_wait(&l_bar[((wg ^ 1) * 2 + (took & 1)) * 4 + quarter], (took >> 1) & 1, p.status);
+          if (!(ok = warp_wait(&l_bar[((wg ^ 1) * 2 + (took & 1)) * 4 + quarter], (took >> 1) & 1, p.status))) break;
           l_other = s_l[(took & 1) * 128 + r];
           ++took;
         }
-        if (!__all_sync(0xffffffffu, e_ok && mbar_wait(&pv_done[gl & 3], (gl >> 2) & 1, p.status))) {
-          ok = false;
-          break;
-        }
+        if (!(ok = warp_wait(&pv_done[gl & 3], (gl >> 2) & 1, p.status))) break;
         tc_fence_after();
         const bool bad = bad_v[(items + 1) & 7] == items + 1;
-        uint32_t o[128];
-        tmem_ld32(lane_addr + kTmemO + 0, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
-        tmem_ld32(lane_addr + kTmemO + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
-        tmem_ld32(lane_addr + kTmemO + 64, *reinterpret_cast<uint32_t(*)[32]>(&o[64]));
-        tmem_ld32(lane_addr + kTmemO + 96, *reinterpret_cast<uint32_t(*)[32]>(&o[96]));
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster_cta(o_free_even);
         const float L = l + l_other * (m_prev == m_own ? 1.f : fast_exp2(m_prev - m_own));
         const float inv = L == 0.f ? 0.f : 1.f / L;
         const float lse2 = L == 0.f ? -INFINITY : m_own + __log2f(L);
         // Rows go out through 4 KB of staging per warp, so that a store instruction writes whole 128-byte lines (a
-        // thread storing its own row touches 32 lines with 16 bytes each: 6000 cycles an item).
+        // thread storing its own row touches 32 lines with 16 bytes each). The loops stay rolled: this code runs once
+        // an item, and what it costs is mostly being fetched.
         const bool direct = it.part < 0;
         const bool live = row_ok && (direct || L != 0.f);  // a part without a visible key leaves only its -inf
         const int tok = it.q0 + ti, head = it.hkv * p.G + it.g0 + rg;
         const int64_t rec = it.part + (int64_t)ti * it.part_ts + rg;
         const int64_t row_off = direct ? tok * p.o_st + head * p.o_sh : rec * kHeadDim;  // elements
         const unsigned rows_live = __ballot_sync(0xffffffffu, live);
+        uint8_t* row_out = (direct ? reinterpret_cast<uint8_t*>(p.o) : reinterpret_cast<uint8_t*>(p.part_o)) +
+                           row_off * (direct ? 2 : 4) + (lane & 7) * 16;
+        const int sub = lane >> 3;
         uint8_t* stage = sStage + (wg * 4 + quarter) * 4096;
-        uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
-        const int sub = lane >> 3, ch = lane & 7;
-        uint8_t* base = direct ? reinterpret_cast<uint8_t*>(p.o) : reinterpret_cast<uint8_t*>(p.part_o);
-        auto flush = [&](int pass) {  // 128 bytes of every row, `pass` x 128 bytes into it
-          __syncwarp();
+#pragma unroll 1
+        for (int pass = 0; pass < 4; ++pass) {  // 32 channels
+          uint32_t o[32];
+          tmem_ld32(lane_addr + kTmemO + pass * 32, o);
+          tmem_wait_ld();
+          if (pass == 3) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_cta(o_free_even);
+          }
+          uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int rr = k * 4 + sub;
-            const int64_t off = __shfl_sync(0xffffffffu, row_off, rr);
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * inv);
+          if (direct) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t w4[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w4[e] = pack_bf16x2(__uint_as_float(o[c * 8 + 2 * e]), __uint_as_float(o[c * 8 + 2 * e + 1]));
+              mine[((pass & 1) * 4 + c) ^ (lane & 7)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+            }
+            if (!(pass & 1)) continue;
+          } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              mine[c ^ (lane & 7)] = make_uint4(o[c * 4], o[c * 4 + 1], o[c * 4 + 2], o[c * 4 + 3]);
+          }
+          __syncwarp();
+          const int line = direct ? pass >> 1 : pass;  // 128 bytes of every row
+#pragma unroll 2
+          for (int rr = sub; rr < 32; rr += 4) {
+            // the row's address, with the chunk of the lane it came from: lane rr holds chunk rr & 7
+            uint8_t* dst = reinterpret_cast<uint8_t*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row_out), rr));
             if (rows_live >> rr & 1)
-              *reinterpret_cast<uint4*>(base + off * (direct ? 2 : 4) + pass * 128 + ch * 16) =
-                  *reinterpret_cast<const uint4*>(stage + rr * 128 + ((ch ^ (rr & 7)) << 4));
+              *reinterpret_cast<uint4*>(dst + line * 128 + ((lane & 7) - (rr & 7)) * 16) =
+                  *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
           }
           __syncwarp();
-        };
+        }
         if (direct) {
-#pragma unroll
-          for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const uint32_t* x = o + pass * 64 + c * 8;
-              uint4 w4;
-              w4.x = pack_bf16x2(__uint_as_float(x[0]) * inv, __uint_as_float(x[1]) * inv);
-              w4.y = pack_bf16x2(__uint_as_float(x[2]) * inv, __uint_as_float(x[3]) * inv);
-              w4.z = pack_bf16x2(__uint_as_float(x[4]) * inv, __uint_as_float(x[5]) * inv);
-              w4.w = pack_bf16x2(__uint_as_float(x[6]) * inv, __uint_as_float(x[7]) * inv);
-              mine[c ^ (lane & 7)] = w4;
-            }
-            flush(pass);
-          }
           if (row_ok && p.lse != nullptr) p.lse[tok * p.lse_st + head * p.lse_sh] = lse2 * 0.69314718055994531f;
-        } else {
-#pragma unroll
-          for (int pass = 0; pass < 4; ++pass) {
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const uint32_t* x = o + pass * 32 + c * 4;
-              mine[c ^ (lane & 7)] = make_uint4(__float_as_uint(__uint_as_float(x[0]) * inv),
-                                                __float_as_uint(__uint_as_float(x[1]) * inv),
-                                                __float_as_uint(__uint_as_float(x[2]) * inv),
-                                                __float_as_uint(__uint_as_float(x[3]) * inv));
-            }
-            flush(pass);
-          }
-          if (row_ok) p.part_lse[rec] = lse2;
+        } else if (row_ok) {
+          p.part_lse[rec] = lse2;
         }
         if (bad && live) {
           // rare: values that the V gate took out go to the rows that see them (the row's stores by other lanes come
           // first: they are ordered by the barrier after them)
           const __nv_bfloat16* vrow = p.v + (int64_t)it.k0 * p.kv_st + it.hkv * p.kv_sh;
+#pragma unroll 1
           for (int key = max(it.kb, it.lim0 + 1); key <= lim; ++key) {
 #pragma unroll 1
             for (int d = 0; d < kHeadDim; ++d) {
@@ -1026,9 +1043,13 @@ void pair_tile(PairParams& p) {
   p.nh = (p.Hq / p.G) * p.n_gs;
 }
 
-int launch_pair(const PairParams& p, const __nv_bfloat16* q, int64_t q_rows, int64_t q_st, int64_t q_sh,
+int launch_pair(const PairParams& given, const __nv_bfloat16* q, int64_t q_rows, int64_t q_st, int64_t q_sh,
                 const __nv_bfloat16* k, const __nv_bfloat16* v, int64_t kv_rows, int64_t kv_st, int64_t kv_sh,
                 int pairs, bool dependent, cudaStream_t stream, const char* what) {
+  PairParams p = given;
+  p.by_nh = FastDiv::of(p.nh);
+  p.by_ngs = FastDiv::of(p.n_gs);
+  p.by_nrt = FastDiv::of(std::max(p.n_rt, 1));
   CUtensorMap tmQ, tmK, tmV;
   int rc = rows_map(&tmQ, q, q_rows, q_st, p.Hq, q_sh, p.Gs, p.tpt, true);
   if (rc) return rc;

@@ -376,27 +376,23 @@ __device__ __forceinline__ void umma_ts_pair(uint32_t d_tmem, uint32_t a_tmem, u
 // that the pair's other CTA has written (about 400 cycles more than mbar_wait).
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* status) {
   const uint32_t a = smem_u32(bar);
-  uint64_t t0 = 0;
-  uint32_t spins = 0;
+  uint32_t t0 = 0, now, ok;
+#pragma unroll 1
   while (true) {
-    uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.b32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(a), "r"(parity)
+        : "r"(a), "r"(parity), "r"(1000000u)
         : "memory");
     if (ok) return true;
-    if ((++spins & 63u) == 0u) {
-      const uint64_t now = globaltimer_ns();
-      if (t0 == 0) t0 = now;
-      if (now - t0 > kWaitLimitNs) {
-        if (status) atomicOr(status, kStatusWaitTimeout);
-        return false;
-      }
-    }
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(now));
+    if (t0 == 0) t0 = now;
+    if (now - t0 > (uint32_t)kWaitLimitNs) break;
   }
+  if (status) atomicOr(status, kStatusWaitTimeout);
+  return false;
 }
 
 // One lane of the (converged) warp. Code around it stays warp-uniform, so that
@@ -415,12 +411,13 @@ __device__ __forceinline__ bool elect_one() {
 
 // Bounded wait like mbar_wait that lets the warp sleep in the barrier (up to 1 ms
 // a try) instead of polling: polling warps take issue slots from the others of
-// their scheduler.
+// their scheduler. Little code, because it is inlined at every wait (the low
+// word of the timer wraps after 4.29 s, twice the budget).
 __device__ __forceinline__ bool mbar_sleep(uint64_t* bar, uint32_t parity, uint32_t* status) {
   const uint32_t a = smem_u32(bar);
-  uint64_t t0 = 0;
+  uint32_t t0 = 0, now, ok;
+#pragma unroll 1
   while (true) {
-    uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -429,13 +426,12 @@ __device__ __forceinline__ bool mbar_sleep(uint64_t* bar, uint32_t parity, uint3
         : "r"(a), "r"(parity), "r"(1000000u)
         : "memory");
     if (ok) return true;
-    const uint64_t now = globaltimer_ns();
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(now));
     if (t0 == 0) t0 = now;
-    if (now - t0 > kWaitLimitNs) {
-      if (status) atomicOr(status, kStatusWaitTimeout);
-      return false;
-    }
+    if (now - t0 > (uint32_t)kWaitLimitNs) break;
   }
+  if (status) atomicOr(status, kStatusWaitTimeout);
+  return false;
 }
 
 // The same for a whole warp, with a warp-uniform result.
