@@ -19,7 +19,7 @@
 // waits for the chain S -> softmax -> P V -> next S of a tile. (With P written
 // over S, three S buffers and that chain, a tile took 1700 cycles.)
 //
-// Warp roles (12 warps per CTA):
+// Warp roles (16 warps per CTA):
 //   warp 0      producer: Q, K, V tiles by TMA (128-byte swizzle)
 //   warp 1      issues S = Q K^T (the even CTA's, for both), ahead of P V and
 //               across item borders
@@ -30,12 +30,15 @@
 //               it first puts zeros over the rows past the last key and over
 //               infinities and NaNs in rows that only some queries see, because
 //               a zero weight times such a value would not be zero
-//   warps 4-7, 8-11  softmax of the even / odd key tiles, thread = row. The
+//   warps 4-7   output: O of a finished item from TMEM, divided by the joined sums,
+//               while the softmax warps are already in the next item (when the
+//               warpgroup with the last tile did this, an item cost 10000 cycles
+//               more)
+//   warps 8-11, 12-15  softmax of the even / odd key tiles, thread = row. The
 //               running maximum passes from one warpgroup to the other through
 //               shared memory; it moves only when a row outgrows it by 2^8, and
 //               then O is rescaled in TMEM (exact: the sums use the same
-//               maximum). Each warpgroup keeps its own sum; the one with an
-//               item's last tile joins them and writes the output.
+//               maximum). Each warpgroup keeps its own sum.
 #include <algorithm>
 #include <utility>
 
@@ -48,7 +51,7 @@ namespace {
 
 constexpr int kBN = 128;        // keys per tile
 constexpr int kHeadDim = 128;
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kAhead = 3;       // key tiles that K is loaded ahead of V
 constexpr int kKStages = 4;
 constexpr int kVStages = 4;
@@ -56,9 +59,10 @@ constexpr int kQBytes = 32768;   // 128 rows x 128 channels
 constexpr int kQHalf = 16384;    // 64 channels
 constexpr int kKBytes = 16384;   // 64 keys x 128 channels
 constexpr int kVBytes = 16384;   // 128 keys x 64 channels
-constexpr int kStageBytes = 8 * 4096;  // 4 KB per softmax warp
+constexpr int kStageBytes = 4 * 4096;  // 4 KB per output warp
 constexpr int kTileSmem = 2 * kQBytes + kKStages * kKBytes + kVStages * kVBytes + kStageBytes;
-constexpr int kSmemBytes = kTileSmem + 3072;
+constexpr int kCtrlBytes = 5 * 1024 + 512;
+constexpr int kSmemBytes = kTileSmem + kCtrlBytes;
 #ifndef FMKA_PE
 #define FMKA_PE 100
 #endif
@@ -68,12 +72,14 @@ constexpr uint32_t kTmemO = 0, kTmemS = 128, kTmemP = 384;  // S: 2 x 128 column
 // Register split between the control warps and the softmax warps (setmaxnreg);
 // the sum has to fit in what the block is launched with.
 #ifndef FMKA_RC
-#define FMKA_RC 72
-#define FMKA_RS 216
+#define FMKA_RC 56
+#define FMKA_RO 88
+#define FMKA_RS 184
 #endif
 constexpr int kRegsControl = FMKA_RC;
+constexpr int kRegsOutput = FMKA_RO;
 constexpr int kRegsSoftmax = FMKA_RS;
-constexpr int kMinLaunchRegs = (128 * kRegsControl + 256 * kRegsSoftmax + kThreads - 1) / kThreads;
+constexpr int kMinLaunchRegs = (128 * (kRegsControl + kRegsOutput) + 256 * kRegsSoftmax + kThreads - 1) / kThreads;
 
 struct PairItem {
   int q0, nq;      // first row token, tokens (over both CTAs)
@@ -238,8 +244,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint8_t* sV = sK + kKStages * kKBytes;
   uint8_t* sStage = sV + kVStages * kVBytes;
   float* s_m = reinterpret_cast<float*>(sStage + kStageBytes);  // [128] running maximum
-  float* s_l = s_m + 128;                                           // [2][128] sums handed on at an item's end
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + 256);
+  float* s_lm = s_m + 128;  // [warpgroup][2 slots][sum, maximum][128] handed on at an item's end
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_lm + 1024);
   uint64_t* q_full = bars;                 // [2] even CTA
   uint64_t* q_empty = q_full + 2;          // [2] both
   uint64_t* k_full = q_empty + 2;          // [kKStages] even CTA
@@ -258,7 +264,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* bad_v = abort_flag + 1;    // [8] by item number: 1 + the last item with taken-out values
-  static_assert(512 * 3 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 6 + 4 + 1 + 24 + 2) + 40 <= 3072,
+  static_assert(512 * 9 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 6 + 4 + 1 + 24 + 2) + 48 <= kCtrlBytes,
                 "control block fits behind the tiles");
 
   const int warp = __shfl_sync(0xffffffffu, warp_id(), 0);
@@ -291,7 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&p_full[i], 8);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&pv_done[i], 1);
-    mbar_init(o_free, 8);
+    mbar_init(o_free, 8);  // output warps of both CTAs
     for (int i = 0; i < 8; ++i) mbar_init(&m_bar[i], 1);
     for (int i = 0; i < 16; ++i) mbar_init(&l_bar[i], 1);
     mbar_init(&mma_done[0], 1);
@@ -505,18 +511,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int live = min(kBN, it.ke - it.kb - j * kBN);  // rows that hold keys
         const int some = rows_all_see(it, j);
         if (some < kBN) {
-          // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes four rows at a time
+          // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes 32 rows at a time
           bool bad = false;
+          uint8_t* tile = sV + vr.s * kVBytes + (lane & 7) * 16;
 #pragma unroll 1
-          for (int row = some + (lane >> 3); row < kBN; row += 4) {
-            uint4* at = reinterpret_cast<uint4*>(sV + vr.s * kVBytes + row * 128 + (lane & 7) * 16);
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (row < live) {
-              x = *at;
-              if (!zero_nonfinite(x)) continue;
-              bad = true;
+          for (int row0 = some & ~31; row0 < kBN; row0 += 32) {
+            uint4 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = *reinterpret_cast<uint4*>(tile + (row0 + k * 4 + (lane >> 3)) * 128);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int row = row0 + k * 4 + (lane >> 3);
+              const bool taken = zero_nonfinite(x[k]) && row < live;
+              if (row >= live) x[k] = make_uint4(0, 0, 0, 0);
+              if (row >= some && (taken || row >= live)) *reinterpret_cast<uint4*>(tile + row * 128) = x[k];
+              bad |= taken && row >= some;
             }
-            *at = x;
           }
           if (__any_sync(0xffffffffu, bad) && lane == 0) {
             // the gate is at most four tiles ahead of the products, so eight slots never meet
@@ -533,22 +543,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok) *abort_flag = 1;
-  } else if (warp >= 4) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-    // ------------------------------------------------------------- softmax --
-    const int wg = (warp - 4) >> 2;
-    const int quarter = warp & 3;  // the TMEM lanes this warp may touch
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOutput));
+    // -------------------------------------------------------------- output --
+    const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t p_full_even = cluster_addr(&p_full[wg], 0);
-    const uint32_t s_free_even = cluster_addr(&s_free[wg], 0);
     const uint32_t o_free_even = cluster_addr(o_free, 0);
-    const int ri = r / p.Gs, rg = r - ri * p.Gs;  // token of the CTA's tile, head of the slice
-    const int ti = (int)rank * p.tpt + ri;         // token of the pair's tile
-    const uint32_t s_col = kTmemS + wg * 128, p_col = kTmemP + wg * 64;
-    int g0 = 0;                                    // tiles before this item
-    int items = 0;                                 // items with tiles before this one
-    int gave = 0, took = 0;                        // sums handed to / by the other warpgroup so far
+    const int ri = r / p.Gs, rg = r - ri * p.Gs;
+    const int ti = (int)rank * p.tpt + ri;
+    uint8_t* stage = sStage + quarter * 4096;  // 128 bytes of each row; chunk c of row i at c ^ (i & 7)
+    uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
+    int g0 = 0, items = 0;
+    int took[2] = {0, 0};
     bool ok = true;
     PairItem it;
     ItemWalk w;
@@ -556,23 +563,154 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     while (ok && w.next(p, pair, pairs, it, true)) {
       const bool row_ok = ri < p.tpt && ti < it.nq && rg < it.gn;
       const int n = it.n;
-      if (n == 0) {
-        // no row of the tile sees a key
-        if (wg == 0 && row_ok) {
-          uint4* dst = reinterpret_cast<uint4*>(p.o + (it.q0 + ti) * p.o_st + (it.hkv * p.G + it.g0 + rg) * p.o_sh);
-          for (int c = 0; c < 16; ++c) dst[c] = make_uint4(0, 0, 0, 0);
-          if (p.lse != nullptr)
-            p.lse[(it.q0 + ti) * p.lse_st + (it.hkv * p.G + it.g0 + rg) * p.lse_sh] = -INFINITY;
+      const int tok = it.q0 + ti, head = it.hkv * p.G + it.g0 + rg;
+      const bool direct = it.part < 0;
+      float L = 0.f, m_end = -INFINITY;
+      bool bad = false;
+      if (n > 0) {
+        // the sums of the two warpgroups, at the maximum of the one with the last tile
+        const int last = (g0 + n - 1) & 1;
+        float lw[2], mw[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          lw[e] = 0.f;
+          mw[e] = -INFINITY;
+          if (n >= 2 || e == last) {
+            const int slot = e * 2 + (took[e] & 1);
+            if (!(ok = warp_wait(&l_bar[slot * 4 + quarter], (took[e] >> 1) & 1, p.status))) break;
+            lw[e] = s_lm[(slot * 2 + 0) * 128 + r];
+            mw[e] = s_lm[(slot * 2 + 1) * 128 + r];
+            ++took[e];
+          }
         }
-        continue;
+        if (!ok) break;
+        m_end = last ? mw[1] : mw[0];
+        const float m_other = last ? mw[0] : mw[1], l_other = last ? lw[0] : lw[1];
+        L = (last ? lw[1] : lw[0]) + l_other * (m_other == m_end ? 1.f : fast_exp2(m_other - m_end));
+        const int gl = g0 + n - 1;
+        if (!(ok = warp_wait(&pv_done[gl & 3], (gl >> 2) & 1, p.status))) break;
+        tc_fence_after();
+        bad = bad_v[(items + 1) & 7] == items + 1;
+        g0 += n;
+        ++items;
       }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const float lse2 = L == 0.f ? -INFINITY : m_end + __log2f(L);
+      const bool live = row_ok && (direct || L != 0.f);  // a part without a visible key leaves only its -inf
+      const int64_t rec = it.part + (int64_t)ti * it.part_ts + rg;
+      const int64_t row_off = direct ? tok * p.o_st + head * p.o_sh : rec * kHeadDim;  // elements
+      uint8_t* row_out = (direct ? reinterpret_cast<uint8_t*>(p.o) : reinterpret_cast<uint8_t*>(p.part_o)) +
+                         row_off * (direct ? 2 : 4);
+      if (!live) row_out = nullptr;
+      const int passes = direct ? 2 : 4;
+#pragma unroll 1
+      for (int pass = 0; pass < passes; ++pass) {  // 128 bytes of every row: 64 channels in bf16, 32 in fp32
+        uint32_t o[64];
+        if (n > 0) {
+          const uint32_t col = lane_addr + kTmemO + pass * (direct ? 64 : 32);
+          tmem_ld32(col, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+          if (direct) tmem_ld32(col + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+          tmem_wait_ld();
+          if (pass == passes - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster_cta(o_free_even);
+          }
+        } else {  // no row of the tile sees a key
+#pragma unroll
+          for (int c = 0; c < 64; ++c) o[c] = 0u;
+        }
+        if (direct) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t w4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w4[e] = pack_bf16x2(__uint_as_float(o[c * 8 + 2 * e]) * inv, __uint_as_float(o[c * 8 + 2 * e + 1]) * inv);
+            mine[c ^ (lane & 7)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t w4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w4[e] = __float_as_uint(__uint_as_float(o[c * 4 + e]) * inv);
+            mine[c ^ (lane & 7)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          }
+        }
+        // Four rows of 128 bytes per store instruction, whole lines (a thread storing its own row would touch 32 lines
+        // with 16 bytes each); the loads of four come before their stores.
+        __syncwarp();
+#pragma unroll 1
+        for (int k0 = 0; k0 < 32; k0 += 16) {
+          uint4 x[4];
+          unsigned long long dst[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int rr = k0 + k * 4 + (lane >> 3);
+            dst[k] = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row_out), rr);
+            x[k] = *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane ^ rr) & 7) << 4));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (dst[k] != 0ull) *reinterpret_cast<uint4*>(dst[k] + pass * 128 + (lane & 7) * 16) = x[k];
+        }
+        __syncwarp();
+      }
+      if (direct) {
+        if (row_ok && p.lse != nullptr) p.lse[tok * p.lse_st + head * p.lse_sh] = lse2 * 0.69314718055994531f;
+      } else if (row_ok) {
+        p.part_lse[rec] = lse2;
+      }
+      if (bad && live) {
+        // rare: values that the V gate took out go to the rows that see them (the row's stores by other lanes come
+        // first: they are ordered by the barrier after them)
+        const int lim = min(it.ke - 1, it.lim0 + ti);
+        const __nv_bfloat16* vrow = p.v + (int64_t)it.k0 * p.kv_st + it.hkv * p.kv_sh;
+#pragma unroll 1
+        for (int key = max(it.kb, it.lim0 + 1); key <= lim; ++key) {
+#pragma unroll 1
+          for (int d = 0; d < kHeadDim; ++d) {
+            const float x = __bfloat162float(vrow[key * p.kv_st + d]);
+            if (fabsf(x) <= 3.4e38f) continue;
+            if (direct) {
+              __nv_bfloat16* y = p.o + row_off + d;
+              *y = __float2bfloat16(__bfloat162float(*y) + x);
+            } else {
+              p.part_o[row_off + d] += x;
+            }
+          }
+        }
+      }
+    }
+    if (!ok) *abort_flag = 1;
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    // ------------------------------------------------------------- softmax --
+    const int wg = (warp - 8) >> 2;
+    const int quarter = warp & 3;  // the TMEM lanes this warp may touch
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t p_full_even = cluster_addr(&p_full[wg], 0);
+    const uint32_t s_free_even = cluster_addr(&s_free[wg], 0);
+    const int ri = r / p.Gs, rg = r - ri * p.Gs;  // token of the CTA's tile, head of the slice
+    const int ti = (int)rank * p.tpt + ri;         // token of the pair's tile
+    const uint32_t s_col = kTmemS + wg * 128, p_col = kTmemP + wg * 64;
+    int g0 = 0;                                    // tiles before this item
+    int gave = 0;                                  // sums handed to the output warps so far
+    bool ok = true;
+    PairItem it;
+    ItemWalk w;
+    w.start(p, n_items, pair, pairs);
+    while (ok && w.next(p, pair, pairs, it, false)) {
+      const bool row_ok = ri < p.tpt && ti < it.nq && rg < it.gn;
+      const int n = it.n;
       // Last visible key. Rows that are not there (behind the last token, or the last rows where the group does not
       // divide 128) multiply whatever their Q holds; nothing of theirs is stored or has a say in the rescaling.
       const int lim = row_ok ? min(it.ke - 1, it.lim0 + ti) : 0x3FFFFFFF;
       // keys that every row of this CTA sees (from the first one on)
       const int rows_see = min(it.ke, max(it.kb, it.lim0 + 1 + (int)rank * p.tpt));
-      const int last_wg = (g0 + n - 1) & 1;
-      float m_own = -INFINITY, m_prev = -INFINITY, l = 0.f;
+      float m_own = -INFINITY, l = 0.f;
       // from this tile on, some row of this CTA does not see every key
       const int first_masked = (rows_see - it.kb) / kBN;
 #pragma unroll 1
@@ -622,7 +760,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
         float m_ref = j > 0 ? s_m[r] : -INFINITY;
-        m_prev = m_ref;
         float alpha = 1.f;
         const bool grow = __any_sync(0xffffffffu, row_ok && mx > m_ref + kRescaleThreshold);
         if (grow) {
@@ -678,112 +815,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_cluster_cta(p_full_even);
       }
       if (!ok) break;
-      if (wg != last_wg) {
-        if (n >= 2) {
-          // the sum so far, at this warpgroup's maximum, for the warpgroup that ends the item
-          // Two slots and barriers: the next item's sum can be ready before this one is read, the one after cannot,
-          // because its tiles wait for a maximum that the reader passes on after reading.
-          s_l[(gave & 1) * 128 + r] = l;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&l_bar[(wg * 2 + (gave & 1)) * 4 + quarter]);
-          ++gave;
-        }
-      } else {
-        // ---- epilogue: O of all tiles, both sums ----
-        const int gl = g0 + n - 1;
-        float l_other = 0.f;  // at m_prev, the maximum after the tile before the last
-        if (n >= 2) {
-          if (!(ok = warp_wait(&l_bar[((wg ^ 1) * 2 + (took & 1)) * 4 + quarter], (took >> 1) & 1, p.status))) break;
-          l_other = s_l[(took & 1) * 128 + r];
-          ++took;
-        }
-        if (!(ok = warp_wait(&pv_done[gl & 3], (gl >> 2) & 1, p.status))) break;
-        tc_fence_after();
-        const bool bad = bad_v[(items + 1) & 7] == items + 1;
-        const float L = l + l_other * (m_prev == m_own ? 1.f : fast_exp2(m_prev - m_own));
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        const float lse2 = L == 0.f ? -INFINITY : m_own + __log2f(L);
-        // Rows go out through 4 KB of staging per warp, so that a store instruction writes whole 128-byte lines (a
-        // thread storing its own row touches 32 lines with 16 bytes each). The loops stay rolled: this code runs once
-        // an item, and what it costs is mostly being fetched.
-        const bool direct = it.part < 0;
-        const bool live = row_ok && (direct || L != 0.f);  // a part without a visible key leaves only its -inf
-        const int tok = it.q0 + ti, head = it.hkv * p.G + it.g0 + rg;
-        const int64_t rec = it.part + (int64_t)ti * it.part_ts + rg;
-        const int64_t row_off = direct ? tok * p.o_st + head * p.o_sh : rec * kHeadDim;  // elements
-        const unsigned rows_live = __ballot_sync(0xffffffffu, live);
-        uint8_t* row_out = (direct ? reinterpret_cast<uint8_t*>(p.o) : reinterpret_cast<uint8_t*>(p.part_o)) +
-                           row_off * (direct ? 2 : 4) + (lane & 7) * 16;
-        const int sub = lane >> 3;
-        uint8_t* stage = sStage + (wg * 4 + quarter) * 4096;
-#pragma unroll 1
-        for (int pass = 0; pass < 4; ++pass) {  // 32 channels
-          uint32_t o[32];
-          tmem_ld32(lane_addr + kTmemO + pass * 32, o);
-          tmem_wait_ld();
-          if (pass == 3) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster_cta(o_free_even);
-          }
-          uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * inv);
-          if (direct) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t w4[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w4[e] = pack_bf16x2(__uint_as_float(o[c * 8 + 2 * e]), __uint_as_float(o[c * 8 + 2 * e + 1]));
-              mine[((pass & 1) * 4 + c) ^ (lane & 7)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-            }
-            if (!(pass & 1)) continue;
-          } else {
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              mine[c ^ (lane & 7)] = make_uint4(o[c * 4], o[c * 4 + 1], o[c * 4 + 2], o[c * 4 + 3]);
-          }
-          __syncwarp();
-          const int line = direct ? pass >> 1 : pass;  // 128 bytes of every row
-#pragma unroll 2
-          for (int rr = sub; rr < 32; rr += 4) {
-            // the row's address, with the chunk of the lane it came from: lane rr holds chunk rr & 7
-            uint8_t* dst = reinterpret_cast<uint8_t*>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row_out), rr));
-            if (rows_live >> rr & 1)
-              *reinterpret_cast<uint4*>(dst + line * 128 + ((lane & 7) - (rr & 7)) * 16) =
-                  *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-          }
-          __syncwarp();
-        }
-        if (direct) {
-          if (row_ok && p.lse != nullptr) p.lse[tok * p.lse_st + head * p.lse_sh] = lse2 * 0.69314718055994531f;
-        } else if (row_ok) {
-          p.part_lse[rec] = lse2;
-        }
-        if (bad && live) {
-          // rare: values that the V gate took out go to the rows that see them (the row's stores by other lanes come
-          // first: they are ordered by the barrier after them)
-          const __nv_bfloat16* vrow = p.v + (int64_t)it.k0 * p.kv_st + it.hkv * p.kv_sh;
-#pragma unroll 1
-          for (int key = max(it.kb, it.lim0 + 1); key <= lim; ++key) {
-#pragma unroll 1
-            for (int d = 0; d < kHeadDim; ++d) {
-              const float x = __bfloat162float(vrow[key * p.kv_st + d]);
-              if (fabsf(x) <= 3.4e38f) continue;
-              if (direct) {
-                __nv_bfloat16* y = p.o + row_off + d;
-                *y = __float2bfloat16(__bfloat162float(*y) + x);
-              } else {
-                p.part_o[row_off + d] += x;
-              }
-            }
-          }
-        }
+      if (n >= 2 || (g0 & 1) == wg) {
+        // This warpgroup's sum and maximum go to the output warps. Two slots: before the one after next is written,
+        // a product has been waited for that comes after the output warps have read this one.
+        s_lm[((wg * 2 + (gave & 1)) * 2 + 0) * 128 + r] = l;
+        s_lm[((wg * 2 + (gave & 1)) * 2 + 1) * 128 + r] = m_own;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&l_bar[(wg * 2 + (gave & 1)) * 4 + quarter]);
+        ++gave;
       }
       g0 += n;
-      ++items;
     }
     if (!ok) *abort_flag = 1;
   }
