@@ -61,8 +61,9 @@ constexpr int kKBytes = 16384;   // 64 keys x 128 channels
 constexpr int kVBytes = 16384;   // 128 keys x 64 channels
 constexpr int kStageBytes = 4 * 4096;  // 4 KB per output warp
 constexpr int kTileSmem = 2 * kQBytes + kKStages * kKBytes + kVStages * kVBytes + kStageBytes;
+constexpr int kMaxItems = 128;         // items of a pair in one launch
 constexpr int kCtrlBytes = 5 * 1024 + 512;
-constexpr int kSmemBytes = kTileSmem + kCtrlBytes;
+constexpr int kSmemBytes = kTileSmem + kCtrlBytes + kMaxItems * 48;
 #ifndef FMKA_PE
 #define FMKA_PE 100
 #endif
@@ -81,16 +82,18 @@ constexpr int kRegsOutput = FMKA_RO;
 constexpr int kRegsSoftmax = FMKA_RS;
 constexpr int kMinLaunchRegs = (128 * (kRegsControl + kRegsOutput) + 256 * kRegsSoftmax + kThreads - 1) / kThreads;
 
+// One item as the roles read it, in shared memory. Keys are counted from the item's first.
 struct PairItem {
   int q0, nq;      // first row token, tokens (over both CTAs)
-  int k0;          // packed row of the sequence's key 0
-  int kb, ke;      // keys [kb, ke)
+  int k0, n;       // packed row of the first key, key tiles
+  int klen;        // keys
   int lim0;        // last key token 0 sees (token i sees lim0 + i)
-  int hkv, g0, gn;
-  int n;           // key tiles
-  int64_t part;    // first partial row, or -1
+  int hkv, head0;  // kv head, first query head
+  int gn;          // query heads
   int part_ts;     // partial rows per token
+  int64_t part;    // first partial row, or -1
 };
+static_assert(sizeof(PairItem) == 48, "three 16-byte words");
 
 // Division by a number known on the host: q = (umulhi(n, m) + n) >> s for 0 <= n < 2^31.
 struct FastDiv {
@@ -121,6 +124,7 @@ struct PairParams {
   const int* header;         // [0] list entries; null: uniform items
   const int4* list;          // {q0, nq, k0, kb}, {ke, lim0, part, 0}
   int B, P, n_rt, n_splits, keys_per_split;  // uniform items
+  int round0;                // first round of this launch
   float* part_o;
   float* part_lse;
   uint32_t* status;
@@ -136,72 +140,46 @@ __device__ __forceinline__ int pair_item_index(int r, int pair, int pairs) {
   return r * pairs + ((r & 1) ? pairs - 1 - pair : pair);
 }
 
-// The items of one pair, one after the other. The list entry of the next item is
-// loaded while the current one runs; all lanes of a warp walk together.
-struct ItemWalk {
-  int r, idx, n_items;  // round of the entry held in (a, b), its item, all items
-  int4 a, b;
-  __device__ __forceinline__ void fetch(const PairParams& p, int pair, int pairs) {
-    // the snake's odd rounds run backwards, so only some pairs have an item in the last round
-    idx = pair_item_index(r, pair, pairs);
-    if (idx >= n_items) idx = r * pairs >= n_items ? -1 : -2;  // -1: past the end, -2: none in this round
-    if (idx >= 0 && p.header != nullptr) {
-      const int li = p.by_nh.div(idx);
-      a = __ldcg(p.list + 2 * li);
-      b = __ldcg(p.list + 2 * li + 1);
-    }
+__device__ __forceinline__ PairItem make_item(const PairParams& p, int idx) {
+  PairItem it;
+  const int li = p.by_nh.div(idx), h = idx - li * p.nh;
+  it.hkv = p.by_ngs.div(h);
+  const int g0 = (h - it.hkv * p.n_gs) * p.Gs;
+  it.head0 = it.hkv * p.G + g0;
+  it.gn = min(p.Gs, p.G - g0);
+  int kb, ke;
+  if (p.header != nullptr) {
+    const int4 a = __ldcg(p.list + 2 * li), b = __ldcg(p.list + 2 * li + 1);
+    it.q0 = a.x;
+    it.nq = a.y;
+    it.k0 = a.z + a.w;
+    kb = a.w;
+    ke = b.x;
+    it.lim0 = b.y - kb;
+    it.part = b.z < 0 ? -1 : (int64_t)b.z + (int64_t)h * a.y * p.Gs;
+    it.part_ts = p.Gs;
+  } else {
+    const int split = p.by_nrt.div(li), rt = li - split * p.n_rt;
+    it.q0 = rt * 2 * p.tpt;
+    it.nq = min(2 * p.tpt, p.B - it.q0);
+    kb = split * p.keys_per_split;
+    ke = min(p.P, kb + p.keys_per_split);
+    it.k0 = kb;
+    it.lim0 = p.P;
+    it.part = ((int64_t)split * p.B + it.q0) * p.Hq + it.head0;
+    it.part_ts = p.Hq;
   }
-  __device__ __forceinline__ void start(const PairParams& p, int n, int pair, int pairs) {
-    r = 0;
-    n_items = n;
-    fetch(p, pair, pairs);
-  }
-  // The next item, or false after the last. Items without key tiles (n == 0) are only given where `empty` asks.
-  __device__ __forceinline__ bool next(const PairParams& p, int pair, int pairs, PairItem& it, bool empty) {
-    while (true) {
-      const int i = idx;
-      if (i == -1) return false;
-      if (i >= 0) {
-        const int li = p.by_nh.div(i), h = i - li * p.nh;
-        it.hkv = p.by_ngs.div(h);
-        it.g0 = (h - it.hkv * p.n_gs) * p.Gs;
-        it.gn = min(p.Gs, p.G - it.g0);
-        if (p.header != nullptr) {
-          // the shuffles tell the compiler that the whole warp holds the same values
-          it.q0 = __shfl_sync(0xffffffffu, a.x, 0);
-          it.nq = __shfl_sync(0xffffffffu, a.y, 0);
-          it.k0 = __shfl_sync(0xffffffffu, a.z, 0);
-          it.kb = __shfl_sync(0xffffffffu, a.w, 0);
-          it.ke = __shfl_sync(0xffffffffu, b.x, 0);
-          it.lim0 = __shfl_sync(0xffffffffu, b.y, 0);
-          const int part = __shfl_sync(0xffffffffu, b.z, 0);
-          it.part = part < 0 ? -1 : (int64_t)part + (int64_t)h * it.nq * p.Gs;
-          it.part_ts = p.Gs;
-        } else {
-          const int split = p.by_nrt.div(li), rt = li - split * p.n_rt;
-          it.q0 = rt * 2 * p.tpt;
-          it.nq = min(2 * p.tpt, p.B - it.q0);
-          it.k0 = 0;
-          it.kb = split * p.keys_per_split;
-          it.ke = min(p.P, it.kb + p.keys_per_split);
-          it.lim0 = p.P;
-          it.part = ((int64_t)split * p.B + it.q0) * p.Hq + it.hkv * p.G + it.g0;
-          it.part_ts = p.Hq;
-        }
-        it.n = it.ke > it.kb ? (it.ke - it.kb + kBN - 1) / kBN : 0;
-      }
-      ++r;
-      fetch(p, pair, pairs);
-      if (i >= 0 && (it.n > 0 || empty)) return true;
-    }
-  }
-};
+  it.klen = max(0, ke - kb);
+  it.n = (it.klen + kBN - 1) / kBN;
+  return it;
+}
 
-// Keys of tile j that hold a key which every row of the item sees.
-__device__ __forceinline__ int rows_all_see(const PairItem& it, int j) {
-  const int kt = it.kb + j * kBN;
-  const int live = min(kBN, it.ke - kt);
-  return it.nq > 1 ? min(live, max(0, it.lim0 + 1 - kt)) : live;
+// The same value in all lanes, and known to be so by the compiler.
+__device__ __forceinline__ int uni(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// Keys (from the item's first) that every row sees: beyond them tiles have masked or missing keys.
+__device__ __forceinline__ int keys_all_see(const PairItem& it) {
+  return it.nq > 1 ? min(it.klen, max(0, it.lim0 + 1)) : it.klen;
 }
 
 // Position in a ring of N stages and the parity of its current round.
@@ -264,6 +242,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* bad_v = abort_flag + 1;    // [8] by item number: 1 + the last item with taken-out values
+  PairItem* items = reinterpret_cast<PairItem*>(smem + kTileSmem + kCtrlBytes);
   static_assert(512 * 9 + 8 * (2 * 2 + 2 * kKStages + 3 * kVStages + 6 + 4 + 1 + 24 + 2) + 48 <= kCtrlBytes,
                 "control block fits behind the tiles");
 
@@ -327,7 +306,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();  // the item list (or the previous kernel's outputs) is complete
   grid_launch_dependents();
+  // this pair's items, decoded once for all roles
   const int n_items = pair_item_count(p);
+  const int cnt = min(kMaxItems, max(0, (n_items + pairs - 1) / pairs - p.round0));
+  if (threadIdx.x < kMaxItems && (int)threadIdx.x < cnt) {
+    const int idx = pair_item_index(p.round0 + threadIdx.x, pair, pairs);
+    PairItem it = {};  // the last round may have none for this pair
+    it.part = -1;
+    if (idx < n_items) it = make_item(p, idx);
+    items[threadIdx.x] = it;
+  }
+  __syncthreads();
 
   if (warp == 0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
@@ -336,29 +325,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t q_full_even = cluster_addr(&q_full[0], 0);
     const uint32_t k_full_even = cluster_addr(&k_full[0], 0);
     const int q_box = p.Gs * p.tpt * 128;  // bytes of one 64-channel box
-    ItemWalk kw, vw;
-    PairItem ki, vi;
-    kw.start(p, n_items, pair, pairs);
-    vw = kw;
-    int kj = 0, vj = 0, ahead = 0, gk = 0, gv = 0, k_items = -1;
-    ki.n = vi.n = 0;
+    int ki = -1, vi = -1;  // items of the K and the V walk
+    int kn = 0, vn = 0, k_row = 0, v_row = 0, k_head = 0, v_head = 0;
+    int kj = 0, vj = 0, ahead = 0, gk = 0, gv = 0, q_use = -1;
     bool k_more = true;
     Ring<kKStages> kr;
     Ring<kVStages> vr;
     bool ok = true;
     while (ok) {
       while (k_more && ahead < kAhead) {
-        if (kj == ki.n) {
-          if (!(k_more = kw.next(p, pair, pairs, ki, false))) break;
-          kj = 0;
-          ++k_items;
-          const int qs = k_items & 1;
+        if (kj == kn) {
+          kj = kn = 0;
+          while (++ki < cnt && (kn = uni(items[ki].n)) == 0) {}
+          if (!(k_more = ki < cnt)) break;
+          k_row = uni(items[ki].k0) + (int)rank * 64;
+          k_head = uni(items[ki].hkv);
+          ++q_use;
+          const int qs = q_use & 1;
           if (!(ok = !__any_sync(0xffffffffu, *abort_flag) &&
-                     warp_wait(&q_empty[qs], ((k_items >> 1) & 1) ^ 1u, p.status))) break;
+                     warp_wait(&q_empty[qs], ((q_use >> 1) & 1) ^ 1u, p.status))) break;
           if (elect_one()) {
             if (rank == 0) mbar_arrive_expect_tx(&q_full[qs], 4 * q_box);
-            const int tok = ki.q0 + (int)rank * p.tpt;
-            const int head = ki.hkv * p.G + ki.g0;
+            const int tok = items[ki].q0 + (int)rank * p.tpt, head = items[ki].head0;
             tma_load_3d_pair(sQ + qs * kQBytes, &tmQ, q_full_even + qs * 8, 0, head, tok);
             tma_load_3d_pair(sQ + qs * kQBytes + kQHalf, &tmQ, q_full_even + qs * 8, 64, head, tok);
           }
@@ -367,27 +355,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (!(ok = warp_wait(&k_empty[kr.s], kr.ph ^ 1u, p.status))) break;
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&k_full[kr.s], 2 * kKBytes);
-          const int key = ki.k0 + ki.kb + kj * kBN + (int)rank * 64;
-          tma_load_3d_pair(sK + kr.s * kKBytes, &tmK, k_full_even + kr.s * 8, 0, key, ki.hkv);
-          tma_load_3d_pair(sK + kr.s * kKBytes + kKBytes / 2, &tmK, k_full_even + kr.s * 8, 64, key, ki.hkv);
+          tma_load_3d_pair(sK + kr.s * kKBytes, &tmK, k_full_even + kr.s * 8, 0, k_row, k_head);
+          tma_load_3d_pair(sK + kr.s * kKBytes + kKBytes / 2, &tmK, k_full_even + kr.s * 8, 64, k_row, k_head);
         }
         __syncwarp();
+        k_row += kBN;
         ++gk;
         ++ahead;
         ++kj;
         kr.step();
       }
       if (!ok) break;
-      if (vj == vi.n) {
-        if (!vw.next(p, pair, pairs, vi, false)) break;
-        vj = 0;
+      if (vj == vn) {
+        vj = vn = 0;
+        while (++vi < cnt && (vn = uni(items[vi].n)) == 0) {}
+        if (vi >= cnt) break;
+        v_row = uni(items[vi].k0);
+        v_head = uni(items[vi].hkv);
       }
       if (!(ok = warp_wait(&v_empty[vr.s], vr.ph ^ 1u, p.status))) break;
       if (elect_one()) {
         mbar_arrive_expect_tx(&v_land[vr.s], kVBytes);
-        tma_load_3d(sV + vr.s * kVBytes, &tmV, &v_land[vr.s], 64 * (int)rank, vi.k0 + vi.kb + vj * kBN, vi.hkv);
+        tma_load_3d(sV + vr.s * kVBytes, &tmV, &v_land[vr.s], 64 * (int)rank, v_row, v_head);
       }
       __syncwarp();
+      v_row += kBN;
       ++gv;
       --ahead;
       ++vj;
@@ -409,17 +401,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint64_t q_desc = desc_kmajor_sw128(smem_u32(sQ));
       const uint64_t k_desc = desc_kmajor_sw128(smem_u32(sK));
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      ItemWalk w;
-      PairItem it;
-      w.start(p, n_items, pair, pairs);
       Ring<kKStages> kr;
       Ring<2> sr, qr;
       bool ok = true;
-      while (ok && w.next(p, pair, pairs, it, false)) {
+      for (int i = 0; ok && i < cnt; ++i) {
+        const int n = uni(items[i].n);
+        if (n == 0) continue;
         if (!(ok = warp_wait(&q_full[qr.s], qr.ph, p.status))) break;
         const uint64_t qd = q_desc + (uint64_t)(qr.s * (kQBytes >> 4));
 #pragma unroll 1
-        for (int j = 0; j < it.n; ++j) {
+        for (int j = 0; j < n; ++j) {
           // the K tile, and the S buffer (its last scores are in registers)
           if (!(ok = warp_wait(&k_full[kr.s], kr.ph, p.status) && warp_wait(&s_free[sr.s], sr.ph ^ 1u, p.status))) break;
           tc_fence_after();
@@ -454,22 +445,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       constexpr uint32_t id_pv = make_idesc_bf16(256, kHeadDim, false, true);
       const uint64_t v_desc = desc_mnmajor_sw128(smem_u32(sV), kVBytes);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      ItemWalk w;
-      PairItem it;
-      w.start(p, n_items, pair, pairs);
       Ring<kVStages> vr;
       Ring<2> pr;
       Ring<4> dr;
       uint32_t o_phase = 1;  // nothing to wait for before the first item
       bool ok = true;
-      while (ok && w.next(p, pair, pairs, it, false)) {
+      for (int i = 0; ok && i < cnt; ++i) {
+        const int n = uni(items[i].n), gated = uni(keys_all_see(items[i])) / kBN;
+        if (n == 0) continue;
         if (!(ok = warp_wait(o_free, o_phase, p.status))) break;
         o_phase ^= 1u;
 #pragma unroll 1
-        for (int j = 0; j < it.n; ++j) {
+        for (int j = 0; j < n; ++j) {
           // a tile that the gates may have written to is acquired from the other CTA as well
-          ok = rows_all_see(it, j) < kBN ? __all_sync(0xffffffffu, mbar_wait_cluster(&v_ready[vr.s], vr.ph, p.status))
-                                         : warp_wait(&v_ready[vr.s], vr.ph, p.status);
+          ok = j >= gated ? __all_sync(0xffffffffu, mbar_wait_cluster(&v_ready[vr.s], vr.ph, p.status))
+                          : warp_wait(&v_ready[vr.s], vr.ph, p.status);
           if (!ok || !(ok = warp_wait(&p_full[pr.s], pr.ph, p.status))) break;
           tc_fence_after();
           const uint64_t vd = v_desc + (uint64_t)(vr.s * (kVBytes >> 4));
@@ -499,32 +489,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------- V gate --
     const uint32_t ready_even = cluster_addr(&v_ready[0], 0);
     const uint32_t bad_peer = cluster_addr(const_cast<int*>(bad_v), rank ^ 1u);
-    ItemWalk w;
-    PairItem it;
-    w.start(p, n_items, pair, pairs);
     Ring<kVStages> vr;
+    int item = 0;  // items with key tiles so far
     bool ok = true;
-    for (int item = 1; ok && w.next(p, pair, pairs, it, false); ++item) {
+    for (int i = 0; ok && i < cnt; ++i) {
+      const int n = uni(items[i].n), klen = uni(items[i].klen), see = uni(keys_all_see(items[i]));
+      item += n > 0;
 #pragma unroll 1
-      for (int j = 0; j < it.n; ++j) {
+      for (int j = 0; j < n; ++j) {
         if (!(ok = warp_wait(&v_land[vr.s], vr.ph, p.status))) break;
-        const int live = min(kBN, it.ke - it.kb - j * kBN);  // rows that hold keys
-        const int some = rows_all_see(it, j);
+        const int some = max(0, see - j * kBN);  // rows that every query sees
         if (some < kBN) {
-          // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes 32 rows at a time
+          const int live = klen - j * kBN;  // rows that hold keys
+          // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes 16 rows at a time
           bool bad = false;
-          uint8_t* tile = sV + vr.s * kVBytes + (lane & 7) * 16;
+          uint8_t* tile = sV + vr.s * kVBytes + (lane >> 3) * 128 + (lane & 7) * 16;
 #pragma unroll 1
-          for (int row0 = some & ~31; row0 < kBN; row0 += 32) {
-            uint4 x[8];
+          for (int row0 = some & ~15; row0 < kBN; row0 += 16) {
+            uint4 x[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = *reinterpret_cast<uint4*>(tile + (row0 + k * 4 + (lane >> 3)) * 128);
+            for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<uint4*>(tile + (row0 + k * 4) * 128);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < 4; ++k) {
               const int row = row0 + k * 4 + (lane >> 3);
-              const bool taken = zero_nonfinite(x[k]) && row < live;
-              if (row >= live) x[k] = make_uint4(0, 0, 0, 0);
-              if (row >= some && (taken || row >= live)) *reinterpret_cast<uint4*>(tile + row * 128) = x[k];
+              const bool gone = row >= live;
+              const bool taken = zero_nonfinite(x[k]) && !gone;
+              if (gone) x[k] = make_uint4(0, 0, 0, 0);
+              if (row >= some && (taken || gone)) *reinterpret_cast<uint4*>(tile + (row0 + k * 4) * 128) = x[k];
               bad |= taken && row >= some;
             }
           }
@@ -554,45 +545,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int ti = (int)rank * p.tpt + ri;
     uint8_t* stage = sStage + quarter * 4096;  // 128 bytes of each row; chunk c of row i at c ^ (i & 7)
     uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
-    int g0 = 0, items = 0;
-    int took[2] = {0, 0};
+    int g0 = 0, item = 0;
+    int took0 = 0, took1 = 0;
     bool ok = true;
-    PairItem it;
-    ItemWalk w;
-    w.start(p, n_items, pair, pairs);
-    while (ok && w.next(p, pair, pairs, it, true)) {
+    for (int i = 0; ok && i < cnt; ++i) {
+      const PairItem it = items[i];
       const bool row_ok = ri < p.tpt && ti < it.nq && rg < it.gn;
-      const int n = it.n;
-      const int tok = it.q0 + ti, head = it.hkv * p.G + it.g0 + rg;
+      const int n = uni(it.n);
+      const int tok = it.q0 + ti, head = it.head0 + rg;
       const bool direct = it.part < 0;
       float L = 0.f, m_end = -INFINITY;
       bool bad = false;
       if (n > 0) {
         // the sums of the two warpgroups, at the maximum of the one with the last tile
         const int last = (g0 + n - 1) & 1;
-        float lw[2], mw[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          lw[e] = 0.f;
-          mw[e] = -INFINITY;
-          if (n >= 2 || e == last) {
-            const int slot = e * 2 + (took[e] & 1);
-            if (!(ok = warp_wait(&l_bar[slot * 4 + quarter], (took[e] >> 1) & 1, p.status))) break;
-            lw[e] = s_lm[(slot * 2 + 0) * 128 + r];
-            mw[e] = s_lm[(slot * 2 + 1) * 128 + r];
-            ++took[e];
+        float l_other = 0.f, m_other = -INFINITY;
+#pragma unroll 1
+        for (int k = n >= 2 ? 0 : 1; k < 2; ++k) {  // the other one's, the last one's
+          const int e = last ^ k ^ 1;
+          const int took = e ? took1++ : took0++;
+          const int slot = e * 2 + (took & 1);
+          if (!(ok = warp_wait(&l_bar[slot * 4 + quarter], (took >> 1) & 1, p.status))) break;
+          if (k == 0) {
+            l_other = s_lm[(slot * 2 + 0) * 128 + r];
+            m_other = s_lm[(slot * 2 + 1) * 128 + r];
+          } else {
+            L = s_lm[(slot * 2 + 0) * 128 + r];
+            m_end = s_lm[(slot * 2 + 1) * 128 + r];
           }
         }
-        if (!ok) break;
-        m_end = last ? mw[1] : mw[0];
-        const float m_other = last ? mw[0] : mw[1], l_other = last ? lw[0] : lw[1];
-        L = (last ? lw[1] : lw[0]) + l_other * (m_other == m_end ? 1.f : fast_exp2(m_other - m_end));
         const int gl = g0 + n - 1;
-        if (!(ok = warp_wait(&pv_done[gl & 3], (gl >> 2) & 1, p.status))) break;
+        if (!ok || !(ok = warp_wait(&pv_done[gl & 3], (gl >> 2) & 1, p.status))) break;
         tc_fence_after();
-        bad = bad_v[(items + 1) & 7] == items + 1;
+        L += l_other * (m_other == m_end ? 1.f : fast_exp2(m_other - m_end));
         g0 += n;
-        ++items;
+        ++item;
+        bad = bad_v[item & 7] == item;
       }
       const float inv = L == 0.f ? 0.f : 1.f / L;
       const float lse2 = L == 0.f ? -INFINITY : m_end + __log2f(L);
@@ -602,58 +590,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint8_t* row_out = (direct ? reinterpret_cast<uint8_t*>(p.o) : reinterpret_cast<uint8_t*>(p.part_o)) +
                          row_off * (direct ? 2 : 4);
       if (!live) row_out = nullptr;
-      const int passes = direct ? 2 : 4;
 #pragma unroll 1
-      for (int pass = 0; pass < passes; ++pass) {  // 128 bytes of every row: 64 channels in bf16, 32 in fp32
-        uint32_t o[64];
+      for (int pass = 0; pass < 4; ++pass) {  // 32 channels
+        uint32_t o[32];
         if (n > 0) {
-          const uint32_t col = lane_addr + kTmemO + pass * (direct ? 64 : 32);
-          tmem_ld32(col, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
-          if (direct) tmem_ld32(col + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+          tmem_ld32(lane_addr + kTmemO + pass * 32, o);
           tmem_wait_ld();
-          if (pass == passes - 1) {
+          if (pass == 3) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster_cta(o_free_even);
           }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * inv);
         } else {  // no row of the tile sees a key
 #pragma unroll
-          for (int c = 0; c < 64; ++c) o[c] = 0u;
+          for (int c = 0; c < 32; ++c) o[c] = 0u;
         }
         if (direct) {
+          const int c0 = (pass & 1) * 4;
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
+          for (int c = 0; c < 4; ++c) {
             uint32_t w4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w4[e] = pack_bf16x2(__uint_as_float(o[c * 8 + 2 * e]) * inv, __uint_as_float(o[c * 8 + 2 * e + 1]) * inv);
-            mine[c ^ (lane & 7)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+              w4[e] = pack_bf16x2(__uint_as_float(o[c * 8 + 2 * e]), __uint_as_float(o[c * 8 + 2 * e + 1]));
+            mine[(c0 + c) ^ (lane & 7)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
           }
+          if (c0 == 0) continue;
         } else {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            uint32_t w4[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w4[e] = __float_as_uint(__uint_as_float(o[c * 4 + e]) * inv);
-            mine[c ^ (lane & 7)] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-          }
+          for (int c = 0; c < 8; ++c) mine[c ^ (lane & 7)] = make_uint4(o[c * 4], o[c * 4 + 1], o[c * 4 + 2], o[c * 4 + 3]);
         }
-        // Four rows of 128 bytes per store instruction, whole lines (a thread storing its own row would touch 32 lines
-        // with 16 bytes each); the loads of four come before their stores.
+        // 128 bytes of every row are staged. Four rows per store instruction, whole lines (a thread storing its own
+        // row would touch 32 lines with 16 bytes each); the loads of four come before their stores.
+        const int line = (direct ? pass >> 1 : pass) * 128 + (lane & 7) * 16;
         __syncwarp();
 #pragma unroll 1
-        for (int k0 = 0; k0 < 32; k0 += 16) {
+        for (int k0 = lane >> 3; k0 < 32; k0 += 16) {
           uint4 x[4];
           unsigned long long dst[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int rr = k0 + k * 4 + (lane >> 3);
+            const int rr = k0 + k * 4;
             dst[k] = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row_out), rr);
             x[k] = *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane ^ rr) & 7) << 4));
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (dst[k] != 0ull) *reinterpret_cast<uint4*>(dst[k] + pass * 128 + (lane & 7) * 16) = x[k];
+            if (dst[k] != 0ull) *reinterpret_cast<uint4*>(dst[k] + line) = x[k];
         }
         __syncwarp();
       }
@@ -665,10 +650,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (bad && live) {
         // rare: values that the V gate took out go to the rows that see them (the row's stores by other lanes come
         // first: they are ordered by the barrier after them)
-        const int lim = min(it.ke - 1, it.lim0 + ti);
+        const int lim = min(it.klen - 1, it.lim0 + ti);
         const __nv_bfloat16* vrow = p.v + (int64_t)it.k0 * p.kv_st + it.hkv * p.kv_sh;
 #pragma unroll 1
-        for (int key = max(it.kb, it.lim0 + 1); key <= lim; ++key) {
+        for (int key = max(0, it.lim0 + 1); key <= lim; ++key) {
 #pragma unroll 1
           for (int d = 0; d < kHeadDim; ++d) {
             const float x = __bfloat162float(vrow[key * p.kv_st + d]);
@@ -699,20 +684,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int g0 = 0;                                    // tiles before this item
     int gave = 0;                                  // sums handed to the output warps so far
     bool ok = true;
-    PairItem it;
-    ItemWalk w;
-    w.start(p, n_items, pair, pairs);
-    while (ok && w.next(p, pair, pairs, it, false)) {
-      const bool row_ok = ri < p.tpt && ti < it.nq && rg < it.gn;
-      const int n = it.n;
+    for (int i = 0; ok && i < cnt; ++i) {
+      const int n = uni(items[i].n);
+      if (n == 0) continue;
+      const int klen = items[i].klen, lim0 = items[i].lim0;
+      const bool row_ok = ri < p.tpt && ti < items[i].nq && rg < items[i].gn;
       // Last visible key. Rows that are not there (behind the last token, or the last rows where the group does not
       // divide 128) multiply whatever their Q holds; nothing of theirs is stored or has a say in the rescaling.
-      const int lim = row_ok ? min(it.ke - 1, it.lim0 + ti) : 0x3FFFFFFF;
-      // keys that every row of this CTA sees (from the first one on)
-      const int rows_see = min(it.ke, max(it.kb, it.lim0 + 1 + (int)rank * p.tpt));
+      const int lim = row_ok ? min(klen - 1, lim0 + ti) : 0x3FFFFFFF;
       float m_own = -INFINITY, l = 0.f;
       // from this tile on, some row of this CTA does not see every key
-      const int first_masked = (rows_see - it.kb) / kBN;
+      const int first_masked = uni(min(klen, max(0, lim0 + 1 + (int)rank * p.tpt))) / kBN;
 #pragma unroll 1
       for (int j = (g0 & 1) == wg ? 0 : 1; j < n; j += 2) {
         const int g = g0 + j;  // g & 1 == wg
@@ -728,7 +710,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_cta(s_free_even);
         if (j >= first_masked) {
-          const int seen = lim - it.kb - j * kBN;  // last visible column of the tile
+          const int seen = lim - j * kBN;  // last visible column of the tile
           const int all_see = __reduce_min_sync(0xffffffffu, seen);
 #pragma unroll
           for (int c0 = 0; c0 < 128; c0 += 16) {
@@ -1086,7 +1068,7 @@ void pair_tile(PairParams& p) {
 
 int launch_pair(const PairParams& given, const __nv_bfloat16* q, int64_t q_rows, int64_t q_st, int64_t q_sh,
                 const __nv_bfloat16* k, const __nv_bfloat16* v, int64_t kv_rows, int64_t kv_st, int64_t kv_sh,
-                int pairs, bool dependent, cudaStream_t stream, const char* what) {
+                int pairs, int64_t max_items, bool dependent, cudaStream_t stream, const char* what) {
   PairParams p = given;
   p.by_nh = FastDiv::of(p.nh);
   p.by_ngs = FastDiv::of(p.n_gs);
@@ -1109,9 +1091,16 @@ int launch_pair(const PairParams& given, const __nv_bfloat16* q, int64_t q_rows,
     return set_error(kErrUnsupported, std::string(what) + ": compiled register count too small for the warpgroup split");
   rc = check_cuda(cudaFuncSetAttribute(attn_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes), what);
   if (rc) return rc;
-  return check_cuda(launch_after(attn_pair_kernel, dim3(2 * pairs), kThreads, kSmemBytes, dependent, stream, tmQ, tmK,
-                                 tmV, p),
+  // kMaxItems of each pair per launch; the bound on the items is loose, a launch without any ends at once
+  const int64_t rounds = (max_items + pairs - 1) / pairs;
+  for (int64_t r0 = 0; r0 < rounds; r0 += kMaxItems) {
+    p.round0 = (int)r0;
+    rc = check_cuda(launch_after(attn_pair_kernel, dim3(2 * pairs), kThreads, kSmemBytes, dependent || r0 > 0, stream,
+                                 tmQ, tmK, tmV, p),
                     what);
+    if (rc) return rc;
+  }
+  return kOk;
 }
 
 // Scratch of the packed form, in bytes from its start.
@@ -1201,7 +1190,8 @@ int launch_attn_pair_varlen(const PackedAttnParams& a, int max_k, void* workspac
   attn_plan_kernel<<<1, kPlanThreads, 0, stream>>>(pl);
   int rc = check_cuda(cudaGetLastError(), "attn_varlen plan launch");
   if (rc) return rc;
-  rc = launch_pair(p, a.q, a.total_q, a.q_st, a.q_sh, a.k, a.v, a.total_k, a.kv_st, a.kv_sh, pairs, true, stream,
+  rc = launch_pair(p, a.q, a.total_q, a.q_st, a.q_sh, a.k, a.v, a.total_k, a.kv_st, a.kv_sh, pairs, (int64_t)w.max_list * p.nh,
+                   true, stream,
                    "attn_varlen launch");
   if (rc || !w.split) return rc;
   return check_cuda(launch_after(attn_join_kernel, dim3(w.max_parts, 8), 256, 0, true, stream, p, p.header,
@@ -1254,7 +1244,7 @@ int launch_attn_pair_prefix(const PackedAttnParams& a, cudaStream_t stream) {
   const int64_t items = (int64_t)p.n_rt * p.n_splits * p.nh;
   if (items > 0x3FFFFFFF) return set_error(kErrUnsupported, "attn_decode_shared: problem too large");
   const int pairs = (int)std::min<int64_t>(num_sms_current_device() / 2, items);
-  return launch_pair(p, a.q, a.B, a.q_st, a.q_sh, a.k, a.v, a.P, a.kv_st, a.kv_sh, pairs, false, stream,
+  return launch_pair(p, a.q, a.B, a.q_st, a.q_sh, a.k, a.v, a.P, a.kv_st, a.kv_sh, pairs, items, false, stream,
                      "attn_decode_shared prefix launch");
 }
 
