@@ -489,15 +489,38 @@ def silu_mul(g: torch.Tensor, u: torch.Tensor, out: Optional[torch.Tensor] = Non
 
 
 # ------------------------------------------- packed serving operators --
-def _check_same_device(dev: torch.device, what: str, *ts: Optional[torch.Tensor]) -> None:
+# These are called once per layer and step on small inputs, so their host time
+# counts: sizes and strides are read once, defaults take the short way, and the
+# device is only switched when it is not the current one.
+_DEFAULT_SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _same_device(what: str, dev: torch.device, *ts: Optional[torch.Tensor]) -> None:
     for t in ts:
         if t is not None and t.device != dev:
+            if not t.is_cuda:
+                raise RuntimeError("FastMKA B200 ops need CUDA tensors (there is no CPU fallback)")
             raise RuntimeError(f"{what}: all tensors must be on {dev}")
+
+
+def _on_device(dev: torch.device, name: str, *args) -> None:
+    """Calls entry point `name` with args and the current stream of `dev` behind them."""
+    fn = getattr(_lib.load(), name)
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev.index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _strides(t: torch.Tensor) -> Tuple[int, ...]:
     """Element strides, 0 for dimensions of one element (whose stride says nothing)."""
-    return tuple(0 if n == 1 else st for n, st in zip(t.shape, t.stride()))
+    return tuple([0 if n == 1 else st for n, st in zip(t.shape, t.stride())])
 
 
 def _check_out(what: str, out: torch.Tensor, shape: Sequence[int], dev: torch.device) -> None:
@@ -506,6 +529,14 @@ def _check_out(what: str, out: torch.Tensor, shape: Sequence[int], dev: torch.de
             st == 0 and n > 1 for n, st in zip(out.shape, out.stride())):
         raise RuntimeError(f"{what} must be a bf16 tensor of shape {tuple(shape)} on {dev} with contiguous channels "
                            "and no expanded dimension")
+
+
+def _rope_tables(cos: torch.Tensor, sin: torch.Tensor, B: int, T: int):
+    """cos/sin as fp32 rows of 128 with their strides (as _rope_args, without its conversions where none is needed)."""
+    if (cos.dtype is _F32 and sin.dtype is _F32 and cos.dim() == 2 and cos.shape == sin.shape
+            and cos.shape[0] == T and cos.shape[1] == HEAD_DIM and cos.is_contiguous() and sin.is_contiguous()):
+        return cos, sin, 0, HEAD_DIM
+    return _rope_args((cos, sin), B, T)
 
 
 def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[torch.Tensor] = None,
@@ -528,44 +559,54 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
     q_out / k_out: any strided tensors of the inputs' shapes, q and k themselves
     included. Returns (q_out, k_out).
     """
-    _check_cuda(q, k, q_weight, k_weight, positions)
-    _check_bf16(q, k)
     dev = q.device
-    _check_same_device(dev, "qk_norm_rope", k, q_weight, k_weight, positions)
-    if q.dim() not in (3, 4) or q.shape[-1] != HEAD_DIM or q.stride(-1) != 1:
+    if not q.is_cuda:
+        raise RuntimeError("FastMKA B200 ops need CUDA tensors (there is no CPU fallback)")
+    if q.dtype is not _BF16 or (k is not None and k.dtype is not _BF16):
+        _check_bf16(q, k)
+    _same_device("qk_norm_rope", dev, k, q_weight, k_weight, positions)
+    qs, qst = q.shape, _strides(q)
+    nd = len(qs)
+    if nd not in (3, 4) or qs[-1] != HEAD_DIM or q.stride(-1) != 1:
         raise RuntimeError("qk_norm_rope: q must be [T, Hq, 128] or [B, T, Hq, 128] with contiguous channels")
-    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != HEAD_DIM
-                          or k.stride(-1) != 1):
-        raise RuntimeError("qk_norm_rope: k must be q's shape with Hkv heads and contiguous channels")
+    Hkv, kst = 0, None
+    if k is not None:
+        ks, kst = k.shape, _strides(k)
+        if len(ks) != nd or ks[:-2] != qs[:-2] or ks[-1] != HEAD_DIM or k.stride(-1) != 1:
+            raise RuntimeError("qk_norm_rope: k must be q's shape with Hkv heads and contiguous channels")
+        Hkv = ks[-2]
     w_f32 = 0
-    for bit, w in enumerate((q_weight, k_weight)):
-        if w is None:
-            continue
-        if w.shape != (HEAD_DIM,) or not w.is_contiguous() or w.dtype not in (torch.bfloat16, torch.float32):
+    for bit, w in ((1, q_weight), (2, k_weight)):
+        if w is not None and w.dtype is not _BF16:
+            w_f32 |= bit
+            if w.dtype is not _F32:
+                raise RuntimeError("qk_norm_rope: the norm weights must be contiguous bf16 or fp32 [128] tensors")
+        if w is not None and (w.dim() != 1 or w.shape[0] != HEAD_DIM or w.stride(0) != 1):
             raise RuntimeError("qk_norm_rope: the norm weights must be contiguous bf16 or fp32 [128] tensors")
-        w_f32 |= int(w.dtype == torch.float32) << bit
-    T, Hq = q.shape[-3], q.shape[-2]
-    B = q.shape[0] if q.dim() == 4 else 1
-    Hkv = 0 if k is None else k.shape[-2]
-    pos_i64 = n_pos = 0
+    T, Hq = qs[-3], qs[-2]
+    B = qs[0] if nd == 4 else 1
+    cos = sin = None
+    rsb = rst = pos_i64 = n_pos = 0
     if positions is not None:
         if rope is None:
             raise RuntimeError("qk_norm_rope: positions need the cos/sin tables")
-        if positions.shape != q.shape[:-2] or positions.dtype not in (torch.int32, torch.int64):
+        if positions.shape != qs[:-2] or (positions.dtype is not _I32 and positions.dtype is not _I64):
             raise RuntimeError("qk_norm_rope: positions must be int32 or int64 of q's token shape")
         positions = positions.contiguous()
-        pos_i64 = int(positions.dtype == torch.int64)
-        n_pos = rope[0].shape[0]
-        if rope[0].dim() != 2 or rope[0].shape != rope[1].shape or n_pos == 0:
+        pos_i64 = int(positions.dtype is _I64)
+        cos, sin = rope
+        n_pos = cos.shape[0]
+        if cos.dim() != 2 or cos.shape != sin.shape or n_pos == 0:
             raise RuntimeError("qk_norm_rope: with positions, cos and sin must be tables [P, 128]")
-        cos, sin, rsb, rst = _rope_args(rope, 1, n_pos)
-    else:
-        cos, sin, rsb, rst = _rope_args(rope, B, T)
-    _check_same_device(dev, "qk_norm_rope", cos, sin)
+        cos, sin, rsb, rst = _rope_tables(cos, sin, 1, n_pos)
+    elif rope is not None:
+        cos, sin, rsb, rst = _rope_tables(rope[0], rope[1], B, T)
+    if cos is not None:
+        _same_device("qk_norm_rope", dev, cos, sin)
     if q_out is None:
         q_out = torch.empty_like(q)
     else:
-        _check_out("qk_norm_rope: q_out", q_out, q.shape, dev)
+        _check_out("qk_norm_rope: q_out", q_out, qs, dev)
     if k is None:
         k_out = None
     elif k_out is None:
@@ -576,14 +617,14 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
         return q_out, k_out
     if Hq == 0:
         raise RuntimeError("qk_norm_rope: q needs at least one head")
-
-    def st(t):
-        return (0, 0, 0) if t is None else (0,) * (4 - t.dim()) + _strides(t)[:-1]
-
-    with torch.cuda.device(dev):
-        _lib.call("fmka_qk_norm_rope_bf16", q.data_ptr(), *st(q), _ptr(k), *st(k), _ptr(q_weight), _ptr(k_weight),
-                  w_f32, float(eps), _ptr(cos), _ptr(sin), rsb, rst, _ptr(positions), pos_i64, n_pos,
-                  q_out.data_ptr(), *st(q_out), _ptr(k_out), *st(k_out), B, T, Hq, Hkv, HEAD_DIM, _stream(q))
+    ost = _strides(q_out)
+    kst = kst or (0,) * nd
+    kost = kst if k is None else _strides(k_out)
+    sb = 0 if nd == 3 else qst[0], 0 if nd == 3 else kst[0], 0 if nd == 3 else ost[0], 0 if nd == 3 else kost[0]
+    _on_device(dev, "fmka_qk_norm_rope_bf16", q.data_ptr(), sb[0], qst[-3], qst[-2], _ptr(k), sb[1], kst[-3], kst[-2],
+               _ptr(q_weight), _ptr(k_weight), w_f32, eps, _ptr(cos), _ptr(sin), rsb, rst, _ptr(positions), pos_i64,
+               n_pos, q_out.data_ptr(), sb[2], ost[-3], ost[-2], _ptr(k_out), sb[3], kost[-3], kost[-2], B, T, Hq, Hkv,
+               HEAD_DIM)
     return q_out, k_out
 
 
@@ -595,9 +636,11 @@ def _check_heads(what: str, Hq: int, Hkv: int, *ts: torch.Tensor) -> None:
         raise RuntimeError(f"{what}: query heads must be a multiple of kv heads")
 
 
-def _same_kv(what: str, k: torch.Tensor, v: torch.Tensor) -> None:
-    if k.shape != v.shape or _strides(k) != _strides(v):
+def _kv_strides(what: str, k: torch.Tensor, v: torch.Tensor) -> Tuple[int, ...]:
+    ks = _strides(k)
+    if k.shape != v.shape or ks != _strides(v):
         raise RuntimeError(f"{what}: k and v must have the same shape and strides")
+    return ks
 
 
 def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
@@ -619,44 +662,44 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     (or `out`, any strides; rows outside every sequence are left as they were)
     and lse [Hq, Tq] fp32.
     """
-    _check_cuda(q, k, v, cu_q, cu_k)
-    _check_bf16(q, k, v)
     dev = q.device
-    _check_same_device(dev, "attn_varlen", k, v, cu_q, cu_k)
+    if not q.is_cuda:
+        raise RuntimeError("FastMKA B200 ops need CUDA tensors (there is no CPU fallback)")
+    if q.dtype is not _BF16 or k.dtype is not _BF16 or v.dtype is not _BF16:
+        _check_bf16(q, k, v)
+    _same_device("attn_varlen", dev, k, v, cu_q, cu_k)
     if q.dim() != 3 or k.dim() != 3:
         raise RuntimeError("attn_varlen: expected q [Tq, Hq, 128] and k/v [Tk, Hkv, 128]")
-    _same_kv("attn_varlen", k, v)
+    ks, qs = _kv_strides("attn_varlen", k, v), _strides(q)
     Tq, Hq, Dh = q.shape
     Tk, Hkv, _ = k.shape
     _check_heads("attn_varlen", Hq, Hkv, q, k, v)
     for cu in (cu_q, cu_k):
-        if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() < 1 or not cu.is_contiguous():
+        if cu.dtype is not _I32 or cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
             raise RuntimeError("attn_varlen: cu_q and cu_k must be contiguous int32 [S + 1] tensors")
-    if cu_q.numel() != cu_k.numel():
+    S = cu_q.shape[0] - 1
+    if cu_k.shape[0] != S + 1:
         raise RuntimeError("attn_varlen: cu_q and cu_k must describe the same sequences")
-    S = cu_q.numel() - 1
-    if max_k is None:
+    if max_k is None or max_k > Tk:
         max_k = Tk
     elif max_k < 0:
         raise RuntimeError("attn_varlen: max_k must not be negative")
     if out is None:
-        out = torch.empty((Tq, Hq, Dh), dtype=torch.bfloat16, device=dev)
+        out = q.new_empty((Tq, Hq, Dh))
+        os_ = (Hq * Dh, Dh)
     else:
         _check_out("attn_varlen: out", out, q.shape, dev)
-    lse = torch.empty((Hq, Tq), dtype=torch.float32, device=dev) if want_lse else None
+        os_ = _strides(out)
+    lse = q.new_empty((Hq, Tq), dtype=_F32) if want_lse else None
     if Tq == 0 or S == 0:
         return out, lse
-    max_k = min(int(max_k), Tk)
-    qs, ks, os_ = _strides(q), _strides(k), _strides(out)
-    with torch.cuda.device(dev):
-        ws_bytes = _lib.load().fmka_attn_varlen_workspace_size(S, Tq, max_k, Hq, Hkv)
-        # one allocation per call: a buffer kept between calls would be shared by
-        # captured graphs that replay on different streams
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        _lib.call("fmka_attn_varlen", q.data_ptr(), qs[0], qs[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
-                  cu_q.data_ptr(), cu_k.data_ptr(), S, out.data_ptr(), os_[0], os_[1], _ptr(lse), 1, Tq, Tq, Tk,
-                  max_k, Hq, Hkv, Dh, int(causal), 1.0 / math.sqrt(Dh) if scale is None else float(scale), _ptr(ws),
-                  ws_bytes, _stream(q))
+    # one allocation per call: a buffer kept between calls would be shared by
+    # captured graphs that replay on different streams
+    ws_bytes = _lib.load().fmka_attn_varlen_workspace_size(S, Tq, max_k, Hq, Hkv)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    _on_device(dev, "fmka_attn_varlen", q.data_ptr(), qs[0], qs[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
+               cu_q.data_ptr(), cu_k.data_ptr(), S, out.data_ptr(), os_[0], os_[1], _ptr(lse), 1, Tq, Tq, Tk, max_k,
+               Hq, Hkv, Dh, int(causal), _DEFAULT_SCALE if scale is None else scale, _ptr(ws), ws_bytes)
     return out, lse
 
 
@@ -675,10 +718,13 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     empty; a request without any key gives zeros and a log-sum-exp of -inf.
     Returns o [B, 1, Hq, 128] and lse [B, Hq].
     """
-    _check_cuda(q, k_prefix, v_prefix, k, v, lens)
-    _check_bf16(q, k_prefix, v_prefix, k, v)
     dev = q.device
-    _check_same_device(dev, "attn_decode_shared", k_prefix, v_prefix, k, v, lens)
+    if not q.is_cuda:
+        raise RuntimeError("FastMKA B200 ops need CUDA tensors (there is no CPU fallback)")
+    if not (q.dtype is _BF16 and k_prefix.dtype is _BF16 and v_prefix.dtype is _BF16 and k.dtype is _BF16
+            and v.dtype is _BF16):
+        _check_bf16(q, k_prefix, v_prefix, k, v)
+    _same_device("attn_decode_shared", dev, k_prefix, v_prefix, k, v, lens)
     if q.dim() == 4 and q.shape[2] == 1:
         q = q[:, :, 0]
     if q.dim() != 3:
@@ -687,31 +733,32 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
         k_prefix, v_prefix = k_prefix[0], v_prefix[0]
     if k_prefix.dim() != 3 or k.dim() != 4:
         raise RuntimeError("attn_decode_shared: expected a prefix [Hkv, P, 128] and k/v [B, Hkv, Tcap, 128]")
-    _same_kv("attn_decode_shared", k_prefix, v_prefix)
-    _same_kv("attn_decode_shared", k, v)
+    ps, ks = _kv_strides("attn_decode_shared", k_prefix, v_prefix), _kv_strides("attn_decode_shared", k, v)
+    qs = _strides(q)
     B, Hq, Dh = q.shape
     Hkv, P, _ = k_prefix.shape
-    Tcap = k.shape[2]
-    if k.shape[0] != B or k.shape[1] != Hkv:
+    kB, kH, Tcap, _ = k.shape
+    if kB != B or kH != Hkv:
         raise RuntimeError("attn_decode_shared: k/v must hold q's batch and the prefix's kv heads")
     _check_heads("attn_decode_shared", Hq, Hkv, q, k_prefix, v_prefix, k, v)
-    if lens is not None and (lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous()):
+    if lens is not None and (lens.dtype is not _I32 or lens.dim() != 1 or lens.shape[0] != B
+                             or not lens.is_contiguous()):
         raise RuntimeError("attn_decode_shared: lens must be a contiguous int32 [B] tensor")
     if out is None:
-        out = torch.empty((B, 1, Hq, Dh), dtype=torch.bfloat16, device=dev)
+        out = q.new_empty((B, 1, Hq, Dh))
+        os_ = (Hq * Dh, 0, Dh)
     else:
         _check_out("attn_decode_shared: out", out, (B, 1, Hq, Dh), dev)
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if want_lse else None
+        os_ = _strides(out)
+    lse = q.new_empty((B, Hq), dtype=_F32) if want_lse else None
     if B == 0:
         return out, lse
-    qs, ps, ks, os_ = _strides(q), _strides(k_prefix), _strides(k), _strides(out)
-    with torch.cuda.device(dev):
-        ws_bytes = _lib.load().fmka_attn_decode_shared_workspace_size(B, Hq, Hkv, P, Tcap)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None  # as in attn_varlen
-        _lib.call("fmka_attn_decode_shared", q.data_ptr(), qs[0], qs[1], k_prefix.data_ptr(), v_prefix.data_ptr(),
-                  ps[0], ps[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], _ptr(lens), out.data_ptr(), os_[0],
-                  os_[2], _ptr(lse), Hq, B, Hq, Hkv, P, Tcap, Dh,
-                  1.0 / math.sqrt(Dh) if scale is None else float(scale), _ptr(ws), ws_bytes, _stream(q))
+    ws_bytes = _lib.load().fmka_attn_decode_shared_workspace_size(B, Hq, Hkv, P, Tcap)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None  # as in attn_varlen
+    _on_device(dev, "fmka_attn_decode_shared", q.data_ptr(), qs[0], qs[1], k_prefix.data_ptr(), v_prefix.data_ptr(),
+               ps[0], ps[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], _ptr(lens), out.data_ptr(), os_[0],
+               os_[2], _ptr(lse), Hq, B, Hq, Hkv, P, Tcap, Dh, _DEFAULT_SCALE if scale is None else scale, _ptr(ws),
+               ws_bytes)
     return out, lse
 
 
