@@ -829,6 +829,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // share is cut along its keys into parts that are joined afterwards.
 constexpr int kPlanThreads = 512;
 constexpr int kBins = 512;
+constexpr int kPlanSeqs = 1024;
 constexpr int kMinPartTiles = 4;  // a part is worth its partial output from 512 keys on
 
 struct PlanParams {
@@ -850,16 +851,18 @@ struct TileOf {
   int q0, nq, k0, ke, lim0, tiles;
 };
 
-__device__ __forceinline__ TileOf tile_of(const PlanParams& p, int f) {
+// Row tile f: `first` holds the tiles before each sequence.
+__device__ __forceinline__ TileOf tile_of(const PlanParams& p, const int* cu_q, const int* cu_k, const int* first,
+                                          int f) {
   int lo = 0, hi = p.n_seqs - 1;  // the last sequence whose first tile is at or before f
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p.seq_tiles[mid] <= f) lo = mid;
+    if (first[mid] <= f) lo = mid;
     else hi = mid - 1;
   }
-  const int q0 = p.cu_q[lo], lq = p.cu_q[lo + 1] - q0;
-  const int k0 = p.cu_k[lo], lk = p.cu_k[lo + 1] - k0;
-  const int t0 = (f - p.seq_tiles[lo]) * p.tok_tile;
+  const int q0 = cu_q[lo], lq = cu_q[lo + 1] - q0;
+  const int k0 = cu_k[lo], lk = cu_k[lo + 1] - k0;
+  const int t0 = (f - first[lo]) * p.tok_tile;
   TileOf t;
   t.q0 = q0 + t0;
   t.nq = min(p.tok_tile, lq - t0);
@@ -870,45 +873,70 @@ __device__ __forceinline__ TileOf tile_of(const PlanParams& p, int f) {
   return t;
 }
 
+// Inclusive sum over the block (kPlanThreads threads); `all` gets the total. s_warp: one int per warp.
+__device__ __forceinline__ int block_sum(int x, int* s_warp, int& all) {
+  const int lane = lane_id(), warp = warp_id();
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  int w = lane < kPlanThreads / 32 ? s_warp[lane] : 0;
+#pragma unroll
+  for (int d = 1; d < kPlanThreads / 32; d <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, d);
+    if (lane >= d) w += y;
+  }
+  all = __shfl_sync(0xffffffffu, w, kPlanThreads / 32 - 1);
+  const int before = __shfl_sync(0xffffffffu, w, max(0, warp - 1));
+  __syncthreads();
+  return x + (warp > 0 ? before : 0);
+}
+
 __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const __grid_constant__ PlanParams p) {
   __shared__ int s_warp[kPlanThreads / 32];
   __shared__ int s_hist[kBins];
   __shared__ unsigned long long s_total;
   __shared__ int s_groups, s_rows, s_max;
-  const int tid = threadIdx.x, lane = lane_id(), warp = warp_id();
+  __shared__ int s_seq[3][kPlanSeqs + 1];  // offsets and tiles of up to kPlanSeqs sequences; more stay in memory
+  const int tid = threadIdx.x, lane = lane_id();
   grid_launch_dependents();
-  for (int i = tid; i < kBins; i += kPlanThreads) s_hist[i] = 0;
+  s_hist[tid] = 0;
+  static_assert(kBins == kPlanThreads, "one bin per thread");
   if (tid == 0) {
     s_total = 0;
     s_groups = s_rows = s_max = 0;
   }
+  const bool small = p.n_seqs <= kPlanSeqs;
+  const int* cu_q = small ? s_seq[0] : p.cu_q;
+  const int* cu_k = small ? s_seq[1] : p.cu_k;
+  int* first = small ? s_seq[2] : p.seq_tiles;
   // tiles before each sequence
-  int base = 0;
+  int n_tiles = 0;
   bool bad = false;
   for (int s0 = 0; s0 < p.n_seqs; s0 += kPlanThreads) {
     const int s = s0 + tid;
     int nt = 0;
     if (s < p.n_seqs) {
-      const int q0 = p.cu_q[s], q1 = p.cu_q[s + 1], k0 = p.cu_k[s], k1 = p.cu_k[s + 1];
+      const int q0 = __ldg(p.cu_q + s), q1 = __ldg(p.cu_q + s + 1);
+      const int k0 = __ldg(p.cu_k + s), k1 = __ldg(p.cu_k + s + 1);
       bad |= q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k;
       nt = bad ? 0 : (q1 - q0 + p.tok_tile - 1) / p.tok_tile;
+      if (small) {
+        s_seq[0][s] = q0;
+        s_seq[1][s] = k0;
+        if (s == p.n_seqs - 1) {
+          s_seq[0][s + 1] = q1;
+          s_seq[1][s + 1] = k1;
+        }
+      }
     }
-    int incl = nt;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += x;
-    }
-    if (lane == 31) s_warp[warp] = incl;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
-      before += w < warp ? s_warp[w] : 0;
-      all += s_warp[w];
-    }
-    if (s < p.n_seqs) p.seq_tiles[s] = base + before + incl - nt;
-    base += all;
-    __syncthreads();
+    int all;
+    const int incl = block_sum(nt, s_warp, all);
+    if (s < p.n_seqs) first[s] = n_tiles + incl - nt;
+    n_tiles += all;
   }
   if (__syncthreads_or(bad)) {
     if (tid == 0) {
@@ -917,60 +945,50 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const __grid_co
     }
     return;
   }
-  const int n_tiles = base;
   // all work, and the largest tile
-  unsigned long long sum = 0;
+  unsigned sum = 0;
   int most = 1;
   for (int f = tid; f < n_tiles; f += kPlanThreads) {
-    const int c = tile_of(p, f).tiles;
-    sum += c;
+    const int c = tile_of(p, cu_q, cu_k, first, f).tiles;
+    sum += c;  // below 2^32: total_q / tok_tile tiles per thread of at most 2^24 key tiles would be needed
     most = max(most, c);
   }
-  atomicAdd(&s_total, sum);
-  atomicMax(&s_max, most);
+  const unsigned warp_sum = __reduce_add_sync(0xffffffffu, sum & 0xFFFFFu);
+  const unsigned warp_high = __reduce_add_sync(0xffffffffu, sum >> 20);
+  const int warp_most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) {
+    atomicAdd(&s_total, (unsigned long long)warp_sum + ((unsigned long long)warp_high << 20));
+    atomicMax(&s_max, warp_most);
+  }
   __syncthreads();
   const unsigned long long work = s_total * p.nh;
   const int share = (int)max((unsigned long long)kMinPartTiles, (work + p.pairs - 1) / p.pairs);
+  const int top = min(s_max, p.split ? share : s_max);
+  const float scale = (float)kBins / (float)(top + 1);
   auto parts_of = [&](int tiles) { return p.split && tiles > share ? (tiles + share - 1) / share : 1; };
-  const int top = min(s_max, p.split ? max(share, 1) : s_max);
-  auto bin_of = [&](int tiles) {
-    return kBins - 1 - (int)min((long long)kBins - 1, (long long)tiles * kBins / (top + 1));
-  };
+  auto bin_of = [&](int tiles) { return kBins - 1 - min(kBins - 1, (int)((float)tiles * scale)); };
   for (int f = tid; f < n_tiles; f += kPlanThreads) {
-    const int c = tile_of(p, f).tiles, np = parts_of(c);
+    const int c = tile_of(p, cu_q, cu_k, first, f).tiles, np = parts_of(c);
     atomicAdd(&s_hist[bin_of((c + np - 1) / np)], np);
   }
   __syncthreads();
   // exclusive sums over the bins, heavy bins first
   {
-    static_assert(kBins == kPlanThreads, "one bin per thread");
     const int n = s_hist[tid];
-    int incl = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += x;
-    }
-    if (lane == 31) s_warp[warp] = incl;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
-      before += w < warp ? s_warp[w] : 0;
-      all += s_warp[w];
-    }
-    s_hist[tid] = before + incl - n;
+    int all;
+    const int incl = block_sum(n, s_warp, all);
+    s_hist[tid] = incl - n;
     if (tid == 0) p.header[0] = all;
   }
   __syncthreads();
   for (int f = tid; f < n_tiles; f += kPlanThreads) {
-    const TileOf t = tile_of(p, f);
+    const TileOf t = tile_of(p, cu_q, cu_k, first, f);
     const int np = parts_of(t.tiles);
     const int per = (t.tiles + np - 1) / np;
     const int at = atomicAdd(&s_hist[bin_of(per)], np);
-    int row0 = -1;
     if (np > 1) {
       const int rows = t.nq * p.Gs * p.nh;
-      row0 = atomicAdd(&s_rows, np * rows);
+      const int row0 = atomicAdd(&s_rows, np * rows);
       p.groups[atomicAdd(&s_groups, 1)] = make_int4(t.q0, t.nq, np, row0);
       for (int i = 0; i < np; ++i) {
         p.list[2 * (at + i)] = make_int4(t.q0, t.nq, t.k0, i * per * kBN);
