@@ -20,7 +20,7 @@ LIB_NAME = "libfastmka_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 
 SOURCES = ["capi.cu", "gemm.cu", "route_scan.cu", "attn_prefill.cu", "attn_decode.cu", "peer.cu", "norm.cu", "l3_recall.cu",
-           "qk_norm.cu", "attn_rows.cu", "attn_pair.cu"]
+           "qk_norm.cu", "attn_rows.cu", "attn_pair.cu", "attn_plan.cu"]
 HEADERS = ["ptx.cuh", "fmka_internal.h"]
 
 NVCC_FLAGS = [

@@ -40,7 +40,6 @@
 //               then O is rescaled in TMEM (exact: the sums use the same
 //               maximum). Each warpgroup keeps its own sum.
 #include <algorithm>
-#include <utility>
 
 #include "fmka_internal.h"
 #include "ptx.cuh"
@@ -820,245 +819,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-// ------------------------------------------------------------------- plan --
-// (List, header and parts are read past L1: the reading kernels start before their writers end.)
-// One CTA turns the sequences' offsets into the item list: row tiles of 2 * tpt
-// tokens, each against the keys its rows see, sorted by falling work (a counting
-// sort over kBins classes of tile counts), so that the snake of the main kernel
-// gives every pair about the same. A tile with more work than a pair's fair
-// share is cut along its keys into parts that are joined afterwards.
-constexpr int kPlanThreads = 512;
-constexpr int kBins = 512;
-constexpr int kPlanSeqs = 1024;
-constexpr int kMinPartTiles = 4;  // a part is worth its partial output from 512 keys on
-
-struct PlanParams {
-  const int* cu_q;
-  const int* cu_k;
-  int n_seqs, total_q, total_k, causal;
-  int tok_tile;    // tokens per item
-  int nh, Gs, pairs;
-  int split;       // parts are allowed
-  int max_parts;   // list entries set aside for parts
-  int* header;     // [0] list entries, [1] groups of parts
-  int* seq_tiles;  // [n_seqs + 1] tiles before each sequence
-  int4* list;
-  int4* groups;    // {q0, nq, parts, first partial row}
-  uint32_t* status;
-};
-
-struct TileOf {
-  int q0, nq, k0, ke, lim0, tiles;
-};
-
-// Row tile f: `first` holds the tiles before each sequence.
-__device__ __forceinline__ TileOf tile_of(const PlanParams& p, const int* cu_q, const int* cu_k, const int* first,
-                                          int f) {
-  int lo = 0, hi = p.n_seqs - 1;  // the last sequence whose first tile is at or before f
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first[mid] <= f) lo = mid;
-    else hi = mid - 1;
-  }
-  const int q0 = cu_q[lo], lq = cu_q[lo + 1] - q0;
-  const int k0 = cu_k[lo], lk = cu_k[lo + 1] - k0;
-  const int t0 = (f - first[lo]) * p.tok_tile;
-  TileOf t;
-  t.q0 = q0 + t0;
-  t.nq = min(p.tok_tile, lq - t0);
-  t.k0 = k0;
-  t.lim0 = p.causal ? t0 + lk - lq : lk;
-  t.ke = p.causal ? max(0, min(lk, t.lim0 + t.nq)) : lk;
-  t.tiles = (t.ke + kBN - 1) / kBN;
-  return t;
-}
-
-// Inclusive sum over the block (kPlanThreads threads); `all` gets the total. s_warp: one int per warp.
-__device__ __forceinline__ int block_sum(int x, int* s_warp, int& all) {
-  const int lane = lane_id(), warp = warp_id();
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, d);
-    if (lane >= d) x += y;
-  }
-  if (lane == 31) s_warp[warp] = x;
-  __syncthreads();
-  int w = lane < kPlanThreads / 32 ? s_warp[lane] : 0;
-#pragma unroll
-  for (int d = 1; d < kPlanThreads / 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, w, d);
-    if (lane >= d) w += y;
-  }
-  all = __shfl_sync(0xffffffffu, w, kPlanThreads / 32 - 1);
-  const int before = __shfl_sync(0xffffffffu, w, max(0, warp - 1));
-  __syncthreads();
-  return x + (warp > 0 ? before : 0);
-}
-
-__global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const __grid_constant__ PlanParams p) {
-  __shared__ int s_warp[kPlanThreads / 32];
-  __shared__ int s_hist[kBins];
-  __shared__ unsigned long long s_total;
-  __shared__ int s_groups, s_rows, s_max;
-  __shared__ int s_seq[3][kPlanSeqs + 1];  // offsets and tiles of up to kPlanSeqs sequences; more stay in memory
-  const int tid = threadIdx.x, lane = lane_id();
-  grid_launch_dependents();
-  s_hist[tid] = 0;
-  static_assert(kBins == kPlanThreads, "one bin per thread");
-  if (tid == 0) {
-    s_total = 0;
-    s_groups = s_rows = s_max = 0;
-  }
-  const bool small = p.n_seqs <= kPlanSeqs;
-  const int* cu_q = small ? s_seq[0] : p.cu_q;
-  const int* cu_k = small ? s_seq[1] : p.cu_k;
-  int* first = small ? s_seq[2] : p.seq_tiles;
-  // tiles before each sequence
-  int n_tiles = 0;
-  bool bad = false;
-  for (int s0 = 0; s0 < p.n_seqs; s0 += kPlanThreads) {
-    const int s = s0 + tid;
-    int nt = 0;
-    if (s < p.n_seqs) {
-      const int q0 = __ldg(p.cu_q + s), q1 = __ldg(p.cu_q + s + 1);
-      const int k0 = __ldg(p.cu_k + s), k1 = __ldg(p.cu_k + s + 1);
-      bad |= q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k;
-      nt = bad ? 0 : (q1 - q0 + p.tok_tile - 1) / p.tok_tile;
-      if (small) {
-        s_seq[0][s] = q0;
-        s_seq[1][s] = k0;
-        if (s == p.n_seqs - 1) {
-          s_seq[0][s + 1] = q1;
-          s_seq[1][s + 1] = k1;
-        }
-      }
-    }
-    int all;
-    const int incl = block_sum(nt, s_warp, all);
-    if (s < p.n_seqs) first[s] = n_tiles + incl - nt;
-    n_tiles += all;
-  }
-  if (__syncthreads_or(bad)) {
-    if (tid == 0) {
-      atomicOr(p.status, kStatusBadLaunch);
-      p.header[0] = p.header[1] = 0;
-    }
-    return;
-  }
-  // all work, and the largest tile
-  unsigned sum = 0;
-  int most = 1;
-  for (int f = tid; f < n_tiles; f += kPlanThreads) {
-    const int c = tile_of(p, cu_q, cu_k, first, f).tiles;
-    sum += c;  // below 2^32: total_q / tok_tile tiles per thread of at most 2^24 key tiles would be needed
-    most = max(most, c);
-  }
-  const unsigned warp_sum = __reduce_add_sync(0xffffffffu, sum & 0xFFFFFu);
-  const unsigned warp_high = __reduce_add_sync(0xffffffffu, sum >> 20);
-  const int warp_most = __reduce_max_sync(0xffffffffu, most);
-  if (lane == 0) {
-    atomicAdd(&s_total, (unsigned long long)warp_sum + ((unsigned long long)warp_high << 20));
-    atomicMax(&s_max, warp_most);
-  }
-  __syncthreads();
-  const unsigned long long work = s_total * p.nh;
-  const int share = (int)max((unsigned long long)kMinPartTiles, (work + p.pairs - 1) / p.pairs);
-  const int top = min(s_max, p.split ? share : s_max);
-  const float scale = (float)kBins / (float)(top + 1);
-  auto parts_of = [&](int tiles) { return p.split && tiles > share ? (tiles + share - 1) / share : 1; };
-  auto bin_of = [&](int tiles) { return kBins - 1 - min(kBins - 1, (int)((float)tiles * scale)); };
-  for (int f = tid; f < n_tiles; f += kPlanThreads) {
-    const int c = tile_of(p, cu_q, cu_k, first, f).tiles, np = parts_of(c);
-    atomicAdd(&s_hist[bin_of((c + np - 1) / np)], np);
-  }
-  __syncthreads();
-  // exclusive sums over the bins, heavy bins first
-  {
-    const int n = s_hist[tid];
-    int all;
-    const int incl = block_sum(n, s_warp, all);
-    s_hist[tid] = incl - n;
-    if (tid == 0) p.header[0] = all;
-  }
-  __syncthreads();
-  for (int f = tid; f < n_tiles; f += kPlanThreads) {
-    const TileOf t = tile_of(p, cu_q, cu_k, first, f);
-    const int np = parts_of(t.tiles);
-    const int per = (t.tiles + np - 1) / np;
-    const int at = atomicAdd(&s_hist[bin_of(per)], np);
-    if (np > 1) {
-      const int rows = t.nq * p.Gs * p.nh;
-      const int row0 = atomicAdd(&s_rows, np * rows);
-      p.groups[atomicAdd(&s_groups, 1)] = make_int4(t.q0, t.nq, np, row0);
-      for (int i = 0; i < np; ++i) {
-        p.list[2 * (at + i)] = make_int4(t.q0, t.nq, t.k0, i * per * kBN);
-        p.list[2 * (at + i) + 1] = make_int4(min(t.ke, (i + 1) * per * kBN), t.lim0, row0 + i * rows, 0);
-      }
-    } else {
-      p.list[2 * at] = make_int4(t.q0, t.nq, t.k0, 0);
-      p.list[2 * at + 1] = make_int4(t.ke, t.lim0, -1, 0);
-    }
-  }
-  __syncthreads();
-  if (tid == 0) p.header[1] = s_groups;
-}
-
-// Joins the parts of the rows whose keys were cut: a block per group of parts (x) and slice of its rows (y), a warp
-// per row.
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ PairParams p, const int* header,
-                                                        const int4* groups) {
-  grid_dependency_wait();
-  if ((int)blockIdx.x >= __ldcg(header + 1)) return;
-  const int4 gr = __ldcg(groups + blockIdx.x);
-  const int lane = lane_id();
-  const int item_rows = gr.y * p.Gs, rows = item_rows * p.nh;
-  for (int row = blockIdx.y * 8 + warp_id(); row < rows; row += gridDim.y * 8) {
-    const int h = row / item_rows, ti = (row - h * item_rows) / p.Gs, g = row % p.Gs;
-    const int hkv = h / p.n_gs, hg = (h - hkv * p.n_gs) * p.Gs + g;
-    if (hg >= p.G) continue;
-    float M = -INFINITY;
-    for (int s = 0; s < gr.z; ++s) M = fmaxf(M, __ldcg(p.part_lse + gr.w + (int64_t)s * rows + row));
-    const float Ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < gr.z; ++s) {
-      const int64_t rec = (int64_t)gr.w + (int64_t)s * rows + row;
-      const float x = __ldcg(p.part_lse + rec);
-      if (x == -INFINITY) continue;  // this part saw no key of the row: nothing was written
-      const float w = fast_exp2(x - Ms);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + rec * kHeadDim) + lane);
-      L += w;
-      acc.x += w * v.x;
-      acc.y += w * v.y;
-      acc.z += w * v.z;
-      acc.w += w * v.w;
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int64_t tok = gr.x + ti;
-    const int head = hkv * p.G + hg;
-    reinterpret_cast<uint2*>(p.o + tok * p.o_st + head * p.o_sh)[lane] =
-        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    if (lane == 0 && p.lse != nullptr)
-      p.lse[tok * p.lse_st + head * p.lse_sh] = L == 0.f ? -INFINITY : (Ms + __log2f(L)) * 0.69314718055994531f;
-  }
-}
-
-template <class... Params, class... Args>
-cudaError_t launch_after(void (*kern)(Params...), dim3 grid, int threads, size_t smem, bool dependent,
-                         cudaStream_t stream, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
-
 // Tensor map over [rows][heads][128] with a box of box_h heads x box_r rows x 64 channels. The stride of a dimension
 // of one element says nothing.
 int rows_map(CUtensorMap* out, const __nv_bfloat16* base, int64_t rows, int64_t st, int heads, int64_t sh, int box_h,
@@ -1121,51 +881,17 @@ int launch_pair(const PairParams& given, const __nv_bfloat16* q, int64_t q_rows,
   return kOk;
 }
 
-// Scratch of the packed form, in bytes from its start.
-struct VarlenLayout {
-  int max_list, max_parts, split;
-  int64_t part_rows;
-  size_t seq_tiles, list, groups, part_o, part_lse, total;
-};
-
-size_t up16(size_t x) { return (x + 15) & ~size_t(15); }
-
-VarlenLayout varlen_layout(int n_seqs, int total_q, int max_k, const PairParams& p, int pairs) {
-  VarlenLayout w;
-  const int tok_tile = 2 * p.tpt;
-  // a tile with more than a pair's share of the work is cut into at most twice work / share parts, so all parts of
-  // all heads number at most twice the pairs
-  w.split = max_k > kMinPartTiles * kBN;
-  w.max_parts = w.split ? 2 * pairs : 0;
-  w.max_list = total_q / tok_tile + n_seqs + w.max_parts;
-  w.part_rows = (int64_t)w.max_parts * tok_tile * p.Gs;
-  size_t at = 16;
-  w.seq_tiles = at;
-  at = up16(at + sizeof(int) * (size_t)(n_seqs + 1));
-  w.list = at;
-  at += sizeof(int4) * 2 * (size_t)w.max_list;
-  w.groups = at;
-  at += sizeof(int4) * (size_t)w.max_parts;
-  w.part_o = at;
-  at += sizeof(float) * kHeadDim * (size_t)w.part_rows;
-  w.part_lse = at;
-  at += sizeof(float) * (size_t)w.part_rows;
-  w.total = up16(at);
-  return w;
-}
-
 }  // namespace
 
-size_t attn_pair_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv) {
+PackedPlan attn_pair_plan(int n_seqs, int total_q, int max_k, int Hq, int Hkv) {
   PairParams p = {};
   p.Hq = Hq;
   p.G = Hq / Hkv;
   pair_tile(p);
-  return varlen_layout(n_seqs, total_q, max_k, p, num_sms_current_device() / 2).total;
+  return packed_plan(n_seqs, total_q, max_k, Hkv, p.G, p.Gs, 2 * p.tpt, num_sms_current_device() / 2);
 }
 
-int launch_attn_pair_varlen(const PackedAttnParams& a, int max_k, void* workspace, cudaStream_t stream) {
-  const int pairs = num_sms_current_device() / 2;
+int launch_attn_pair_varlen(const PackedAttnParams& a, const PackedPlan& w, cudaStream_t stream) {
   PairParams p = {};
   p.o = a.o;
   p.o_st = a.o_st;
@@ -1181,40 +907,12 @@ int launch_attn_pair_varlen(const PackedAttnParams& a, int max_k, void* workspac
   pair_tile(p);
   p.scale_log2 = a.scale_log2;
   p.status = a.status;
-  const VarlenLayout w = varlen_layout(a.n_seqs, a.total_q, max_k, p, pairs);
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.header = reinterpret_cast<const int*>(ws);
-  p.list = reinterpret_cast<const int4*>(ws + w.list);
-  p.part_o = reinterpret_cast<float*>(ws + w.part_o);
-  p.part_lse = reinterpret_cast<float*>(ws + w.part_lse);
-  PlanParams pl = {};
-  pl.cu_q = a.cu_q;
-  pl.cu_k = a.cu_k;
-  pl.n_seqs = a.n_seqs;
-  pl.total_q = a.total_q;
-  pl.total_k = a.total_k;
-  pl.causal = a.causal;
-  pl.tok_tile = 2 * p.tpt;
-  pl.nh = p.nh;
-  pl.Gs = p.Gs;
-  pl.pairs = pairs;
-  pl.split = w.split;
-  pl.max_parts = w.max_parts;
-  pl.header = reinterpret_cast<int*>(ws);
-  pl.seq_tiles = reinterpret_cast<int*>(ws + w.seq_tiles);
-  pl.list = reinterpret_cast<int4*>(ws + w.list);
-  pl.groups = reinterpret_cast<int4*>(ws + w.groups);
-  pl.status = a.status;
-  attn_plan_kernel<<<1, kPlanThreads, 0, stream>>>(pl);
-  int rc = check_cuda(cudaGetLastError(), "attn_varlen plan launch");
-  if (rc) return rc;
-  rc = launch_pair(p, a.q, a.total_q, a.q_st, a.q_sh, a.k, a.v, a.total_k, a.kv_st, a.kv_sh, pairs, (int64_t)w.max_list * p.nh,
-                   true, stream,
-                   "attn_varlen launch");
-  if (rc || !w.split) return rc;
-  return check_cuda(launch_after(attn_join_kernel, dim3(w.max_parts, 8), 256, 0, true, stream, p, p.header,
-                                 reinterpret_cast<const int4*>(ws + w.groups)),
-                    "attn_varlen join launch");
+  p.header = w.header;
+  p.list = w.list;
+  p.part_o = w.part_o;
+  p.part_lse = w.part_lse;
+  return launch_pair(p, a.q, a.total_q, a.q_st, a.q_sh, a.k, a.v, a.total_k, a.kv_st, a.kv_sh, w.workers,
+                     (int64_t)w.max_list * p.nh, true, stream, "attn_varlen launch");
 }
 
 // Parts of the shared prefix: cut along the keys so that all pairs have work, in about equal rounds.
@@ -1244,9 +942,9 @@ int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int* keys_per_split) 
 
 int launch_attn_pair_prefix(const PackedAttnParams& a, cudaStream_t stream) {
   PairParams p = {};
-  p.v = a.v;
-  p.kv_st = a.kv_st;
-  p.kv_sh = a.kv_sh;
+  p.v = a.vp;
+  p.kv_st = a.kp_st;
+  p.kv_sh = a.kp_sh;
   p.Hq = a.Hq;
   p.G = a.G;
   pair_tile(p);
@@ -1255,14 +953,14 @@ int launch_attn_pair_prefix(const PackedAttnParams& a, cudaStream_t stream) {
   p.B = a.B;
   p.P = a.P;
   p.n_rt = (a.B + 2 * p.tpt - 1) / (2 * p.tpt);
-  p.n_splits = a.n_splits;
-  p.keys_per_split = a.keys_per_split;
+  p.n_splits = a.prefix_splits;
+  p.keys_per_split = a.prefix_keys;
   p.part_o = a.part_o;
   p.part_lse = a.part_lse;
   const int64_t items = (int64_t)p.n_rt * p.n_splits * p.nh;
   if (items > 0x3FFFFFFF) return set_error(kErrUnsupported, "attn_decode_shared: problem too large");
   const int pairs = (int)std::min<int64_t>(num_sms_current_device() / 2, items);
-  return launch_pair(p, a.q, a.B, a.q_st, a.q_sh, a.k, a.v, a.P, a.kv_st, a.kv_sh, pairs, items, false, stream,
+  return launch_pair(p, a.q, a.B, a.q_st, a.q_sh, a.kp, a.vp, a.P, a.kp_st, a.kp_sh, pairs, items, false, stream,
                      "attn_decode_shared prefix launch");
 }
 

@@ -32,7 +32,11 @@ constexpr int kThreads = 128;
 constexpr int kRingBytes = kStages * 2 * kTileBytes;
 constexpr int kSmemBytes = kRingBytes + 16;
 
-enum RowsMode : int { kModeVarlen = 0, kModePrefix = 1, kModeOwn = 2 };
+enum RowsMode : int {
+  kModeVarlen = 0,  // packed sequences, every tile found from the offsets
+  kModeList = 1,    // packed sequences, items of a plan (attn_plan.cu)
+  kModeShared = 2   // shared prefix (the first prefix_blocks blocks) and own keys
+};
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -147,35 +151,62 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
   const int gn = min(p.Gs, p.G - g0);
   const int tpt = kRows / p.Gs;  // tokens per tile
 
+  grid_launch_dependents();
   RowsItem it;
+  const __nv_bfloat16 *kp = p.k, *vp = p.v;
+  int64_t kv_st = p.kv_st;
+  int64_t part = -1;  // part row of token 0, head 0 of the slice, or -1: the output itself
+  int part_ts = p.Hq;
   if constexpr (MODE == kModeVarlen) {
     if (!find_tile(p, tpt, blockIdx.x, it)) return;
     it.kv_off += hkv * p.kv_sh;
-  } else if constexpr (MODE == kModePrefix) {
-    const int tile = blockIdx.x / p.n_splits;
-    it.row0 = tile * tpt;
-    it.n_tok = min(tpt, p.B - it.row0);
-    it.kv_off = hkv * p.kv_sh;
-    it.kb = (blockIdx.x % p.n_splits) * p.keys_per_split;
-    it.ke = min(p.P, it.kb + p.keys_per_split);
-    it.lim0 = p.P;
+  } else if constexpr (MODE == kModeList) {
+    grid_dependency_wait();
+    if ((int)blockIdx.x >= __ldcg(p.header)) return;
+    const int4 a = __ldcg(p.list + 2 * blockIdx.x), c = __ldcg(p.list + 2 * blockIdx.x + 1);
+    it.row0 = a.x;
+    it.n_tok = a.y;
+    it.kv_off = (int64_t)a.z * p.kv_st + hkv * p.kv_sh;
+    it.kb = a.w;
+    it.ke = c.x;
+    it.lim0 = c.y;
+    part_ts = p.Gs;
+    if (c.z >= 0) part = (int64_t)c.z + (int64_t)blockIdx.y * a.y * p.Gs;
   } else {
-    it.row0 = blockIdx.x / p.n_splits;
-    it.n_tok = 1;
-    it.kv_off = it.row0 * p.kv_sb + hkv * p.kv_sh;
-    const int len = p.lens != nullptr ? max(0, min(p.cap, __ldg(p.lens + it.row0))) : p.cap;
-    it.kb = (blockIdx.x % p.n_splits) * p.keys_per_split;
-    it.ke = min(len, it.kb + p.keys_per_split);
-    it.lim0 = p.cap;
+    int split;
+    if ((int)blockIdx.x < p.prefix_blocks) {
+      const int tile = blockIdx.x / p.prefix_splits;
+      split = blockIdx.x - tile * p.prefix_splits;
+      it.row0 = tile * tpt;
+      it.n_tok = min(tpt, p.B - it.row0);
+      it.kv_off = hkv * p.kp_sh;
+      it.kb = split * p.prefix_keys;
+      it.ke = min(p.P, it.kb + p.prefix_keys);
+      kp = p.kp;
+      vp = p.vp;
+      kv_st = p.kp_st;
+    } else {
+      const int x = blockIdx.x - p.prefix_blocks;
+      it.row0 = x / p.own_splits;
+      split = x - it.row0 * p.own_splits;
+      it.n_tok = 1;
+      it.kv_off = it.row0 * p.kv_sb + hkv * p.kv_sh;
+      it.kb = split * p.own_keys;
+      const int len = p.lens != nullptr ? max(0, min(p.cap, __ldg(p.lens + it.row0))) : p.cap;
+      it.ke = min(len, it.kb + p.own_keys);
+      split += p.prefix_splits;
+    }
+    it.lim0 = 0x3FFFFFFF;
+    part = ((int64_t)split * p.B + it.row0) * p.Hq + hkv * p.G + g0;
   }
   // tiles from this one on hold keys that some rows see and others do not
-  const int diag_tile = MODE == kModeVarlen && it.n_tok > 1 ? max(0, it.lim0 + 1 - it.kb) / kTileKeys : 0x7FFFFFFF;
+  const int diag_tile = MODE != kModeShared && it.n_tok > 1 ? max(0, it.lim0 + 1 - it.kb) / kTileKeys : 0x7FFFFFFF;
   volatile int* bad_v = reinterpret_cast<volatile int*>(smem + kRingBytes);
   if (threadIdx.x == 0) *bad_v = 0;
   const int n_tiles = it.ke > it.kb ? (it.ke - it.kb + kTileKeys - 1) / kTileKeys : 0;
 
-  const __nv_bfloat16* kp = p.k + it.kv_off;
-  const __nv_bfloat16* vp = p.v + it.kv_off;
+  kp += it.kv_off;
+  vp += it.kv_off;
   const uint32_t s_base = smem_u32(smem);
   auto load_tile = [&](int i) {
     if (i < n_tiles) {
@@ -186,7 +217,7 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
         const int id = c * kThreads + threadIdx.x;
         const int row = id >> 4, ch = id & 15;
         const bool live = key0 + row < it.ke;
-        const int64_t off = live ? (int64_t)(key0 + row) * p.kv_st + ch * 8 : 0;
+        const int64_t off = live ? (int64_t)(key0 + row) * kv_st + ch * 8 : 0;
         cp_async16(ks + tile_off(row, ch), kp + off, live);
         cp_async16(ks + kTileBytes + tile_off(row, ch), vp + off, live);
       }
@@ -229,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
 
   for (int i = 0; i < n_tiles; ++i) {
     cp_async_wait<kStages - 2>();
-    if (MODE == kModeVarlen && i >= diag_tile) {
+    if (MODE != kModeShared && i >= diag_tile) {
       // this thread's own copies are visible to it before the barrier
 #pragma unroll
       for (int c = 0; c < kTileKeys * 16 / kThreads; ++c) {
@@ -312,144 +343,151 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_consta
       }
     }
   }
-  if (MODE == kModeVarlen && n_tiles > diag_tile && *bad_v) {
-    // rare: the infinities and NaNs taken out above go to the rows that see them
-    for (int e = 0; e < 2; ++e) {
-      for (int j = it.kb + diag_tile * kTileKeys; row_ok[e] && j <= lim[e]; ++j) {
-        const __nv_bfloat16* src = vp + j * p.kv_st + kq;
-#pragma unroll
-        for (int dt = 0; dt < 16; ++dt) {
-          const uint32_t x = *reinterpret_cast<const uint32_t*>(src + dt * 8);
-          if ((x & 0x7F80u) == 0x7F80u) o[dt][2 * e] += bf16lo_to_f32(x);
-          if ((x & 0x7F800000u) == 0x7F800000u) o[dt][2 * e + 1] += bf16hi_to_f32(x);
-        }
-      }
-    }
-  }
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
   }
+  cp_async_wait<0>();
+  // Started beside the prefix's kernel, this one must not end before it: whatever comes next waits for this one only.
+  if (MODE == kModeShared && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) grid_dependency_wait();
 
   if constexpr (WK > 1) {
-    // merge the warps that hold other keys of the same rows
-    cp_async_wait<0>();
+    // The four warps hold other keys of the same rows: through shared memory, then eight threads per row
+    static_assert(WM == 1, "16 rows");
     __syncthreads();
-    float* so = reinterpret_cast<float*>(smem);            // [4][16][128]
-    float* sm = so + 4 * 16 * kHeadDim;                     // [4][16][2]
+    float* so = reinterpret_cast<float*>(smem);     // [4][16][128]
+    float* sm = so + 4 * 16 * kHeadDim;              // [4][16][2]
+    const int r0 = lane >> 2;
 #pragma unroll
     for (int dt = 0; dt < 16; ++dt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<float2*>(so + (warp * 16 + (lane >> 2) + 8 * e) * kHeadDim + dt * 8 + kq) =
+        *reinterpret_cast<float2*>(so + (warp * 16 + r0 + 8 * e) * kHeadDim + ((dt ^ r0) * 8 + kq)) =
             make_float2(o[dt][2 * e], o[dt][2 * e + 1]);
     }
     if ((lane & 3) == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        sm[(warp * 16 + (lane >> 2) + 8 * e) * 2] = m[e];
-        sm[(warp * 16 + (lane >> 2) + 8 * e) * 2 + 1] = l[e];
+        sm[(warp * 16 + r0 + 8 * e) * 2] = m[e];
+        sm[(warp * 16 + r0 + 8 * e) * 2 + 1] = l[e];
       }
     }
     __syncthreads();
-    if (wk != 0) return;
+    const int row = threadIdx.x >> 3, seg = threadIdx.x & 7;  // channels [16 seg, 16 seg + 16)
+    const int i = row / p.Gs, g = row - i * p.Gs;
+    const bool live_row = i < it.n_tok && g < gn;
+    const int64_t tok0 = it.row0 + i;
+    const int head0 = hkv * p.G + g0 + g;
+    const int lim_row = min(it.ke - 1, it.lim0 + i);
+    float L = 0.f, M = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = (lane >> 2) + 8 * e;
-      float M = -INFINITY;
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[(w * 16 + row) * 2]);
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float wt[4];
 #pragma unroll
-      for (int w = 0; w < WK; ++w) M = fmaxf(M, sm[((w * WM + wm) * 16 + r) * 2]);
-      const float Ms = M == -INFINITY ? 0.f : M;
-      float L = 0.f, wt[WK];
+    for (int w = 0; w < 4; ++w) {
+      wt[w] = fast_exp2(sm[(w * 16 + row) * 2] - Ms);
+      L += wt[w] * sm[(w * 16 + row) * 2 + 1];
+    }
+    if (!live_row) return;
+    float acc[16];
 #pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        wt[w] = fast_exp2(sm[((w * WM + wm) * 16 + r) * 2] - Ms);
-        L += wt[w] * sm[((w * WM + wm) * 16 + r) * 2 + 1];
-      }
-      m[e] = M;
-      l[e] = L;
+    for (int c = 0; c < 16; ++c) acc[c] = 0.f;
 #pragma unroll
-      for (int dt = 0; dt < 16; ++dt) {
-        float a = 0.f, b = 0.f;
+    for (int w = 0; w < 4; ++w) {
 #pragma unroll
-        for (int w = 0; w < WK; ++w) {
-          const float2 x = *reinterpret_cast<const float2*>(so + ((w * WM + wm) * 16 + r) * kHeadDim + dt * 8 + kq);
-          a += wt[w] * x.x;
-          b += wt[w] * x.y;
-        }
-        o[dt][2 * e] = a;
-        o[dt][2 * e + 1] = b;
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int dt = seg * 2 + (q4 >> 1);
+        const float4 x = *reinterpret_cast<const float4*>(so + (w * 16 + row) * kHeadDim + (dt ^ (row & 7)) * 8 + (q4 & 1) * 4);
+        acc[q4 * 4 + 0] = fmaf(wt[w], x.x, acc[q4 * 4 + 0]);
+        acc[q4 * 4 + 1] = fmaf(wt[w], x.y, acc[q4 * 4 + 1]);
+        acc[q4 * 4 + 2] = fmaf(wt[w], x.z, acc[q4 * 4 + 2]);
+        acc[q4 * 4 + 3] = fmaf(wt[w], x.w, acc[q4 * 4 + 3]);
       }
     }
-  }
+    if (MODE != kModeShared && n_tiles > diag_tile && *bad_v) {
+      // rare: the infinities and NaNs taken out above go to the rows that see them
+      for (int j = it.kb + diag_tile * kTileKeys; j <= lim_row; ++j) {
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (!row_ok[e]) continue;
-    const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];  // a row that sees no key gives zeros
-    const float lse2 = l[e] == 0.f ? -INFINITY : m[e] + log2f(l[e]);
-    if constexpr (MODE == kModeVarlen) {
+        for (int c = 0; c < 16; ++c) {
+          const float x = __bfloat162float(vp[j * kv_st + seg * 16 + c]);
+          if (!(fabsf(x) <= 3.4e38f)) acc[c] += x;
+        }
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees no key gives zeros
+    const float lse2 = L == 0.f ? -INFINITY : M + __log2f(L);
+    if (part < 0) {
+      uint4* dst = reinterpret_cast<uint4*>(p.o + tok0 * p.o_st + head0 * p.o_sh + seg * 16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        dst[h] = make_uint4(pack_bf16x2(acc[h * 8 + 0] * inv, acc[h * 8 + 1] * inv),
+                            pack_bf16x2(acc[h * 8 + 2] * inv, acc[h * 8 + 3] * inv),
+                            pack_bf16x2(acc[h * 8 + 4] * inv, acc[h * 8 + 5] * inv),
+                            pack_bf16x2(acc[h * 8 + 6] * inv, acc[h * 8 + 7] * inv));
+      if (seg == 0 && p.lse != nullptr) p.lse[tok0 * p.lse_st + head0 * p.lse_sh] = lse2 * 0.69314718055994531f;
+    } else {
+      const int64_t rec = part + (int64_t)i * part_ts + g;
+      if (L != 0.f) {
+        float4* dst = reinterpret_cast<float4*>(p.part_o + rec * kHeadDim + seg * 16);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          dst[c] = make_float4(acc[c * 4] * inv, acc[c * 4 + 1] * inv, acc[c * 4 + 2] * inv, acc[c * 4 + 3] * inv);
+      }
+      if (seg == 0) p.part_lse[rec] = lse2;
+    }
+  } else {
+    static_assert(MODE == kModeVarlen, "whole rows");
+    if (n_tiles > diag_tile && *bad_v) {
+      // rare, as above
+      for (int e = 0; e < 2; ++e) {
+        for (int j = diag_tile * kTileKeys; row_ok[e] && j <= lim[e]; ++j) {
+          const __nv_bfloat16* src = vp + j * kv_st + kq;
+#pragma unroll
+          for (int dt = 0; dt < 16; ++dt) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(src + dt * 8);
+            if ((x & 0x7F80u) == 0x7F80u) o[dt][2 * e] += bf16lo_to_f32(x);
+            if ((x & 0x7F800000u) == 0x7F800000u) o[dt][2 * e + 1] += bf16hi_to_f32(x);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (!row_ok[e]) continue;
+      const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
       __nv_bfloat16* dst = p.o + tok[e] * p.o_st + head[e] * p.o_sh + kq;
 #pragma unroll
       for (int dt = 0; dt < 16; ++dt)
         *reinterpret_cast<uint32_t*>(dst + dt * 8) = pack_bf16x2(o[dt][2 * e] * inv, o[dt][2 * e + 1] * inv);
       if ((lane & 3) == 0 && p.lse != nullptr)
-        p.lse[tok[e] * p.lse_st + head[e] * p.lse_sh] = lse2 * 0.69314718055994531f;
-    } else {
-      const int part = p.part0 + blockIdx.x % p.n_splits;
-      const int64_t rec = (int64_t)part * p.B * p.Hq + (int64_t)tok[e] * p.Hq + head[e];
-      if (l[e] != 0.f) {
-        float* dst = p.part_o + rec * kHeadDim + kq;
-#pragma unroll
-        for (int dt = 0; dt < 16; ++dt)
-          *reinterpret_cast<float2*>(dst + dt * 8) = make_float2(o[dt][2 * e] * inv, o[dt][2 * e + 1] * inv);
-      }
-      if ((lane & 3) == 0) p.part_lse[rec] = lse2;
+        p.lse[tok[e] * p.lse_st + head[e] * p.lse_sh] =
+            l[e] == 0.f ? -INFINITY : (m[e] + __log2f(l[e])) * 0.69314718055994531f;
     }
   }
 }
 
-// Joins the parts of every row: one warp per (request, query head).
-__global__ void __launch_bounds__(256) join_parts_kernel(const __grid_constant__ PackedAttnParams p, int n_parts) {
-  const int row = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = lane_id();
+// Joins prefix and own parts of every request: one warp per (request, query head).
+__global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__ PackedAttnParams p, int n_parts) {
+  grid_dependency_wait();
+  const int row = blockIdx.x * 4 + warp_id();
   const int rows = p.B * p.Hq;
   if (row >= rows) return;
-  float M = -INFINITY;
-  for (int s = 0; s < n_parts; ++s) {
-    const float x = p.part_lse[(int64_t)s * rows + row];
-    M = x != x ? x : fmaxf(M, x);  // a NaN stays
-  }
-  const float Ms = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < n_parts; ++s) {
-    const float x = p.part_lse[(int64_t)s * rows + row];
-    if (x == -INFINITY) continue;  // this part saw no key: nothing was written
-    const float w = fast_exp2(x - Ms);
-    const float4 v = reinterpret_cast<const float4*>(p.part_o + ((int64_t)s * rows + row) * kHeadDim)[lane];
-    L += w;
-    acc.x += w * v.x;
-    acc.y += w * v.y;
-    acc.z += w * v.z;
-    acc.w += w * v.w;
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int b = row / p.Hq, h = row % p.Hq;
-  reinterpret_cast<uint2*>(p.o + b * p.o_st + h * p.o_sh)[lane] =
-      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-  if (lane == 0 && p.lse != nullptr)
-    p.lse[b * p.lse_st + h * p.lse_sh] = L == 0.f ? -INFINITY : (Ms + log2f(L)) * 0.69314718055994531f;
+  const int b = row / p.Hq, h = row - b * p.Hq;
+  join_row(p.part_o + (int64_t)row * kHeadDim, p.part_lse + row, rows, n_parts, p.o + b * p.o_st + h * p.o_sh,
+           p.lse == nullptr ? nullptr : p.lse + b * p.lse_st + h * p.lse_sh);
 }
 
 template <int WM, int MODE>
-int launch_rows(const PackedAttnParams& p, int64_t gx, cudaStream_t stream, const char* what) {
+int launch_rows(const PackedAttnParams& p, int64_t gx, bool dependent, cudaStream_t stream, const char* what) {
   auto kern = attn_rows_kernel<WM, MODE>;
   int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes), what);
   if (rc) return rc;
   if (gx > 0x7FFFFFFF) return set_error(kErrUnsupported, std::string(what) + ": problem too large");
-  kern<<<dim3((unsigned)gx, (unsigned)(p.Hkv * p.n_gs)), kThreads, kSmemBytes, stream>>>(p);
-  return check_cuda(cudaGetLastError(), what);
+  return check_cuda(launch_after(kern, dim3((unsigned)gx, (unsigned)(p.Hkv * p.n_gs)), kThreads, kSmemBytes, dependent,
+                                 stream, p),
+                    what);
 }
 
 void slice_group(PackedAttnParams& p, int rows) {
@@ -457,11 +495,21 @@ void slice_group(PackedAttnParams& p, int rows) {
   p.Gs = (p.G + p.n_gs - 1) / p.n_gs;
 }
 
-// Which kernel takes a packed batch. Macro for now.
-#ifndef FMKA_VARLEN_ROWS_MAX
-#define FMKA_VARLEN_ROWS_MAX 0
+// How a packed batch runs.
+enum class VarlenPath { kShort, kThin, kPair };
+
+VarlenPath varlen_path(int n_seqs, int total_q, int max_k, int G) {
+#ifdef FMKA_VARLEN_PATH
+  return static_cast<VarlenPath>(FMKA_VARLEN_PATH);
 #endif
-bool varlen_by_rows(int total_q, int max_k) { return (int64_t)total_q * max_k < FMKA_VARLEN_ROWS_MAX || max_k == 0; }
+  if ((int64_t)total_q * max_k < (1 << 16)) return VarlenPath::kShort;
+  return (int64_t)total_q * G <= (int64_t)n_seqs * 16 ? VarlenPath::kThin : VarlenPath::kPair;
+}
+
+PackedPlan thin_plan(int n_seqs, int total_q, int max_k, int Hkv, PackedAttnParams& p) {
+  slice_group(p, 16);
+  return packed_plan(n_seqs, total_q, max_k, Hkv, p.G, p.Gs, 16 / p.Gs, 2 * num_sms_current_device());
+}
 
 struct SharedPlan {
   int prefix_splits, prefix_keys;  // parts over the prefix, keys per part
@@ -474,6 +522,11 @@ SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
   if (P > 0) {
     s.pair = true;
     s.prefix_splits = attn_pair_prefix_splits(B, Hq, Hkv, P, &s.prefix_keys);
+#ifdef FMKA_SHARED_ROWS
+    s.pair = false;
+    s.prefix_keys = 256;
+    s.prefix_splits = (P + s.prefix_keys - 1) / s.prefix_keys;
+#endif
   }
   if (cap > 0) {
     s.own_keys = 512;
@@ -485,17 +538,39 @@ SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
 }  // namespace
 
 size_t attn_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv) {
-  return varlen_by_rows(total_q, max_k) ? 0 : attn_pair_varlen_workspace_bytes(n_seqs, total_q, max_k, Hq, Hkv);
+  PackedAttnParams p = {};
+  p.G = Hq / Hkv;
+  switch (varlen_path(n_seqs, total_q, max_k, p.G)) {
+    case VarlenPath::kShort: return 0;
+    case VarlenPath::kThin: return thin_plan(n_seqs, total_q, max_k, Hkv, p).total;
+    default: return attn_pair_plan(n_seqs, total_q, max_k, Hq, Hkv).total;
+  }
 }
 
 int launch_attn_varlen(PackedAttnParams p, int max_k, void* workspace, cudaStream_t stream) {
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_varlen: device status word unavailable");
-  if (!varlen_by_rows(p.total_q, max_k) && p.total_k > 0) return launch_attn_pair_varlen(p, max_k, workspace, stream);
-  slice_group(p, 64);
-  const int tpt = 64 / p.Gs;
-  const int64_t tiles = (int64_t)p.total_q / tpt + p.n_seqs;  // at least one tile ends in every sequence
-  return launch_rows<4, kModeVarlen>(p, tiles, stream, "attn_varlen launch");
+  const VarlenPath path = varlen_path(p.n_seqs, p.total_q, max_k, p.G);
+  if (path == VarlenPath::kShort || p.total_k == 0) {
+    slice_group(p, 64);
+    const int tpt = 64 / p.Gs;
+    const int64_t tiles = (int64_t)p.total_q / tpt + p.n_seqs;  // at least one tile ends in every sequence
+    return launch_rows<4, kModeVarlen>(p, tiles, false, stream, "attn_varlen launch");
+  }
+  PackedPlan w = path == VarlenPath::kThin ? thin_plan(p.n_seqs, p.total_q, max_k, p.Hkv, p)
+                                           : attn_pair_plan(p.n_seqs, p.total_q, max_k, p.Hq, p.Hkv);
+  int rc = launch_plan(p, w, workspace, stream);
+  if (rc) return rc;
+  if (path == VarlenPath::kThin) {
+    p.header = w.header;
+    p.list = w.list;
+    p.part_o = w.part_o;
+    p.part_lse = w.part_lse;
+    rc = launch_rows<1, kModeList>(p, w.max_list, true, stream, "attn_varlen launch");
+  } else {
+    rc = launch_attn_pair_varlen(p, w, stream);
+  }
+  return rc ? rc : launch_join(p, w, stream);
 }
 
 size_t attn_decode_shared_workspace_bytes(int B, int Hq, int Hkv, int P, int cap) {
@@ -503,46 +578,35 @@ size_t attn_decode_shared_workspace_bytes(int B, int Hq, int Hkv, int P, int cap
   return (size_t)(s.prefix_splits + s.own_splits) * B * Hq * (kHeadDim + 1) * sizeof(float);
 }
 
-int launch_attn_decode_shared(PackedAttnParams p, const __nv_bfloat16* kp, const __nv_bfloat16* vp, int64_t kp_sh,
-                              int64_t kp_st, void* workspace, cudaStream_t stream) {
+int launch_attn_decode_shared(PackedAttnParams p, void* workspace, cudaStream_t stream) {
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_decode_shared: device status word unavailable");
   const SharedPlan s = plan_shared(p.B, p.Hq, p.Hkv, p.P, p.cap);
   const int parts = s.prefix_splits + s.own_splits;
   p.part_o = static_cast<float*>(workspace);
   p.part_lse = p.part_o + (int64_t)parts * p.B * p.Hq * kHeadDim;
-  if (s.prefix_splits > 0) {
-    PackedAttnParams a = p;
-    a.k = kp;
-    a.v = vp;
-    a.kv_sh = kp_sh;
-    a.kv_st = kp_st;
-    a.n_splits = s.prefix_splits;
-    a.keys_per_split = s.prefix_keys;
-    a.part0 = 0;
-    int rc;
-    if (s.pair) {
-      rc = launch_attn_pair_prefix(a, stream);
-    } else {
-      slice_group(a, 64);
-      const int tpt = 64 / a.Gs;
-      rc = launch_rows<4, kModePrefix>(a, (int64_t)((a.B + tpt - 1) / tpt) * a.n_splits, stream,
-                                       "attn_decode_shared prefix launch");
-    }
+  p.prefix_splits = s.prefix_splits;
+  p.prefix_keys = s.prefix_keys;
+  p.own_splits = s.own_splits;
+  p.own_keys = s.own_keys;
+  if (s.pair) {
+    const int rc = launch_attn_pair_prefix(p, stream);
     if (rc) return rc;
   }
-  if (s.own_splits > 0) {
-    PackedAttnParams a = p;
-    a.n_splits = s.own_splits;
-    a.keys_per_split = s.own_keys;
-    a.part0 = s.prefix_splits;
-    slice_group(a, 16);
-    int rc = launch_rows<1, kModeOwn>(a, (int64_t)a.B * a.n_splits, stream, "attn_decode_shared own launch");
+  slice_group(p, 16);
+  const int tpt = 16 / p.Gs;
+  p.prefix_blocks = s.pair ? 0 : (p.B + tpt - 1) / tpt * s.prefix_splits;
+  const int64_t blocks = p.prefix_blocks + (int64_t)p.B * s.own_splits;
+  if (blocks > 0) {
+    // Behind the pair kernel it depends on nothing of it and does not wait: its blocks fill what SMs the other
+    // leaves free.
+    const int rc = launch_rows<1, kModeShared>(p, blocks, s.pair, stream, "attn_decode_shared launch");
     if (rc) return rc;
   }
-  const int blocks = (p.B * p.Hq + 7) / 8;
-  join_parts_kernel<<<blocks, 256, 0, stream>>>(p, parts);
-  return check_cuda(cudaGetLastError(), "attn_decode_shared join launch");
+  const int64_t rows = (int64_t)p.B * p.Hq;
+  return check_cuda(launch_after(join_parts_kernel, dim3((unsigned)((rows + 3) / 4)), 128, 0, true, stream,
+                                 p, parts),
+                    "attn_decode_shared join launch");
 }
 
 }  // namespace fmka

@@ -65,8 +65,7 @@ int launch_qk_norm_rope(QkNormParams p, cudaStream_t stream);
 size_t attn_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv);
 int launch_attn_varlen(PackedAttnParams p, int max_k, void* workspace, cudaStream_t stream);
 size_t attn_decode_shared_workspace_bytes(int B, int Hq, int Hkv, int P, int cap);
-int launch_attn_decode_shared(PackedAttnParams p, const __nv_bfloat16* kp, const __nv_bfloat16* vp, int64_t kp_sh,
-                              int64_t kp_st, void* workspace, cudaStream_t stream);
+int launch_attn_decode_shared(PackedAttnParams p, void* workspace, cudaStream_t stream);
 
 // ----------------------------------------------------------------- errors --
 namespace {
@@ -829,7 +828,11 @@ int fmka_attn_decode_shared(const void* q, int64_t q_sb, int64_t q_sh, const voi
     return set_error(kErrWorkspace,
                      "attn_decode_shared: workspace too small (need " + std::to_string(need) + " bytes)");
   if (!al16(workspace)) return set_error(kErrInvalidArgument, "attn_decode_shared: workspace must be 16-byte aligned");
-  return launch_attn_decode_shared(p, bf(k_prefix), bf(v_prefix), p_sh, p_st, workspace, as_stream(stream));
+  p.kp = bf(k_prefix);
+  p.vp = bf(v_prefix);
+  p.kp_sh = p_sh;
+  p.kp_st = p_st;
+  return launch_attn_decode_shared(p, workspace, as_stream(stream));
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <utility>
 
 namespace fmka {
 
@@ -149,21 +150,66 @@ struct PackedAttnParams {
   const int* cu_q;
   const int* cu_k;
   int n_seqs, total_q, total_k, causal;
+  // packed sequences with a plan (attn_plan.cu)
+  const int* header;
+  const int4* list;
   // shared prefix / own keys
+  const __nv_bfloat16* kp;     // prefix[head, key, :]
+  const __nv_bfloat16* vp;
+  int64_t kp_sh, kp_st;
   int B, P, cap;
-  const int* lens;             // keys of each request, may be null (all cap)
-  int keys_per_split, n_splits;
-  int part0;                   // index of this launch's first part
+  const int* lens;             // own keys of each request, may be null (all cap)
+  int prefix_splits, prefix_keys, prefix_blocks;  // parts of the prefix, keys of a part
+  int own_splits, own_keys;
   float* part_o;               // [parts][B * Hq][128]
   float* part_lse;             // [parts][B * Hq] log2-sum-exp
   uint32_t* status;
 };
 
+// How a packed batch is cut into items, and where the item list, the parts of rows whose keys are cut and what joins
+// them lie in the scratch memory (attn_plan.cu).
+struct PackedPlan {
+  int n_gs, Gs, nh;      // slices of a kv head's group, heads of a slice, kv heads x slices
+  int tok_tile;          // tokens per item
+  int workers;           // CTAs (or pairs) that share the work
+  int split;             // items may be cut along their keys
+  int max_list, max_parts;
+  int64_t part_rows;
+  size_t at_seq, at_list, at_groups, at_part_o, at_part_lse, total;
+  int* header;           // [0] list entries, [1] groups of parts
+  int* seq_tiles;        // [n_seqs + 1] tiles before each sequence
+  int4* list;            // {q0, nq, k0, kb}, {ke, lim0, first part row or -1, 0}, heavy ones first
+  int4* groups;          // {q0, nq, parts, first part row}
+  float* part_o;         // [part_rows][128] normalised
+  float* part_lse;       // [part_rows] log2-sum-exp
+};
+PackedPlan packed_plan(int n_seqs, int total_q, int max_k, int Hkv, int G, int Gs, int tok_tile, int workers);
+int launch_plan(const PackedAttnParams& a, PackedPlan& w, void* workspace, cudaStream_t stream);
+int launch_join(const PackedAttnParams& a, const PackedPlan& w, cudaStream_t stream);
+
 // attn_pair.cu: the tcgen05 form for many rows.
-size_t attn_pair_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv);
-int launch_attn_pair_varlen(const PackedAttnParams& a, int max_k, void* workspace, cudaStream_t stream);
+PackedPlan attn_pair_plan(int n_seqs, int total_q, int max_k, int Hq, int Hkv);
+int launch_attn_pair_varlen(const PackedAttnParams& a, const PackedPlan& w, cudaStream_t stream);
 int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int* keys_per_split);
 int launch_attn_pair_prefix(const PackedAttnParams& a, cudaStream_t stream);
+
+// Launch that may start while the kernel before it in the stream still runs (that kernel lets it, and it waits itself
+// before it reads what the other writes).
+template <class... Params, class... Args>
+cudaError_t launch_after(void (*kern)(Params...), dim3 grid, int threads, size_t smem, bool dependent,
+                         cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
 
 // Device status word used by kernels to report bounded-wait timeouts; one per
 // device, allocated lazily.

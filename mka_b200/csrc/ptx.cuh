@@ -556,4 +556,46 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
+// Joins the parts of one attention row (a warp): normalised outputs [n][row_stride][128] and log2-sum-exps
+// [n][row_stride] of its key ranges. A lane holds the weight of one part, the outputs are summed four parts at a time;
+// a part that saw no key (-inf) wrote no output and is not read. Read past L1, as the parts may come from a kernel
+// that was still running when this one started.
+__device__ __forceinline__ void join_row(const float* part_o, const float* part_lse, int64_t row_stride, int n,
+                                         __nv_bfloat16* o, float* lse) {
+  const int lane = lane_id();
+  float M = -INFINITY;
+  for (int s = lane; s < n; s += 32) M = fmaxf(M, __ldcg(part_lse + s * row_stride));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  const float Ms = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    const float x = s0 + lane < n ? __ldcg(part_lse + (s0 + lane) * row_stride) : -INFINITY;
+    const float mine = x == -INFINITY ? 0.f : fast_exp2(x - Ms);
+    const unsigned seen = __ballot_sync(0xffffffffu, x != -INFINITY);
+    for (int s1 = 0; s1 < min(32, n - s0); s1 += 4) {
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = seen >> (s1 + k) & 1
+                   ? __ldcg(reinterpret_cast<const float4*>(part_o + (s0 + s1 + k) * row_stride * 128) + lane)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float w = __shfl_sync(0xffffffffu, mine, s1 + k);
+        L += w;
+        acc.x = fmaf(w, v[k].x, acc.x);
+        acc.y = fmaf(w, v[k].y, acc.y);
+        acc.z = fmaf(w, v[k].z, acc.z);
+        acc.w = fmaf(w, v[k].w, acc.w);
+      }
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  reinterpret_cast<uint2*>(o)[lane] =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (lane == 0 && lse != nullptr) *lse = L == 0.f ? -INFINITY : (Ms + __log2f(L)) * 0.69314718055994531f;
+}
+
 }  // namespace fmka
