@@ -136,7 +136,7 @@ __device__ __forceinline__ bool find_tile(const PackedAttnParams& p, int tok_per
 }
 
 template <int WM, int MODE>
-__global__ void __launch_bounds__(kThreads) attn_rows_kernel(const __grid_constant__ PackedAttnParams p) {
+__global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_constant__ PackedAttnParams p) {
   constexpr int WK = 4 / WM;
   constexpr int kRows = 16 * WM;
   constexpr int kWarpKeys = kTileKeys / WK;  // keys of a tile per warp
