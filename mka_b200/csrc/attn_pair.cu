@@ -63,10 +63,6 @@ constexpr int kTileSmem = 2 * kQBytes + kKStages * kKBytes + kVStages * kVBytes 
 constexpr int kMaxItems = 128;         // items of a pair in one launch
 constexpr int kCtrlBytes = 5 * 1024 + 512;
 constexpr int kSmemBytes = kTileSmem + kCtrlBytes + kMaxItems * 48;
-#ifndef FMKA_PE
-#define FMKA_PE 100
-#endif
-constexpr int kPolyEvery = FMKA_PE;   // one pair of exponentials in so many runs on the FMA pipe
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr uint32_t kTmemO = 0, kTmemS = 128, kTmemP = 384;  // S: 2 x 128 columns, P: 2 x 64
 // Register split between the control warps and the softmax warps (setmaxnreg);
@@ -193,24 +189,6 @@ struct Ring {
     }
   }
 };
-
-// 2^x for a pair on the FMA pipe: x = n + f with n = round(x), 2^f on [-1/2, 1/2] from a degree-5 polynomial fitted
-// here by Remez exchange on the relative error (7.5e-8 in exact arithmetic, 2.1e-7 in fp32, about what ex2.approx
-// has), times 2^n built from the exponent bits. Below -126.5 that factor is zero; NaN stays NaN.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  const float2 c = make_float2(fmax_nan(x.x, -127.0f), fmax_nan(x.y, -127.0f));
-  const float2 t = fadd2(c, make_float2(12582912.0f, 12582912.0f));
-  const float2 n = fadd2(t, make_float2(-12582912.0f, -12582912.0f));
-  const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), c);
-  float2 p = ffma2(make_float2(1.3276472e-3f, 1.3276472e-3f), f, make_float2(9.675541e-3f, 9.675541e-3f));
-  p = ffma2(p, f, make_float2(5.5507133e-2f, 5.5507133e-2f));
-  p = ffma2(p, f, make_float2(0.24022120f, 0.24022120f));
-  p = ffma2(p, f, make_float2(0.69314697f, 0.69314697f));
-  p = ffma2(p, f, make_float2(1.0000001f, 1.0000001f));
-  const float2 e = make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3F800000),
-                               __int_as_float((__float_as_int(t.y) << 23) + 0x3F800000));
-  return fmul2(p, e);
-}
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     attn_pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -781,8 +759,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int c = 0; c < 16; ++c) {
             const float2 xx =
                 ffma2(make_float2(__uint_as_float(sc[2 * c]), __uint_as_float(sc[2 * c + 1])), sl2, nm2);
-            const float2 pp =
-                (c % kPolyEvery) == kPolyEvery - 1 ? exp2_poly(xx) : make_float2(fast_exp2(xx.x), fast_exp2(xx.y));
+            const float2 pp = make_float2(fast_exp2(xx.x), fast_exp2(xx.y));
             acc[c & 3] = fadd2(acc[c & 3], pp);
             pk[c] = pack_bf16x2(pp.x, pp.y);
           }

@@ -439,11 +439,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
   return __all_sync(0xffffffffu, mbar_sleep(bar, parity, status));
 }
 
-// Whether the phase is complete, for a whole warp, without waiting long.
-__device__ __forceinline__ bool warp_ready(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
-}
-
 // Programmatic dependent launch: waits until the kernels before this one in the
 // stream have finished and their writes are visible / lets the next one start
 // its prologue.
@@ -535,13 +530,6 @@ __device__ __forceinline__ bool zero_nonfinite(uint4& c) {
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ float2 fmul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
-
-// Maximum that passes NaN on (fmaxf drops it).
-__device__ __forceinline__ float fmax_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 
 // Three-input maximum (one instruction on sm_100a).
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
