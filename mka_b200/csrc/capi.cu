@@ -665,6 +665,11 @@ int fmka_qk_norm_rope_bf16(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
   if (!al16(q) || !al16(k) || !al16(q_out) || !al16(k_out) || !al16(q_weight) || !al16(k_weight) || !al16(rope_cos) ||
       !al16(rope_sin))
     return set_error(kErrInvalidArgument, "qk_norm_rope: tensors must be 16-byte aligned");
+  // the stride of a dimension of one element says nothing
+  if (B == 1) q_sb = k_sb = qo_sb = ko_sb = 0;
+  if (T == 1) q_st = k_st = qo_st = ko_st = 0;
+  if (Hq == 1) q_sh = qo_sh = 0;
+  if (Hkv == 1) k_sh = ko_sh = 0;
   if ((q_sb | q_st | q_sh | k_sb | k_st | k_sh | qo_sb | qo_st | qo_sh | ko_sb | ko_st | ko_sh) & 7)
     return set_error(kErrInvalidArgument, "qk_norm_rope: strides must be multiples of 8 elements");
   if ((rope_sb | rope_st) & 3)
@@ -709,9 +714,14 @@ int fmka_qk_norm_rope_bf16(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
 }
 
 namespace {
-// What both packed attention entry points ask of their tensors.
-int check_packed_attn(const PackedAttnParams& p, int head_dim, float scale, const char* who) {
+// What both packed attention entry points ask of their tensors: `rows` of q, `keys` of k and v. The stride of a
+// dimension of one element says nothing and is dropped.
+int check_packed_attn(PackedAttnParams& p, int rows, int keys, int head_dim, float scale, const char* who) {
   const std::string w(who);
+  if (rows == 1) p.q_st = p.o_st = p.kv_sb = 0;
+  if (keys == 1) p.kv_st = 0;
+  if (p.Hq == 1) p.q_sh = p.o_sh = 0;
+  if (p.Hkv == 1) p.kv_sh = 0;
   if (p.Hq <= 0 || p.Hkv <= 0) return set_error(kErrInvalidArgument, w + ": empty shape");
   if (head_dim != 128) return set_error(kErrUnsupported, w + ": head_dim must be 128");
   if (p.Hq % p.Hkv != 0)
@@ -768,7 +778,7 @@ int fmka_attn_varlen(const void* q, int64_t q_st, int64_t q_sh, const void* k, c
   p.Hkv = Hkv;
   p.causal = causal;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const int rc = check_packed_attn(p, head_dim, scale, "attn_varlen");
+  const int rc = check_packed_attn(p, total_q, total_k, head_dim, scale, "attn_varlen");
   if (rc) return rc;
   p.G = Hq / Hkv;
   const size_t need = attn_varlen_workspace_bytes(n_seqs, total_q, max_k, Hq, Hkv);
@@ -817,8 +827,10 @@ int fmka_attn_decode_shared(const void* q, int64_t q_sb, int64_t q_sh, const voi
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.scale_log2 = scale * 1.4426950408889634f;
-  const int rc = check_packed_attn(p, head_dim, scale, "attn_decode_shared");
+  const int rc = check_packed_attn(p, B, Tcap, head_dim, scale, "attn_decode_shared");
   if (rc) return rc;
+  if (Hkv == 1) p_sh = 0;
+  if (P == 1) p_st = 0;
   if (((p_sh | p_st) & 7) || !al16(k_prefix) || !al16(v_prefix))
     return set_error(kErrInvalidArgument,
                      "attn_decode_shared: the prefix must be 16-byte aligned with strides % 8 == 0");

@@ -508,7 +508,7 @@ def _same_device(what: str, dev: torch.device, *ts: Optional[torch.Tensor]) -> N
 
 def _on_device(dev: torch.device, name: str, *args) -> None:
     """Calls entry point `name` with args and the current stream of `dev` behind them."""
-    fn = getattr(_lib.load(), name)
+    fn = getattr(_lib._lib or _lib.load(), name)
     if dev.index == torch.cuda.current_device():
         rc = fn(*args, _raw_stream(dev.index))
     else:
@@ -565,14 +565,14 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
     if q.dtype is not _BF16 or (k is not None and k.dtype is not _BF16):
         _check_bf16(q, k)
     _same_device("qk_norm_rope", dev, k, q_weight, k_weight, positions)
-    qs, qst = q.shape, _strides(q)
+    qs, qst = q.shape, q.stride()
     nd = len(qs)
-    if nd not in (3, 4) or qs[-1] != HEAD_DIM or q.stride(-1) != 1:
+    if nd not in (3, 4) or qs[-1] != HEAD_DIM or qst[-1] != 1:
         raise RuntimeError("qk_norm_rope: q must be [T, Hq, 128] or [B, T, Hq, 128] with contiguous channels")
-    Hkv, kst = 0, None
+    Hkv, kst = 0, (0,) * nd
     if k is not None:
-        ks, kst = k.shape, _strides(k)
-        if len(ks) != nd or ks[:-2] != qs[:-2] or ks[-1] != HEAD_DIM or k.stride(-1) != 1:
+        ks, kst = k.shape, k.stride()
+        if len(ks) != nd or ks[:-2] != qs[:-2] or ks[-1] != HEAD_DIM or kst[-1] != 1:
             raise RuntimeError("qk_norm_rope: k must be q's shape with Hkv heads and contiguous channels")
         Hkv = ks[-2]
     w_f32 = 0
@@ -617,30 +617,27 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
         return q_out, k_out
     if Hq == 0:
         raise RuntimeError("qk_norm_rope: q needs at least one head")
-    ost = _strides(q_out)
-    kst = kst or (0,) * nd
-    kost = kst if k is None else _strides(k_out)
-    sb = 0 if nd == 3 else qst[0], 0 if nd == 3 else kst[0], 0 if nd == 3 else ost[0], 0 if nd == 3 else kost[0]
-    _on_device(dev, "fmka_qk_norm_rope_bf16", q.data_ptr(), sb[0], qst[-3], qst[-2], _ptr(k), sb[1], kst[-3], kst[-2],
+    ost = q_out.stride()
+    kost = kst if k is None else k_out.stride()
+    if nd == 3:
+        qst, kst, ost, kost = (0, *qst), (0, *kst), (0, *ost), (0, *kost)
+    _on_device(dev, "fmka_qk_norm_rope_bf16", q.data_ptr(), qst[0], qst[1], qst[2], _ptr(k), kst[0], kst[1], kst[2],
                _ptr(q_weight), _ptr(k_weight), w_f32, eps, _ptr(cos), _ptr(sin), rsb, rst, _ptr(positions), pos_i64,
-               n_pos, q_out.data_ptr(), sb[2], ost[-3], ost[-2], _ptr(k_out), sb[3], kost[-3], kost[-2], B, T, Hq, Hkv,
+               n_pos, q_out.data_ptr(), ost[0], ost[1], ost[2], _ptr(k_out), kost[0], kost[1], kost[2], B, T, Hq, Hkv,
                HEAD_DIM)
     return q_out, k_out
 
 
-def _check_heads(what: str, Hq: int, Hkv: int, *ts: torch.Tensor) -> None:
-    for t in ts:
-        if t.shape[-1] != HEAD_DIM or t.stride(-1) != 1:
-            raise RuntimeError(f"{what}: head_dim must be 128 with contiguous channels")
+def _heads_and_strides(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, Hq: int, Hkv: int):
+    """Strides of q and of k/v (which must agree) after the checks that every packed attention makes."""
+    qst, kst = q.stride(), k.stride()
+    if k.shape != v.shape or (kst != v.stride() and _strides(k) != _strides(v)):
+        raise RuntimeError(f"{what}: k and v must have the same shape and strides")
+    if (q.shape[-1] != HEAD_DIM or k.shape[-1] != HEAD_DIM or qst[-1] != 1 or kst[-1] != 1 or v.stride(-1) != 1):
+        raise RuntimeError(f"{what}: head_dim must be 128 with contiguous channels")
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise RuntimeError(f"{what}: query heads must be a multiple of kv heads")
-
-
-def _kv_strides(what: str, k: torch.Tensor, v: torch.Tensor) -> Tuple[int, ...]:
-    ks = _strides(k)
-    if k.shape != v.shape or ks != _strides(v):
-        raise RuntimeError(f"{what}: k and v must have the same shape and strides")
-    return ks
+    return qst, kst
 
 
 def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
@@ -670,10 +667,9 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     _same_device("attn_varlen", dev, k, v, cu_q, cu_k)
     if q.dim() != 3 or k.dim() != 3:
         raise RuntimeError("attn_varlen: expected q [Tq, Hq, 128] and k/v [Tk, Hkv, 128]")
-    ks, qs = _kv_strides("attn_varlen", k, v), _strides(q)
     Tq, Hq, Dh = q.shape
     Tk, Hkv, _ = k.shape
-    _check_heads("attn_varlen", Hq, Hkv, q, k, v)
+    qs, ks = _heads_and_strides("attn_varlen", q, k, v, Hq, Hkv)
     for cu in (cu_q, cu_k):
         if cu.dtype is not _I32 or cu.dim() != 1 or cu.shape[0] < 1 or not cu.is_contiguous():
             raise RuntimeError("attn_varlen: cu_q and cu_k must be contiguous int32 [S + 1] tensors")
@@ -689,7 +685,7 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
         os_ = (Hq * Dh, Dh)
     else:
         _check_out("attn_varlen: out", out, q.shape, dev)
-        os_ = _strides(out)
+        os_ = out.stride()
     lse = q.new_empty((Hq, Tq), dtype=_F32) if want_lse else None
     if Tq == 0 or S == 0:
         return out, lse
@@ -733,23 +729,22 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
         k_prefix, v_prefix = k_prefix[0], v_prefix[0]
     if k_prefix.dim() != 3 or k.dim() != 4:
         raise RuntimeError("attn_decode_shared: expected a prefix [Hkv, P, 128] and k/v [B, Hkv, Tcap, 128]")
-    ps, ks = _kv_strides("attn_decode_shared", k_prefix, v_prefix), _kv_strides("attn_decode_shared", k, v)
-    qs = _strides(q)
     B, Hq, Dh = q.shape
     Hkv, P, _ = k_prefix.shape
     kB, kH, Tcap, _ = k.shape
     if kB != B or kH != Hkv:
         raise RuntimeError("attn_decode_shared: k/v must hold q's batch and the prefix's kv heads")
-    _check_heads("attn_decode_shared", Hq, Hkv, q, k_prefix, v_prefix, k, v)
+    qs, ps = _heads_and_strides("attn_decode_shared", q, k_prefix, v_prefix, Hq, Hkv)
+    _, ks = _heads_and_strides("attn_decode_shared", q, k, v, Hq, Hkv)
     if lens is not None and (lens.dtype is not _I32 or lens.dim() != 1 or lens.shape[0] != B
                              or not lens.is_contiguous()):
         raise RuntimeError("attn_decode_shared: lens must be a contiguous int32 [B] tensor")
     if out is None:
         out = q.new_empty((B, 1, Hq, Dh))
-        os_ = (Hq * Dh, 0, Dh)
+        os_ = (Hq * Dh, Hq * Dh, Dh)
     else:
         _check_out("attn_decode_shared: out", out, (B, 1, Hq, Dh), dev)
-        os_ = _strides(out)
+        os_ = out.stride()
     lse = q.new_empty((B, Hq), dtype=_F32) if want_lse else None
     if B == 0:
         return out, lse
