@@ -67,14 +67,9 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr uint32_t kTmemO = 0, kTmemS = 128, kTmemP = 384;  // S: 2 x 128 columns, P: 2 x 64
 // Register split between the control warps and the softmax warps (setmaxnreg);
 // the sum has to fit in what the block is launched with.
-#ifndef FMKA_RC
-#define FMKA_RC 56
-#define FMKA_RO 88
-#define FMKA_RS 184
-#endif
-constexpr int kRegsControl = FMKA_RC;
-constexpr int kRegsOutput = FMKA_RO;
-constexpr int kRegsSoftmax = FMKA_RS;
+constexpr int kRegsControl = 56;
+constexpr int kRegsOutput = 88;
+constexpr int kRegsSoftmax = 184;
 constexpr int kMinLaunchRegs = (128 * (kRegsControl + kRegsOutput) + 256 * kRegsSoftmax + kThreads - 1) / kThreads;
 
 // One item as the roles read it, in shared memory. Keys are counted from the item's first.
@@ -800,8 +795,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // of one element says nothing.
 int rows_map(CUtensorMap* out, const __nv_bfloat16* base, int64_t rows, int64_t st, int heads, int64_t sh, int box_h,
              int box_r, bool head_inner) {
-  if (rows == 1 || st == 0) st = 128;
-  if (heads == 1 || sh == 0) sh = 128;
+  // the callers send expanded views (a stride of zero over several) elsewhere
+  if (rows == 1) st = 128;
+  if (heads == 1) sh = 128;
   if (head_inner) {
     const uint64_t dims[3] = {128, (uint64_t)heads, (uint64_t)rows};
     const uint64_t strides[2] = {(uint64_t)sh * 2, (uint64_t)st * 2};

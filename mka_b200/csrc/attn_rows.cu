@@ -1,6 +1,6 @@
 // Attention for few or short rows, on mma.sync: packed sequences of different
-// lengths, and single tokens against a prefix shared by the batch plus the
-// request's own keys.
+// lengths, and single tokens against a small prefix shared by the batch plus
+// the request's own keys.
 //
 //   o_r = sum_{j <= lim(r)} softmax_j(scale * q_r k_j) v_j,  lse_r = log sum_j exp(scale * q_r k_j)
 //
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
     part = ((int64_t)split * p.B + it.row0) * p.Hq + hkv * p.G + g0;
   }
   // tiles from this one on hold keys that some rows see and others do not
-  const int diag_tile = MODE != kModeShared && it.n_tok > 1 ? max(0, it.lim0 + 1 - it.kb) / kTileKeys : 0x7FFFFFFF;
+  const int diag_tile = MODE != kModeShared && it.n_tok > 1 ? max(0, it.lim0 + 1 - it.kb) / kTileKeys : 0x3FFFFFF;
   volatile int* bad_v = reinterpret_cast<volatile int*>(smem + kRingBytes);
   if (threadIdx.x == 0) *bad_v = 0;
   const int n_tiles = it.ke > it.kb ? (it.ke - it.kb + kTileKeys - 1) / kTileKeys : 0;
@@ -495,13 +495,20 @@ void slice_group(PackedAttnParams& p, int rows) {
   p.Gs = (p.G + p.n_gs - 1) / p.n_gs;
 }
 
-// How a packed batch runs.
+// Whether a tensor map can hold rows and heads with these strides: an expanded view's zero cannot be one.
+bool mappable(int64_t st, int rows, int64_t sh, int heads) {
+  return (rows == 1 || st > 0) && (heads == 1 || sh > 0);
+}
+
+// How a packed batch runs. Measured in us (short / thin / pair; * the one taken):
+//   kShort: one launch, every CTA of 64 rows finds its tile in the offsets itself: small calls, where each further
+//     launch counts. 5 prompts of 1 to 40 tokens, 28 heads over 4: 5.3* / 8.2 / 12.5.
+//   kThin: tiles of 16 rows from a plan, long sequences split: batches of few rows per sequence, where all the time
+//     goes to reading K and V. 64 single tokens against 100 to 16000 keys, 32 heads over 8: 413 / 122* / 146.
+//   kPair: 256 rows per cluster on tcgen05, from a plan: the rest. 24 prompts of 64 to 2048 tokens, 32 heads over 8: 387 / 783 / 124*.
 enum class VarlenPath { kShort, kThin, kPair };
 
 VarlenPath varlen_path(int n_seqs, int total_q, int max_k, int G) {
-#ifdef FMKA_VARLEN_PATH
-  return static_cast<VarlenPath>(FMKA_VARLEN_PATH);
-#endif
   if ((int64_t)total_q * max_k < (1 << 16)) return VarlenPath::kShort;
   return (int64_t)total_q * G <= (int64_t)n_seqs * 16 ? VarlenPath::kThin : VarlenPath::kPair;
 }
@@ -516,17 +523,30 @@ struct SharedPlan {
   int own_splits, own_keys;
   bool pair;                       // the prefix goes to the pair kernel
 };
-
+// The prefix belongs on the pair kernel (128 rows of the batch read a key once, on tcgen05) unless it is small: then
+// this kernel's 16-row tiles, in the same launch as the own keys, spare a launch and the clusters' start. What they
+// read is (tiles) x (keys); measured in us, rows here / pair kernel, 8 kv heads of 4 query heads:
+//   batch 4, prefix 1024 (8 k keys read): 8.4 / 12.7;   batch 16, prefix 1024 (33 k): 11.3 / 13.1;
+//   batch 16, prefix 2048 (66 k): 16.2 / 14.7;          batch 1, prefix 16384 (131 k): 25.8 / 25.3;
+//   batch 33, prefix 5003 (440 k): 60.5 / 25.6;         batch 64, prefix 32768: 488 / 67.
+// Parts of 256 keys: the 33 k case takes 18.5 with 64, 14.6 with 128, 11.3 with 256.
+// Own keys in parts of 512: 256 and 1024 were slower on batches of 33 to 256 with 400 to 1024 own slots.
+// A stride of zero over several heads or tokens (an expanded view) is not for tensor maps; it stays here, and with
+// the parts that the sizes ask for, as the workspace's size is asked for without the strides.
 SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
   SharedPlan s{0, kTileKeys, 0, kTileKeys, false};
   if (P > 0) {
-    s.pair = true;
-    s.prefix_splits = attn_pair_prefix_splits(B, Hq, Hkv, P, &s.prefix_keys);
-#ifdef FMKA_SHARED_ROWS
-    s.pair = false;
-    s.prefix_keys = 256;
-    s.prefix_splits = (P + s.prefix_keys - 1) / s.prefix_keys;
-#endif
+    PackedAttnParams r = {};
+    r.G = Hq / Hkv;
+    slice_group(r, 16);
+    const int tpt = 16 / r.Gs;
+    s.pair = (int64_t)((B + tpt - 1) / tpt) * Hkv * r.n_gs * P >= (1 << 16);
+    if (s.pair) {
+      s.prefix_splits = attn_pair_prefix_splits(B, Hq, Hkv, P, &s.prefix_keys);
+    } else {
+      s.prefix_keys = 256;
+      s.prefix_splits = (P + s.prefix_keys - 1) / s.prefix_keys;
+    }
   }
   if (cap > 0) {
     s.own_keys = 512;
@@ -551,7 +571,10 @@ int launch_attn_varlen(PackedAttnParams p, int max_k, void* workspace, cudaStrea
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_varlen: device status word unavailable");
   const VarlenPath path = varlen_path(p.n_seqs, p.total_q, max_k, p.G);
-  if (path == VarlenPath::kShort || p.total_k == 0) {
+  // expanded views are right on the first path whatever the size, and it needs no workspace
+  if (path == VarlenPath::kShort || p.total_k == 0 ||
+      (path == VarlenPath::kPair &&
+       (!mappable(p.q_st, p.total_q, p.q_sh, p.Hq) || !mappable(p.kv_st, p.total_k, p.kv_sh, p.Hkv)))) {
     slice_group(p, 64);
     const int tpt = 64 / p.Gs;
     const int64_t tiles = (int64_t)p.total_q / tpt + p.n_seqs;  // at least one tile ends in every sequence
@@ -581,7 +604,8 @@ size_t attn_decode_shared_workspace_bytes(int B, int Hq, int Hkv, int P, int cap
 int launch_attn_decode_shared(PackedAttnParams p, void* workspace, cudaStream_t stream) {
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_decode_shared: device status word unavailable");
-  const SharedPlan s = plan_shared(p.B, p.Hq, p.Hkv, p.P, p.cap);
+  SharedPlan s = plan_shared(p.B, p.Hq, p.Hkv, p.P, p.cap);
+  if (!mappable(p.q_st, p.B, p.q_sh, p.Hq) || !mappable(p.kp_st, p.P, p.kp_sh, p.Hkv)) s.pair = false;
   const int parts = s.prefix_splits + s.own_splits;
   p.part_o = static_cast<float*>(workspace);
   p.part_lse = p.part_o + (int64_t)parts * p.B * p.Hq * kHeadDim;

@@ -435,6 +435,132 @@ def test_shared_strided_views_and_out(ops):
     assert none is None and torch.equal(o2, o)
 
 
+# ---------------------------------------------------- long lists, large sizes --
+def _check_varlen_heads(o, lse, q, k, v, q_lens, k_lens, causal=True, scale=128 ** -0.5):
+    """_check_varlen with all heads of a sequence at once."""
+    G = q.shape[1] // k.shape[1]
+    q0 = k0 = 0
+    for i, (lq, lk) in enumerate(zip(q_lens, k_lens)):
+        qq = q[q0:q0 + lq].double().transpose(0, 1)
+        kk = k[k0:k0 + lk].double().transpose(0, 1).repeat_interleave(G, 0)
+        vv = v[k0:k0 + lk].double().transpose(0, 1).repeat_interleave(G, 0)
+        sc = qq @ kk.transpose(1, 2) * scale
+        if causal:
+            see = torch.arange(lk, device=DEV)[None] <= torch.arange(lq, device=DEV)[:, None] + lk - lq
+            sc = sc.masked_fill(~see, -math.inf)
+        rl = torch.logsumexp(sc, -1)
+        p = torch.exp(sc - rl.masked_fill(rl == -math.inf, 0.0)[..., None])
+        _check_attn(o[q0:q0 + lq].transpose(0, 1), lse[:, q0:q0 + lq], p @ vv, p @ vv.abs(), rl, what=(i, lq, lk))
+        q0, k0 = q0 + lq, k0 + lk
+
+
+@pytest.mark.parametrize("n,most,hist,Hq,Hkv", [
+    (1500, 30, 0, 2, 1),      # more sequences than the plan keeps on chip
+    (2100, 1, 90, 4, 2),      # ... of one token
+    (500, 40, 60, 32, 32),    # more items than one launch takes
+    (1200, 3, 200, 4, 1)])
+def test_varlen_long_lists(ops, n, most, hist, Hq, Hkv):
+    g = _gen(n)
+    r = torch.Generator().manual_seed(n)
+    q_lens = torch.randint(0 if most > 1 else 1, most + 1, (n,), generator=r).tolist()
+    k_lens = [x + y for x, y in zip(q_lens, torch.randint(0, hist + 1, (n,), generator=r).tolist())]
+    q = _randn(g, sum(q_lens), Hq, 128)
+    k, v = _randn(g, sum(k_lens), Hkv, 128), _randn(g, sum(k_lens), Hkv, 128)
+    o, lse = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(k_lens))
+    _check_varlen_heads(o, lse, q, k, v, q_lens, k_lens)
+    assert ops.device_status() == 0
+
+
+def test_varlen_bad_offset_behind_a_thousand(ops):
+    g = _gen(16)
+    n = 1400
+    q, k = _randn(g, n, 4, 128), _randn(g, n, 2, 128)
+    cu = torch.arange(n + 1, device=DEV, dtype=torch.int32)
+    for at in (1024, 1025, 1399):
+        bad = cu.clone()
+        bad[at] = n + 1
+        out = torch.full_like(q, 7.0)
+        ops.attn_varlen(q, k, k, cu, bad, out=out)
+        assert ops.device_status() == ops.STATUS_BAD_LAUNCH
+        assert (out == 7).all()
+
+
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("Hq,Hkv", [(4, 1), (2, 2)])
+def test_varlen_few_tokens_do_not_see_later_keys(ops, poison, Hq, Hkv):
+    """Two to four tokens behind long histories: a bad last key reaches the last token only, parts and joins included."""
+    g = _gen(18)
+    q_lens, k_lens = [2, 4, 1, 3, 4], [700, 9000, 64, 3, 4097]
+    q, k, v = _randn(g, 14, Hq, 128), _randn(g, sum(k_lens), Hkv, 128), _randn(g, sum(k_lens), Hkv, 128)
+    cu_q, cu_k = _cu(q_lens), _cu(k_lens)
+    want, want_lse = ops.attn_varlen(q, k, v, cu_q, cu_k)
+    _check_varlen(want, want_lse, q, k, v, q_lens, k_lens, True)
+    ends = (cu_k[1:] - 1).long()
+    k[ends] = v[ends] = poison
+    o, lse = ops.attn_varlen(q, k, v, cu_q, cu_k)
+    last = (cu_q[1:] - 1).long()
+    rest = [i for i in range(14) if i not in last.tolist()]
+    assert torch.equal(o[rest], want[rest]) and torch.equal(lse[:, rest], want_lse[:, rest])
+    assert not torch.isfinite(o[last].float()).all(-1).any()
+
+
+@pytest.mark.parametrize("q_lens,k_lens", [([3, 40], [3, 40]), ([1, 1, 1], [9000, 30, 4000]), ([300, 700], [900, 800])])
+def test_varlen_expanded_views(ops, q_lens, k_lens):
+    """One kv head under all, one query row for all heads or tokens: strides of zero."""
+    g = _gen(19)
+    Tq, Tk = sum(q_lens), sum(k_lens)
+    cu_q, cu_k = _cu(q_lens), _cu(k_lens)
+    q, k, v = _randn(g, Tq, 8, 128), _randn(g, Tk, 4, 128), _randn(g, Tk, 4, 128)
+    one_k, one_v = k[:, :1].expand(Tk, 4, 128), v[:, :1].expand(Tk, 4, 128)
+    for qq, kk, vv in ((q, one_k, one_v), (q[:, :1].expand(Tq, 8, 128), k, v), (q[:1].expand(Tq, 8, 128), k, v),
+                       (q, k[:1].expand(Tk, 4, 128), v[:1].expand(Tk, 4, 128))):
+        o, lse = ops.attn_varlen(qq, kk, vv, cu_q, cu_k)
+        _check_varlen_heads(o, lse, qq, kk, vv, q_lens, k_lens)
+
+
+@pytest.mark.parametrize("B,P", [(3, 150), (40, 5000)])
+def test_shared_expanded_views(ops, B, P):
+    g = _gen(20)
+    Hq, Hkv, cap = 8, 4, 70
+    q, kp, vp = _randn(g, B, Hq, 128), _randn(g, Hkv, P, 128), _randn(g, Hkv, P, 128)
+    k, v = _randn(g, B, Hkv, cap, 128), _randn(g, B, Hkv, cap, 128)
+    lens = [cap] * B
+    for qq, a, b in ((q[:1].expand(B, Hq, 128), kp, vp), (q, kp[:1].expand(Hkv, P, 128), vp[:1].expand(Hkv, P, 128)),
+                     (q[:, :1].expand(B, Hq, 128), kp[:, :1].expand(Hkv, P, 128), vp[:, :1].expand(Hkv, P, 128))):
+        for kk, vv in ((k, v), (k[:1].expand(B, Hkv, cap, 128), v[:1].expand(B, Hkv, cap, 128))):
+            o, lse = ops.attn_decode_shared(qq, a, b, kk, vv)
+            _check_shared(o, lse, qq, a, b, kk, vv, lens)
+
+
+def test_offsets_past_32_bits(ops):
+    """Rows behind the 2^31st element of a cache; every path, and a request's own slots that far out."""
+    g = _gen(21)
+    rows = 2 ** 31 // (8 * 128) + 4096
+    cache = torch.empty(rows, 8, 128, device=DEV, dtype=torch.bfloat16)
+    tail = 4000
+    cache[-tail:] = _randn(g, tail, 8, 128)
+    end = rows - tail
+    for q_lens, k_lens in (([5], [40]), ([1, 1], [2000, 1900]), ([900, 30], [2000, 2000])):
+        q = _randn(g, sum(q_lens), 16, 128)
+        o, lse = ops.attn_varlen(q, cache, cache, _cu(q_lens), _cu(k_lens) + end, max_k=max(k_lens))
+        _check_varlen_heads(o, lse, q, cache[end:], cache[end:], q_lens, k_lens)
+    # two requests, the second one's slots at the end of the cache; the prefix there too
+    own = cache.as_strided((2, 8, 100, 128), ((rows - 100) * 1024, 128, 1024, 1))
+    cache[:100] = _randn(g, 100, 8, 128)
+    for P in (300, 4000):
+        pre = cache[-P:].transpose(0, 1)
+        q = _randn(g, 2, 32, 128)
+        o, lse = ops.attn_decode_shared(q, pre, pre, own, own)
+        _check_shared(o, lse, q, pre, pre, own, own, [100, 100])
+    big = cache[rows // 2:]
+    w = 1 + _randn(g, 128, scale=0.2)
+    cos, sin = _tables(torch.arange(big.shape[0], device=DEV))
+    out = torch.empty(rows, 8, 128, device=DEV, dtype=torch.bfloat16)[rows // 2:]
+    ops.qk_norm_rope(big, None, w, None, 1e-6, rope=(cos, sin), q_out=out)
+    _check_norm(out[-tail:], big[-tail:], w, 1e-6, cos[-tail:], sin[-tail:])
+    assert ops.device_status() == 0
+
+
 # ---------------------------------------------------------------- refusals --
 def test_refusals(ops):
     bf = lambda *s: torch.zeros(*s, device=DEV, dtype=torch.bfloat16)  # noqa: E731
