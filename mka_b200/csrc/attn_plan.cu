@@ -21,7 +21,7 @@ constexpr int kBN = 128;  // keys per unit of work
 constexpr int kPlanThreads = 512;
 constexpr int kBins = 512;
 constexpr int kPlanSeqs = 1024;
-constexpr int kMinPartTiles = 4;  // a part is worth its partial output from 512 keys on
+constexpr int kMinPartTiles = 4;  // a part is worth its partial output from 512 keys on (256 and 128: no faster)
 
 struct PlanParams {
   const int* cu_q;
@@ -216,12 +216,13 @@ PackedPlan packed_plan(int n_seqs, int total_q, int max_k, int Hkv, int G, int G
   w.nh = Hkv * w.n_gs;
   w.tok_tile = tok_tile;
   w.workers = workers;
-  // An item with more than a worker's share of the work is cut into at most twice work / share parts, so all parts of
-  // all heads number at most twice the workers.
+  // An item with more than a worker's share of the work is cut into less than twice work / share parts, so the parts
+  // of all nh slices number at most twice the workers.
   w.split = max_k > kMinPartTiles * kBN;
-  w.max_parts = w.split ? 2 * workers : 0;
+  w.max_parts = w.split ? 2 * workers / w.nh : 0;
+  w.split = w.max_parts > 0;
   w.max_list = total_q / tok_tile + n_seqs + w.max_parts;
-  w.part_rows = (int64_t)w.max_parts * tok_tile * Gs;
+  w.part_rows = (int64_t)w.max_parts * tok_tile * Gs * w.nh;
   size_t at = 16;
   w.at_seq = at;
   at = up16(at + sizeof(int) * (size_t)(n_seqs + 1));
@@ -260,7 +261,10 @@ int launch_plan(const PackedAttnParams& a, PackedPlan& w, void* workspace, cudaS
 
 int launch_join(const PackedAttnParams& a, const PackedPlan& w, cudaStream_t stream) {
   if (!w.split) return kOk;
-  return check_cuda(launch_after(attn_join_kernel, dim3(w.max_parts, 4), 256, 0, true, stream, a, w),
+  // a group has two parts or more; about four blocks per SM over all groups, at most one per eight rows of a group
+  const int groups = std::max(1, w.max_parts / 2);
+  const int slices = std::min((w.tok_tile * w.Gs * w.nh + 7) / 8, (4 * num_sms_current_device() + groups - 1) / groups);
+  return check_cuda(launch_after(attn_join_kernel, dim3(groups, slices), 256, 0, true, stream, a, w),
                     "attn_varlen join launch");
 }
 

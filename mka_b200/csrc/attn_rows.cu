@@ -500,16 +500,27 @@ bool mappable(int64_t st, int rows, int64_t sh, int heads) {
   return (rows == 1 || st > 0) && (heads == 1 || sh > 0);
 }
 
-// How a packed batch runs. Measured in us (short / thin / pair; * the one taken):
-//   kShort: one launch, every CTA of 64 rows finds its tile in the offsets itself: small calls, where each further
-//     launch counts. 5 prompts of 1 to 40 tokens, 28 heads over 4: 5.3* / 8.2 / 12.5.
-//   kThin: tiles of 16 rows from a plan, long sequences split: batches of few rows per sequence, where all the time
-//     goes to reading K and V. 64 single tokens against 100 to 16000 keys, 32 heads over 8: 413 / 122* / 146.
-//   kPair: 256 rows per cluster on tcgen05, from a plan: the rest. 24 prompts of 64 to 2048 tokens, 32 heads over 8: 387 / 783 / 124*.
+// How a packed batch runs:
+//   kShort: one launch, every CTA of 64 rows finds its tile in the offsets itself. A CTA takes about 19 ns a key, so it
+//     is for keys (times the waves of CTAs) that are done before a plan would be.
+//   kThin: tiles of 16 rows from a plan, long sequences split: batches of few rows per sequence, where the time goes to
+//     reading K and V.
+//   kPair: 256 rows per cluster on tcgen05, from a plan: the rest.
+// Measured in us (short / thin / pair), 32 heads over 8, on both sides of each limit:
+//   waves x keys: 40 prompts' keys 5.3 / 8.2 / 12.5;  200: 8.6 / 15.8 / 16.9;  250: 9.3 / 17.7 / 17.1;
+//     400: 18.6 / 26.7 / 15.8;  500 (32 single tokens): 19.8 / 14.4 / 27.9;
+//   rows per sequence (64 sequences of 100 to 16000 keys): 4: 657 / 379 / 451;  16: 670 / 392 / 470;
+//     32: 678 / 511 / 466;  32 as one kv head: 299 / 84 / 81;  prompts of 64 to 2048 tokens: 387 / 783 / 124.
 enum class VarlenPath { kShort, kThin, kPair };
+constexpr int kShortKeys = 320;
 
-VarlenPath varlen_path(int n_seqs, int total_q, int max_k, int G) {
-  if ((int64_t)total_q * max_k < (1 << 16)) return VarlenPath::kShort;
+VarlenPath varlen_path(int n_seqs, int total_q, int max_k, int Hkv, int G) {
+  PackedAttnParams p = {};
+  p.G = G;
+  slice_group(p, 64);
+  const int64_t ctas = ((int64_t)total_q / (64 / p.Gs) + n_seqs) * Hkv * p.n_gs;
+  const int64_t slots = 2 * num_sms_current_device();
+  if ((ctas + slots - 1) / slots * max_k < kShortKeys) return VarlenPath::kShort;
   return (int64_t)total_q * G <= (int64_t)n_seqs * 16 ? VarlenPath::kThin : VarlenPath::kPair;
 }
 
@@ -560,7 +571,7 @@ SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
 size_t attn_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, int Hkv) {
   PackedAttnParams p = {};
   p.G = Hq / Hkv;
-  switch (varlen_path(n_seqs, total_q, max_k, p.G)) {
+  switch (varlen_path(n_seqs, total_q, max_k, Hkv, p.G)) {
     case VarlenPath::kShort: return 0;
     case VarlenPath::kThin: return thin_plan(n_seqs, total_q, max_k, Hkv, p).total;
     default: return attn_pair_plan(n_seqs, total_q, max_k, Hq, Hkv).total;
@@ -570,7 +581,7 @@ size_t attn_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, i
 int launch_attn_varlen(PackedAttnParams p, int max_k, void* workspace, cudaStream_t stream) {
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_varlen: device status word unavailable");
-  const VarlenPath path = varlen_path(p.n_seqs, p.total_q, max_k, p.G);
+  const VarlenPath path = varlen_path(p.n_seqs, p.total_q, max_k, p.Hkv, p.G);
   // expanded views are right on the first path whatever the size, and it needs no workspace
   if (path == VarlenPath::kShort || p.total_k == 0 ||
       (path == VarlenPath::kPair &&
