@@ -888,23 +888,32 @@ int launch_attn_pair_varlen(const PackedAttnParams& a, const PackedPlan& w, cuda
                      (int64_t)w.max_list * p.nh, true, stream, "attn_varlen launch");
 }
 
-// Parts of the shared prefix: cut along the keys so that all pairs have work, in about equal rounds.
-int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int* keys_per_split) {
+// Parts of the shared prefix. The own keys' kernel cannot share an SM with this one (registers and shared memory are
+// taken whole), so a cut that fills every pair leaves it waiting: the cut is the one with the least time for both, own
+// keys filling the SMs beside a single round of pairs. Against cuts that fill all pairs, in us with own keys and join:
+// 33 requests, 5003 + 400 keys, 25.6 -> 23.1; 64, 32768 + 1024, 67 -> 60; 256, 4096 + 512, 76.6 -> 71.9.
+int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int cap, int* keys_per_split) {
   PairParams p = {};
   p.Hq = Hq;
   p.G = Hq / Hkv;
   pair_tile(p);
-  const int pairs = num_sms_current_device() / 2;
+  const int sms = num_sms_current_device(), pairs = sms / 2;
   const int64_t units = (int64_t)((B + 2 * p.tpt - 1) / (2 * p.tpt)) * p.nh;
   const int tiles = (P + kBN - 1) / kBN;
+  // SM x us that the own keys take at the memory's rate (half of the slots in use, 512 bytes a key, 6.5 KB a ns)
+  const double own = (double)B * Hkv * cap * 0.5 * 512 / 6.5e6 * sms;
   int best = 1;
-  int64_t best_cost = INT64_MAX;
-  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+  double best_us = 1e30;
+  const int most = (int)std::min<int64_t>({64, tiles, 2 * pairs / units + 1});  // two rounds or less
+  for (int s = 1; s <= most; ++s) {
     const int per = (tiles + s - 1) / s;
-    const int64_t rounds = (units * ((tiles + per - 1) / per) + pairs - 1) / pairs;
-    const int64_t cost = rounds * (per + 2) + s / 8;  // two tiles' time per item for its start and end
-    if (cost < best_cost) {
-      best_cost = cost;
+    const int64_t items = units * ((tiles + per - 1) / per);
+    const int64_t rounds = (items + pairs - 1) / pairs;
+    const double prefix = 0.75 * (double)rounds * (per + 4);  // four tiles' time per item for its start and end
+    const double beside = rounds == 1 ? (double)(sms - 2 * items) * prefix : 0.0;
+    const double us = prefix + std::max(0.0, own - beside) / sms + 0.1 * s;
+    if (us < best_us) {
+      best_us = us;
       best = s;
     }
   }

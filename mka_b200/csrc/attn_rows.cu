@@ -553,7 +553,7 @@ SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
     const int tpt = 16 / r.Gs;
     s.pair = (int64_t)((B + tpt - 1) / tpt) * Hkv * r.n_gs * P >= (1 << 16);
     if (s.pair) {
-      s.prefix_splits = attn_pair_prefix_splits(B, Hq, Hkv, P, &s.prefix_keys);
+      s.prefix_splits = attn_pair_prefix_splits(B, Hq, Hkv, P, cap, &s.prefix_keys);
     } else {
       s.prefix_keys = 256;
       s.prefix_splits = (P + s.prefix_keys - 1) / s.prefix_keys;

@@ -190,7 +190,8 @@ int launch_join(const PackedAttnParams& a, const PackedPlan& w, cudaStream_t str
 // attn_pair.cu: the tcgen05 form for many rows.
 PackedPlan attn_pair_plan(int n_seqs, int total_q, int max_k, int Hq, int Hkv);
 int launch_attn_pair_varlen(const PackedAttnParams& a, const PackedPlan& w, cudaStream_t stream);
-int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int* keys_per_split);
+// Parts of a shared prefix: `cap` own slots per request follow, whose kernel runs beside this one on the SMs left free.
+int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int cap, int* keys_per_split);
 int launch_attn_pair_prefix(const PackedAttnParams& a, cudaStream_t stream);
 
 // Launch that may start while the kernel before it in the stream still runs (that kernel lets it, and it waits itself
