@@ -630,10 +630,10 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
 
 def _heads_and_strides(what: str, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, Hq: int, Hkv: int):
     """Strides of q and of k/v (which must agree) after the checks that every packed attention makes."""
-    qst, kst = q.stride(), k.stride()
-    if k.shape != v.shape or (kst != v.stride() and _strides(k) != _strides(v)):
+    qst, kst, vst, ks = q.stride(), k.stride(), v.stride(), k.shape
+    if ks != v.shape or (kst != vst and _strides(k) != _strides(v)):
         raise RuntimeError(f"{what}: k and v must have the same shape and strides")
-    if (q.shape[-1] != HEAD_DIM or k.shape[-1] != HEAD_DIM or qst[-1] != 1 or kst[-1] != 1 or v.stride(-1) != 1):
+    if q.shape[-1] != HEAD_DIM or ks[-1] != HEAD_DIM or qst[-1] != 1 or kst[-1] != 1 or vst[-1] != 1:
         raise RuntimeError(f"{what}: head_dim must be 128 with contiguous channels")
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise RuntimeError(f"{what}: query heads must be a multiple of kv heads")
@@ -721,17 +721,14 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
             and v.dtype is _BF16):
         _check_bf16(q, k_prefix, v_prefix, k, v)
     _same_device("attn_decode_shared", dev, k_prefix, v_prefix, k, v, lens)
-    if q.dim() == 4 and q.shape[2] == 1:
-        q = q[:, :, 0]
-    if q.dim() != 3:
+    qsh, psh, ksh = q.shape, k_prefix.shape, k.shape
+    if not (len(qsh) == 3 or (len(qsh) == 4 and qsh[2] == 1)):
         raise RuntimeError("attn_decode_shared: one query token per request, q [B, Hq, 1, 128] or [B, Hq, 128]")
-    if k_prefix.dim() == 4 and k_prefix.shape[0] == 1 and v_prefix.dim() == 4 and v_prefix.shape[0] == 1:
-        k_prefix, v_prefix = k_prefix[0], v_prefix[0]
-    if k_prefix.dim() != 3 or k.dim() != 4:
+    if not (len(psh) == 3 or (len(psh) == 4 and psh[0] == 1)) or len(ksh) != 4:
         raise RuntimeError("attn_decode_shared: expected a prefix [Hkv, P, 128] and k/v [B, Hkv, Tcap, 128]")
-    B, Hq, Dh = q.shape
-    Hkv, P, _ = k_prefix.shape
-    kB, kH, Tcap, _ = k.shape
+    B, Hq, Dh = qsh[0], qsh[1], HEAD_DIM
+    Hkv, P = psh[-3], psh[-2]
+    kB, kH, Tcap, _ = ksh
     if kB != B or kH != Hkv:
         raise RuntimeError("attn_decode_shared: k/v must hold q's batch and the prefix's kv heads")
     qs, ps = _heads_and_strides("attn_decode_shared", q, k_prefix, v_prefix, Hq, Hkv)
@@ -751,7 +748,7 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     ws_bytes = _lib.load().fmka_attn_decode_shared_workspace_size(B, Hq, Hkv, P, Tcap)
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None  # as in attn_varlen
     _on_device(dev, "fmka_attn_decode_shared", q.data_ptr(), qs[0], qs[1], k_prefix.data_ptr(), v_prefix.data_ptr(),
-               ps[0], ps[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], _ptr(lens), out.data_ptr(), os_[0],
+               ps[-3], ps[-2], k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], _ptr(lens), out.data_ptr(), os_[0],
                os_[2], _ptr(lse), Hq, B, Hq, Hkv, P, Tcap, Dh, _DEFAULT_SCALE if scale is None else scale, _ptr(ws),
                ws_bytes)
     return out, lse
