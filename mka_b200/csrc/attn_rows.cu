@@ -1,6 +1,6 @@
 // Attention for few or short rows, on mma.sync: packed sequences of different
 // lengths, and single tokens against a small prefix shared by the batch plus
-// the request's own keys.
+// the request's own keys (those also beside a long prefix).
 //
 //   o_r = sum_{j <= lim(r)} softmax_j(scale * q_r k_j) v_j,  lse_r = log sum_j exp(scale * q_r k_j)
 //
@@ -35,8 +35,10 @@ constexpr int kSmemBytes = kRingBytes + 16;
 enum RowsMode : int {
   kModeVarlen = 0,  // packed sequences, every tile found from the offsets
   kModeList = 1,    // packed sequences, items of a plan (attn_plan.cu)
-  kModeShared = 2   // shared prefix (the first prefix_blocks blocks) and own keys
+  kModeShared = 2,  // shared prefix (the first prefix_blocks blocks) and own keys
+  kModeOnce = 3     // the same without parts: a cluster of kOnceCtas takes all keys of a request and joins them itself
 };
+constexpr int kOnceCtas = 8;
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -172,6 +174,21 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
     it.lim0 = c.y;
     part_ts = p.Gs;
     if (c.z >= 0) part = (int64_t)c.z + (int64_t)blockIdx.y * a.y * p.Gs;
+  } else if constexpr (MODE == kModeOnce) {
+    it.row0 = blockIdx.x / kOnceCtas;
+    it.n_tok = 1;
+    it.kv_off = it.row0 * p.kv_sb + hkv * p.kv_sh;
+    const int len = p.lens != nullptr ? max(0, min(p.cap, __ldg(p.lens + it.row0))) : p.cap;
+    const int tiles = (p.P + len + kTileKeys - 1) / kTileKeys;
+    const int per = (tiles + kOnceCtas - 1) / kOnceCtas * kTileKeys;
+    it.kb = (blockIdx.x % kOnceCtas) * per;
+    it.ke = min(p.P + len, it.kb + per);
+    it.lim0 = 0x3FFFFFFF;
+    if (p.cap == 0) {  // rows that are filled with zeros still name an address: one that exists
+      kp = p.kp;
+      vp = p.vp;
+      it.kv_off = 0;
+    }
   } else {
     int split;
     if ((int)blockIdx.x < p.prefix_blocks) {
@@ -200,7 +217,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
     part = ((int64_t)split * p.B + it.row0) * p.Hq + hkv * p.G + g0;
   }
   // tiles from this one on hold keys that some rows see and others do not
-  const int diag_tile = MODE != kModeShared && it.n_tok > 1 ? max(0, it.lim0 + 1 - it.kb) / kTileKeys : 0x3FFFFFF;
+  constexpr bool kCausal = MODE == kModeVarlen || MODE == kModeList;
+  const int diag_tile = kCausal && it.n_tok > 1 ? max(0, it.lim0 + 1 - it.kb) / kTileKeys : 0x3FFFFFF;
   volatile int* bad_v = reinterpret_cast<volatile int*>(smem + kRingBytes);
   if (threadIdx.x == 0) *bad_v = 0;
   const int n_tiles = it.ke > it.kb ? (it.ke - it.kb + kTileKeys - 1) / kTileKeys : 0;
@@ -208,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
   kp += it.kv_off;
   vp += it.kv_off;
   const uint32_t s_base = smem_u32(smem);
+  const int own0 = MODE == kModeOnce ? p.P : 0;  // key of kp's first row
   auto load_tile = [&](int i) {
     if (i < n_tiles) {
       const uint32_t ks = s_base + (i % kStages) * 2 * kTileBytes;
@@ -217,9 +236,15 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
         const int id = c * kThreads + threadIdx.x;
         const int row = id >> 4, ch = id & 15;
         const bool live = key0 + row < it.ke;
-        const int64_t off = live ? (int64_t)(key0 + row) * kv_st + ch * 8 : 0;
-        cp_async16(ks + tile_off(row, ch), kp + off, live);
-        cp_async16(ks + kTileBytes + tile_off(row, ch), vp + off, live);
+        if (MODE == kModeOnce && key0 + row < p.P) {  // the prefix's rows first
+          const int64_t off = (int64_t)(key0 + row) * p.kp_st + hkv * p.kp_sh + ch * 8;
+          cp_async16(ks + tile_off(row, ch), p.kp + (live ? off : 0), live);
+          cp_async16(ks + kTileBytes + tile_off(row, ch), p.vp + (live ? off : 0), live);
+        } else {
+          const int64_t off = live ? (int64_t)(key0 + row - own0) * kv_st + ch * 8 : 0;
+          cp_async16(ks + tile_off(row, ch), kp + off, live);
+          cp_async16(ks + kTileBytes + tile_off(row, ch), vp + off, live);
+        }
       }
     }
     cp_async_commit();
@@ -260,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
 
   for (int i = 0; i < n_tiles; ++i) {
     cp_async_wait<kStages - 2>();
-    if (MODE != kModeShared && i >= diag_tile) {
+    if (kCausal && i >= diag_tile) {
       // this thread's own copies are visible to it before the barrier
 #pragma unroll
       for (int c = 0; c < kTileKeys * 16 / kThreads; ++c) {
@@ -390,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
       wt[w] = fast_exp2(sm[(w * 16 + row) * 2] - Ms);
       L += wt[w] * sm[(w * 16 + row) * 2 + 1];
     }
-    if (!live_row) return;
+    if (MODE != kModeOnce && !live_row) return;
     float acc[16];
 #pragma unroll
     for (int c = 0; c < 16; ++c) acc[c] = 0.f;
@@ -406,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
         acc[q4 * 4 + 3] = fmaf(wt[w], x.w, acc[q4 * 4 + 3]);
       }
     }
-    if (MODE != kModeShared && n_tiles > diag_tile && *bad_v) {
+    if (kCausal && n_tiles > diag_tile && *bad_v) {
       // rare: the infinities and NaNs taken out above go to the rows that see them
       for (int j = it.kb + diag_tile * kTileKeys; j <= lim_row; ++j) {
 #pragma unroll
@@ -415,6 +440,50 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
           if (!(fabsf(x) <= 3.4e38f)) acc[c] += x;
         }
       }
+    }
+    if constexpr (MODE == kModeOnce) {
+      // This CTA's keys are done: sums (not yet divided), maximum and weight of each row to where the others read them;
+      // then every CTA joins 16 channels of all rows.
+      float* xo = so + 4 * 16 * kHeadDim + 128;  // [16][128], behind so and sm
+      float* xm = xo + 16 * kHeadDim;            // [16][2]
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        reinterpret_cast<float4*>(xo + row * kHeadDim + seg * 16)[c] =
+            make_float4(acc[c * 4], acc[c * 4 + 1], acc[c * 4 + 2], acc[c * 4 + 3]);
+      if (seg == 0) {
+        xm[row * 2] = M;
+        xm[row * 2 + 1] = L;
+      }
+      cluster_sync();
+      const uint32_t rank = cluster_ctarank();
+      float2 ml[kOnceCtas], v[kOnceCtas];
+#pragma unroll
+      for (int r = 0; r < kOnceCtas; ++r) {
+        ml[r] = ld_cluster_f2(cluster_addr(xm + row * 2, r));
+        v[r] = ld_cluster_f2(cluster_addr(xo + row * kHeadDim + rank * 16 + seg * 2, r));
+      }
+      float Mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < kOnceCtas; ++r) Mx = fmaxf(Mx, ml[r].x);
+      const float Mxs = Mx == -INFINITY ? 0.f : Mx;
+      float Lx = 0.f;
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int r = 0; r < kOnceCtas; ++r) {
+        const float w = fast_exp2(ml[r].x - Mxs);
+        Lx = fmaf(w, ml[r].y, Lx);
+        sum.x = fmaf(w, v[r].x, sum.x);
+        sum.y = fmaf(w, v[r].y, sum.y);
+      }
+      if (live_row) {
+        const float inv = Lx == 0.f ? 0.f : 1.f / Lx;
+        *reinterpret_cast<uint32_t*>(p.o + tok0 * p.o_st + head0 * p.o_sh + rank * 16 + seg * 2) =
+            pack_bf16x2(sum.x * inv, sum.y * inv);
+        if (rank == 0 && seg == 0 && p.lse != nullptr)
+          p.lse[tok0 * p.lse_st + head0 * p.lse_sh] = Lx == 0.f ? -INFINITY : (Mx + __log2f(Lx)) * 0.69314718055994531f;
+      }
+      cluster_sync();  // no CTA leaves while its rows are read
+      return;
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees no key gives zeros
     const float lse2 = L == 0.f ? -INFINITY : M + __log2f(L);
@@ -479,6 +548,26 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
            p.lse == nullptr ? nullptr : p.lse + b * p.lse_st + h * p.lse_sh);
 }
 
+// One launch, clusters of kOnceCtas: request x kv head (x slice of its group).
+int launch_once(const PackedAttnParams& p, cudaStream_t stream) {
+  auto kern = attn_rows_kernel<1, kModeOnce>;
+  int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes),
+                      "attn_decode_shared launch");
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.B * kOnceCtas), (unsigned)(p.Hkv * p.n_gs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kOnceCtas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), "attn_decode_shared launch");
+}
+
 template <int WM, int MODE>
 int launch_rows(const PackedAttnParams& p, int64_t gx, bool dependent, cudaStream_t stream, const char* what) {
   auto kern = attn_rows_kernel<WM, MODE>;
@@ -533,8 +622,15 @@ struct SharedPlan {
   int prefix_splits, prefix_keys;  // parts over the prefix, keys per part
   int own_splits, own_keys;
   bool pair;                       // the prefix goes to the pair kernel
+  bool once;                       // no parts: one launch of clusters
 };
-// The prefix belongs on the pair kernel (128 rows of the batch read a key once, on tcgen05) unless it is small: then
+constexpr int kOnceKeys = 2048;
+
+// Few requests with few keys are one launch of clusters, if these all run at once: no parts in memory, no join, no
+// workspace, which also saves the caller 5 of 22 us. In us on the device, clusters / parts:
+//   batch 1, 8 kv heads, 64 own slots: prefix 1024: 6.4 / 7.5;  2048: 8.4 / 8.0;  4096: 11.9 / 10.2;
+//   batch 4, 4 kv heads of 7, prefix 1000 and 64: 8.1 / 8.4;  batch 30, 1 kv head, prefix 1000 and 100: 8.4 / 8.5.
+// Else the prefix belongs on the pair kernel (128 rows of the batch read a key once, on tcgen05) unless it is small: then
 // this kernel's 16-row tiles, in the same launch as the own keys, spare a launch and the clusters' start. What they
 // read is (tiles) x (keys); measured in us, rows here / pair kernel, 8 kv heads of 4 query heads:
 //   batch 4, prefix 1024 (8 k keys read): 8.4 / 12.7;   batch 16, prefix 1024 (33 k): 11.3 / 13.1;
@@ -545,11 +641,13 @@ struct SharedPlan {
 // A stride of zero over several heads or tokens (an expanded view) is not for tensor maps; it stays here, and with
 // the parts that the sizes ask for, as the workspace's size is asked for without the strides.
 SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
-  SharedPlan s{0, kTileKeys, 0, kTileKeys, false};
+  SharedPlan s{0, kTileKeys, 0, kTileKeys, false, false};
+  PackedAttnParams r = {};
+  r.G = Hq / Hkv;
+  slice_group(r, 16);
+  s.once = (int64_t)B * Hkv * r.n_gs * kOnceCtas <= 2 * num_sms_current_device() && (int64_t)P + cap <= kOnceKeys;
+  if (s.once) return s;
   if (P > 0) {
-    PackedAttnParams r = {};
-    r.G = Hq / Hkv;
-    slice_group(r, 16);
     const int tpt = 16 / r.Gs;
     s.pair = (int64_t)((B + tpt - 1) / tpt) * Hkv * r.n_gs * P >= (1 << 16);
     if (s.pair) {
@@ -617,6 +715,10 @@ int launch_attn_decode_shared(PackedAttnParams p, void* workspace, cudaStream_t 
   if (p.status == nullptr) return set_error(kErrDevice, "attn_decode_shared: device status word unavailable");
   SharedPlan s = plan_shared(p.B, p.Hq, p.Hkv, p.P, p.cap);
   if (!mappable(p.q_st, p.B, p.q_sh, p.Hq) || !mappable(p.kp_st, p.P, p.kp_sh, p.Hkv)) s.pair = false;
+  if (s.once) {
+    slice_group(p, 16);
+    return launch_once(p, stream);
+  }
   const int parts = s.prefix_splits + s.own_splits;
   p.part_o = static_cast<float*>(workspace);
   p.part_lse = p.part_o + (int64_t)parts * p.B * p.Hq * kHeadDim;

@@ -64,8 +64,8 @@ SHARED = dict(q=PTR, q_sb=512, q_sh=128, kp=PTR, vp=PTR, p_sh=1024, p_st=128, k=
     ("fmka_attn_decode_shared", SHARED, dict(Hq=3), 1, "multiple of kv heads"),
     ("fmka_attn_decode_shared", SHARED, dict(p_st=130), 1, "prefix"),
     ("fmka_attn_decode_shared", SHARED, dict(vp=PTR + 8), 1, "prefix"),
-    ("fmka_attn_decode_shared", SHARED, dict(), 4, "workspace"),
-    ("fmka_attn_decode_shared", SHARED, dict(ws=PTR, ws_bytes=16), 4, "workspace"),
+    ("fmka_attn_decode_shared", SHARED, dict(P=5000), 4, "workspace"),
+    ("fmka_attn_decode_shared", SHARED, dict(P=5000, ws=PTR, ws_bytes=16), 4, "workspace"),
 ])
 def test_c_abi_refuses(lib, entry, base, change, code, word):
     rc = getattr(lib, entry)(*{**base, **change}.values())
@@ -84,6 +84,13 @@ def test_workspace_sizes_of_bad_shapes_are_zero(lib):
     assert lib.fmka_attn_varlen_workspace_size(2, 8, 8, 5, 2) == 0
     assert lib.fmka_attn_decode_shared_workspace_size(0, 4, 2, 8, 8) == 0
     assert lib.fmka_attn_decode_shared_workspace_size(2, 4, 0, 8, 8) == 0
+
+
+def test_small_problems_need_no_workspace(lib):
+    assert lib.fmka_attn_varlen_workspace_size(2, 8, 8, 4, 2) == 0
+    assert lib.fmka_attn_decode_shared_workspace_size(2, 4, 2, 8, 8) == 0
+    assert lib.fmka_attn_varlen_workspace_size(2, 8, 5000, 4, 2) > 0
+    assert lib.fmka_attn_decode_shared_workspace_size(2, 4, 2, 5000, 8) > 0
 
 
 def test_cpu_tensors_raise():

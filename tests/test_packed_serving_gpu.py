@@ -435,6 +435,62 @@ def test_shared_strided_views_and_out(ops):
     assert none is None and torch.equal(o2, o)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,P,cap", [
+    (40, 8, 2, 0, 600), (40, 8, 2, 500, 0), (37, 4, 1, 1000, 1048), (37, 4, 1, 1000, 1049), (38, 4, 1, 1000, 30),
+    (1, 16, 1, 63, 1), (2, 8, 8, 2047, 1), (2, 17, 1, 200, 200), (1, 40, 2, 1, 0), (1, 4, 4, 0, 513), (6, 8, 8, 9, 1300)])
+def test_shared_around_the_limits(ops, B, Hq, Hkv, P, cap):
+    """Sizes on both sides of where the work is cut differently, every length of the own keys from none to all."""
+    g = _gen(B * 11 + P + cap)
+    q, kp, vp = _randn(g, B, Hq, 128, scale=1.5), _randn(g, Hkv, P, 128), _randn(g, Hkv, P, 128)
+    k, v = _randn(g, B, Hkv, cap, 128), _randn(g, B, Hkv, cap, 128)
+    n = [i * cap // max(1, B - 1) for i in range(B)]
+    for b in range(B):
+        k[b, :, n[b]:], v[b, :, n[b]:] = float("nan"), float("inf")
+    o, lse = ops.attn_decode_shared(q, kp, vp, k, v, torch.tensor(n, device=DEV, dtype=torch.int32))
+    _check_shared(o, lse, q, kp, vp, k, v, n)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("P", [333, 6000])
+def test_shared_strided_views_of_a_large_batch(ops, P):
+    g = _gen(34)
+    B, Hq, Hkv, cap = 64, 12, 4, 50
+    q = _randn(g, Hq, B, 128).transpose(0, 1)
+    pre = _randn(g, P, 2 * Hkv, 128)
+    kp, vp = pre[:, :Hkv].transpose(0, 1), pre[:, Hkv:].transpose(0, 1)
+    big = _randn(g, 2, B, 128, Hkv, 128).transpose(2, 3)
+    k, v = big[0][:, :, 10:10 + cap], big[1][:, :, 10:10 + cap]
+    lens = torch.randint(0, cap + 1, (B,), device=DEV, generator=g, dtype=torch.int32)
+    buf = torch.full((B, 2, Hq, 192), 7.0, device=DEV, dtype=torch.bfloat16)
+    _, lse = ops.attn_decode_shared(q, kp, vp, k, v, lens, scale=0.15, out=buf[:, 1:, :, 32:160])
+    _check_shared(buf[:, 1:, :, 32:160], lse, q, kp, vp, k, v, lens.tolist(), 0.15)
+    buf[:, 1:, :, 32:160] = 7.0
+    assert (buf == 7).all()
+
+
+@pytest.mark.parametrize("B,P", [(2, 100), (60, 100), (60, 6000)])
+def test_shared_bad_values_show_in_the_rows_that_see_them(ops, B, P):
+    g = _gen(35)
+    Hq, Hkv, cap = 8, 2, 70
+    q, kp, vp = _randn(g, B, Hq, 128), _randn(g, Hkv, P, 128), _randn(g, Hkv, P, 128)
+    k, v = _randn(g, B, Hkv, cap, 128), _randn(g, B, Hkv, cap, 128)
+    want, want_lse = ops.attn_decode_shared(q, kp, vp, k, v)
+    for poison in (float("nan"), float("inf")):
+        v2, k2 = v.clone(), k.clone()
+        v2[1, 0, 69, 5] = poison          # one channel of one request's kv head
+        k2[0, 1, 3, 7] = float("nan")     # one key: all of its heads' channels
+        o, lse = ops.attn_decode_shared(q, kp, vp, k2, v2)
+        assert not torch.isfinite(o[1, 0, :4, 5].float()).any() and torch.isnan(o[0, 0, 4:].float()).all()
+        o[1, 0, :4, 5], o[0, 0, 4:], lse[0, 4:] = want[1, 0, :4, 5], want[0, 0, 4:], want_lse[0, 4:]
+        assert torch.equal(o, want) and torch.equal(lse, want_lse)
+        vp2 = vp.clone()
+        vp2[1, P // 2, 9] = poison
+        o, _ = ops.attn_decode_shared(q, kp, vp2, k, v)
+        assert not torch.isfinite(o[:, 0, 4:, 9].float()).any()
+        o[:, 0, 4:, 9] = want[:, 0, 4:, 9]
+        assert torch.equal(o, want)
+
+
 # ---------------------------------------------------- long lists, large sizes --
 def _check_varlen_heads(o, lse, q, k, v, q_lens, k_lens, causal=True, scale=128 ** -0.5):
     """_check_varlen with all heads of a sequence at once."""
