@@ -353,9 +353,10 @@ FMKA_API int fmka_attn_varlen(const void* q, int64_t q_st, int64_t q_sh, const v
  * prefix shared by the whole batch (k_prefix / v_prefix [Hkv, P, 128], strides
  * p_sh, p_st) followed by the request's own keys (k / v [B, Hkv, Tcap, 128],
  * the first lens[b] slots; lens in device memory, NULL means Tcap for all,
- * values are clamped to [0, Tcap]). The prefix is read once for the batch. P or
- * Tcap may be 0; a request that sees no key gives zeros and -inf. o[b, hq, :] at
- * (o_sb, o_sh); lse[b * lse_sb + hq] may be NULL. */
+ * values are clamped to [0, Tcap]). A long prefix is read once for the batch. P
+ * or Tcap may be 0; a request that sees no key gives zeros and -inf. o[b, hq, :]
+ * at (o_sb, o_sh); lse[b * lse_sb + hq] may be NULL, and so may a workspace of
+ * size 0 (here and above). */
 FMKA_API size_t fmka_attn_decode_shared_workspace_size(int B, int Hq, int Hkv, int P, int Tcap);
 FMKA_API int fmka_attn_decode_shared(const void* q, int64_t q_sb, int64_t q_sh, const void* k_prefix,
                                      const void* v_prefix, int64_t p_sh, int64_t p_st, const void* k, const void* v,

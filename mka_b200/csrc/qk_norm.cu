@@ -30,8 +30,10 @@ namespace {
 constexpr int kHeadDim = 128;
 constexpr int kWarps = 4;
 constexpr int kRowsPerWarp = 4;
-constexpr int kGroupsAhead = 2;   // four-row groups loaded before the first is used
-constexpr int kWarpsPerSm = 32;   // warps wanted before a token's heads share one warp
+constexpr int kGroupsAhead = 2;   // four-row groups loaded before the first is used (32768 tokens: 119 us, with one 142)
+// A token's heads share one warp once that still leaves this many warps per SM (20 are resident). 32 + 8 heads, in us with
+// 1 / 13 / 32 of them: 256 tokens 5.9 / 3.5 / 3.5;  512: 7.3 / 4.7 / 5.6;  1024: 8.3 / 7.0 / 7.0;  2048: 9.8 / 9.9 / 12.0.
+constexpr int kWarpsPerSm = 13;
 
 __device__ __forceinline__ void load_f32x8(const float* p, float2* f) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(p));
@@ -184,7 +186,8 @@ int launch_qk_norm_rope(QkNormParams p, cudaStream_t stream) {
   const int groups = (p.Hq + p.Hk + kRowsPerWarp - 1) / kRowsPerWarp;
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "qk_norm_rope: device status word unavailable");
-  // All heads of a token in one warp, so that its angles are read once, unless that leaves the GPU short of warps.
+  // All heads of a token in one warp, so that its angles are read once, unless that leaves the GPU short of warps; a
+  // warp with one group of four rows has none to load ahead.
   const int64_t want = (int64_t)num_sms_current_device() * kWarpsPerSm;
   p.iters = groups;
   while (p.iters > 1 && tokens * ((groups + p.iters - 1) / p.iters) < want) p.iters = (p.iters + 1) / 2;

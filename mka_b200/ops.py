@@ -706,8 +706,8 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     """Single-token attention of a batch whose requests share a prefix.
 
     q [B, Hq, 1, 128] or [B, Hq, 128]; k_prefix / v_prefix [Hkv, P, 128] (or
-    [1, Hkv, P, 128]), the keys and values every request sees first, read once
-    for the whole batch; k / v [B, Hkv, Tcap, 128], each request's own cache
+    [1, Hkv, P, 128]), the keys and values every request sees first (a long
+    prefix is read once for the whole batch); k / v [B, Hkv, Tcap, 128], each request's own cache
     behind the prefix, of which the first lens[b] slots are valid (int32 [B] on
     the GPU, clamped to [0, Tcap]; None: all of them). Strided views are fine.
     The result is attn_decode's over the concatenated keys. Either part may be
