@@ -906,22 +906,32 @@ int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int cap, int* keys_pe
   const int tiles = (P + kBN - 1) / kBN;
   // SM x us that the own keys take at the memory's rate (half of the slots in use, 512 bytes a key, 6.5 KB a ns)
   const double own = (double)B * Hkv * cap * 0.5 * 512 / 6.5e6 * sms;
-  int best = 1;
-  double best_us = 1e30;
   const int most = (int)std::min<int64_t>({64, tiles, 2 * pairs / units + 1});  // two rounds or less
-  for (int s = 1; s <= most; ++s) {
-    const int per = (tiles + s - 1) / s;
+  int per = tiles;
+  double prefix = 0, beside = 0;
+  auto cut = [&](int parts) {
+    per = (tiles + parts - 1) / parts;
     const int64_t items = units * ((tiles + per - 1) / per);
     const int64_t rounds = (items + pairs - 1) / pairs;
-    const double prefix = 0.75 * (double)rounds * (per + 4);  // four tiles' time per item for its start and end
-    const double beside = rounds == 1 ? (double)(sms - 2 * items) * prefix : 0.0;
-    const double us = prefix + std::max(0.0, own - beside) / sms + 0.1 * s;
-    if (us < best_us) {
+    prefix = 0.75 * (double)rounds * (per + 4) + 0.1 * parts;  // four tiles' time per item for its start and end
+    beside = rounds == 1 ? (double)(sms - 2 * items) * prefix : 0.0;
+  };
+  double alone = 1e30;  // the least time of the prefix by itself; it may take twice that, as slots may hold few keys
+  for (int s = 1; s <= most; ++s) {
+    cut(s);
+    alone = std::min(alone, prefix);
+  }
+  int best = 1;
+  double best_us = 1e30;
+  for (int s = 1; s <= most; ++s) {
+    cut(s);
+    const double us = prefix + std::max(0.0, own - beside) / sms;
+    if (prefix <= 2 * alone && us < best_us) {
       best_us = us;
       best = s;
     }
   }
-  const int per = (tiles + best - 1) / best;
+  cut(best);
   *keys_per_split = per * kBN;
   return (tiles + per - 1) / per;
 }

@@ -17,6 +17,8 @@
 // rounded to bf16 for the second product because the tensor cores take bf16:
 // half a step of 2^-9 on each weight, the same size as the rounding of the
 // output.
+#include <algorithm>
+
 #include "fmka_internal.h"
 #include "ptx.cuh"
 
@@ -637,7 +639,10 @@ constexpr int kOnceKeys = 2048;
 //   batch 16, prefix 2048 (66 k): 16.2 / 14.7;          batch 1, prefix 16384 (131 k): 25.8 / 25.3;
 //   batch 33, prefix 5003 (440 k): 60.5 / 25.6;         batch 64, prefix 32768: 488 / 67.
 // Parts of 256 keys: the 33 k case takes 18.5 with 64, 14.6 with 128, 11.3 with 256.
-// Own keys in parts of 512: 256 and 1024 were slower on batches of 33 to 256 with 400 to 1024 own slots.
+// Own keys in parts of 512 (256 and 1024 were slower on batches of 33 to 256 with 400 to 1024 own slots), but a cache
+// with much room in parts as large as 8 waves of CTAs, or 8 parts, make them: parts that turn out empty are not free.
+// 16 requests, 8 kv heads, room for 131072 keys, 8 / 32 / 256 parts, in us: 100 keys each 22 / 41 / 213; all full 816 /
+// 815 / 1050; one full 224 / 128 / 323. 64 requests, room for 32768, 8 / 32 / 64 parts: 39 / 115 / 209; 800 / 878 / 991.
 // A stride of zero over several heads or tokens (an expanded view) is not for tensor maps; it stays here, and with
 // the parts that the sizes ask for, as the workspace's size is asked for without the strides.
 SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
@@ -658,7 +663,9 @@ SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
     }
   }
   if (cap > 0) {
-    s.own_keys = 512;
+    const int64_t units = (int64_t)B * Hkv * r.n_gs;
+    const int most = (int)std::max<int64_t>(8, 16 * num_sms_current_device() / units);
+    s.own_keys = std::max(512, (cap + most * kTileKeys - 1) / (most * kTileKeys) * kTileKeys);
     s.own_splits = (cap + s.own_keys - 1) / s.own_keys;
   }
   return s;

@@ -451,6 +451,21 @@ def test_shared_around_the_limits(ops, B, Hq, Hkv, P, cap):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("B,P,cap", [(3, 70, 40000), (40, 300, 9000), (24, 9000, 5000)])
+def test_shared_caches_with_much_room(ops, B, P, cap):
+    g = _gen(36)
+    Hq, Hkv = 8, 2
+    q, kp, vp = _randn(g, B, Hq, 128), _randn(g, Hkv, P, 128), _randn(g, Hkv, P, 128)
+    k, v = _randn(g, B, Hkv, cap, 128), _randn(g, B, Hkv, cap, 128)
+    n = torch.randint(0, cap + 1, (B,), device=DEV, generator=g, dtype=torch.int32)
+    n[0], n[1], n[2] = cap, 0, 1
+    for b, x in enumerate(n.tolist()):
+        k[b, :, x:], v[b, :, x:] = float("nan"), float("inf")
+    o, lse = ops.attn_decode_shared(q, kp, vp, k, v, n)
+    _check_shared(o, lse, q, kp, vp, k, v, n.tolist())
+    assert ops.device_status() == 0
+
+
 @pytest.mark.parametrize("P", [333, 6000])
 def test_shared_strided_views_of_a_large_batch(ops, P):
     g = _gen(34)
