@@ -602,6 +602,8 @@ bool mappable(int64_t st, int rows, int64_t sh, int heads) {
 //     400: 18.6 / 26.7 / 15.8;  500 (32 single tokens): 19.8 / 14.4 / 27.9;
 //   rows per sequence (64 sequences of 100 to 16000 keys): 4: 657 / 379 / 451;  16: 670 / 392 / 470;
 //     32: 678 / 511 / 466;  32 as one kv head: 299 / 84 / 81;  prompts of 64 to 2048 tokens: 387 / 783 / 124.
+//   a prompt among single tokens (thin / pair): 512 tokens among 60: 338 / 271;  1024 among 400: 754 / 927;  2048 among
+//     800: 1142 / 1042.
 enum class VarlenPath { kShort, kThin, kPair };
 constexpr int kShortKeys = 320;
 

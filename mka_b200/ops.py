@@ -496,11 +496,13 @@ _DEFAULT_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 _BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _same_device(what: str, dev: torch.device, *ts: Optional[torch.Tensor]) -> None:
+    index = dev.index
     for t in ts:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != index:
             if not t.is_cuda:
                 raise RuntimeError("FastMKA B200 ops need CUDA tensors (there is no CPU fallback)")
             raise RuntimeError(f"{what}: all tensors must be on {dev}")
@@ -509,11 +511,12 @@ def _same_device(what: str, dev: torch.device, *ts: Optional[torch.Tensor]) -> N
 def _on_device(dev: torch.device, name: str, *args) -> None:
     """Calls entry point `name` with args and the current stream of `dev` behind them."""
     fn = getattr(_lib._lib or _lib.load(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(dev.index))
+    index = dev.index
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev.index))
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
 
@@ -590,10 +593,11 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
     if positions is not None:
         if rope is None:
             raise RuntimeError("qk_norm_rope: positions need the cos/sin tables")
-        if positions.shape != qs[:-2] or (positions.dtype is not _I32 and positions.dtype is not _I64):
-            raise RuntimeError("qk_norm_rope: positions must be int32 or int64 of q's token shape")
-        positions = positions.contiguous()
         pos_i64 = int(positions.dtype is _I64)
+        if positions.shape != qs[:-2] or (not pos_i64 and positions.dtype is not _I32):
+            raise RuntimeError("qk_norm_rope: positions must be int32 or int64 of q's token shape")
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
         cos, sin = rope
         n_pos = cos.shape[0]
         if cos.dim() != 2 or cos.shape != sin.shape or n_pos == 0:
@@ -681,7 +685,7 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     elif max_k < 0:
         raise RuntimeError("attn_varlen: max_k must not be negative")
     if out is None:
-        out = q.new_empty((Tq, Hq, Dh))
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((Tq, Hq, Dh))
         os_ = (Hq * Dh, Dh)
     else:
         _check_out("attn_varlen: out", out, q.shape, dev)
