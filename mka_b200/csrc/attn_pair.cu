@@ -844,7 +844,8 @@ int launch_pair(const PairParams& given, const __nv_bfloat16* q, int64_t q_rows,
   }
   if (launch_regs < kMinLaunchRegs)
     return set_error(kErrUnsupported, std::string(what) + ": compiled register count too small for the warpgroup split");
-  rc = check_cuda(cudaFuncSetAttribute(attn_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes), what);
+  static std::atomic<uint64_t> devices{0};
+  rc = check_cuda(allow_smem(attn_pair_kernel, kSmemBytes, devices), what);
   if (rc) return rc;
   // kMaxItems of each pair per launch; the bound on the items is loose, a launch without any ends at once
   const int64_t rounds = (max_items + pairs - 1) / pairs;

@@ -553,8 +553,8 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
 // One launch, clusters of kOnceCtas: request x kv head (x slice of its group).
 int launch_once(const PackedAttnParams& p, cudaStream_t stream) {
   auto kern = attn_rows_kernel<1, kModeOnce>;
-  int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes),
-                      "attn_decode_shared launch");
+  static std::atomic<uint64_t> devices{0};
+  int rc = check_cuda(allow_smem(kern, kSmemBytes, devices), "attn_decode_shared launch");
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.B * kOnceCtas), (unsigned)(p.Hkv * p.n_gs));
@@ -573,7 +573,8 @@ int launch_once(const PackedAttnParams& p, cudaStream_t stream) {
 template <int WM, int MODE>
 int launch_rows(const PackedAttnParams& p, int64_t gx, bool dependent, cudaStream_t stream, const char* what) {
   auto kern = attn_rows_kernel<WM, MODE>;
-  int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes), what);
+  static std::atomic<uint64_t> devices{0};
+  int rc = check_cuda(allow_smem(kern, kSmemBytes, devices), what);
   if (rc) return rc;
   if (gx > 0x7FFFFFFF) return set_error(kErrUnsupported, std::string(what) + ": problem too large");
   return check_cuda(launch_after(kern, dim3((unsigned)gx, (unsigned)(p.Hkv * p.n_gs)), kThreads, kSmemBytes, dependent,

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 #include <utility>
 
@@ -193,6 +194,19 @@ int launch_attn_pair_varlen(const PackedAttnParams& a, const PackedPlan& w, cuda
 // Parts of a shared prefix: `cap` own slots per request follow, whose kernel runs beside this one on the SMs left free.
 int attn_pair_prefix_splits(int B, int Hq, int Hkv, int P, int cap, int* keys_per_split);
 int launch_attn_pair_prefix(const PackedAttnParams& a, cudaStream_t stream);
+
+// Lets `kern` use `bytes` of dynamic shared memory, asked of the runtime once per device.
+template <class... Params>
+cudaError_t allow_smem(void (*kern)(Params...), int bytes, std::atomic<uint64_t>& devices) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (devices.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) devices.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Launch that may start while the kernel before it in the stream still runs (that kernel lets it, and it waits itself
 // before it reads what the other writes).
