@@ -224,7 +224,7 @@ PackedPlan packed_plan(int n_seqs, int total_q, int max_k, int Hkv, int G, int G
   w.split = max_k > kMinPartTiles * kBN;
   w.max_parts = w.split ? 2 * workers / w.nh : 0;
   w.split = w.max_parts > 0;
-  w.max_list = total_q / tok_tile + n_seqs + w.max_parts;
+  w.max_list = (int)(((int64_t)total_q + (int64_t)n_seqs * (tok_tile - 1)) / tok_tile) + w.max_parts;
   w.part_rows = (int64_t)w.max_parts * tok_tile * Gs * w.nh;
   size_t at = 16;
   w.at_seq = at;

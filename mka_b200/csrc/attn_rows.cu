@@ -38,7 +38,8 @@ enum RowsMode : int {
   kModeVarlen = 0,  // packed sequences, every tile found from the offsets
   kModeList = 1,    // packed sequences, items of a plan (attn_plan.cu)
   kModeShared = 2,  // shared prefix (the first prefix_blocks blocks) and own keys
-  kModeOnce = 3     // the same without parts: a cluster of kOnceCtas takes all keys of a request and joins them itself
+  kModeOnce = 3,    // the same without parts: a cluster of kOnceCtas takes all keys of a request and joins them itself
+  kModeOnceVarlen = 4  // tiles found from the offsets as in kModeVarlen, each taken by a cluster as in kModeOnce
 };
 constexpr int kOnceCtas = 8;
 
@@ -176,6 +177,12 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
     it.lim0 = c.y;
     part_ts = p.Gs;
     if (c.z >= 0) part = (int64_t)c.z + (int64_t)blockIdx.y * a.y * p.Gs;
+  } else if constexpr (MODE == kModeOnceVarlen) {
+    if (!find_tile(p, tpt, blockIdx.x / kOnceCtas, it)) return;  // all of a cluster or none
+    it.kv_off += hkv * p.kv_sh;
+    const int per = ((it.ke + kTileKeys - 1) / kTileKeys + kOnceCtas - 1) / kOnceCtas * kTileKeys;
+    it.kb = (blockIdx.x % kOnceCtas) * per;
+    it.ke = min(it.ke, it.kb + per);
   } else if constexpr (MODE == kModeOnce) {
     it.row0 = blockIdx.x / kOnceCtas;
     it.n_tok = 1;
@@ -219,7 +226,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
     part = ((int64_t)split * p.B + it.row0) * p.Hq + hkv * p.G + g0;
   }
   // tiles from this one on hold keys that some rows see and others do not
-  constexpr bool kCausal = MODE == kModeVarlen || MODE == kModeList;
+  constexpr bool kCausal = MODE == kModeVarlen || MODE == kModeList || MODE == kModeOnceVarlen;
+  constexpr bool kCluster = MODE == kModeOnce || MODE == kModeOnceVarlen;
   const int diag_tile = kCausal && it.n_tok > 1 ? max(0, it.lim0 + 1 - it.kb) / kTileKeys : 0x3FFFFFF;
   volatile int* bad_v = reinterpret_cast<volatile int*>(smem + kRingBytes);
   if (threadIdx.x == 0) *bad_v = 0;
@@ -417,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
       wt[w] = fast_exp2(sm[(w * 16 + row) * 2] - Ms);
       L += wt[w] * sm[(w * 16 + row) * 2 + 1];
     }
-    if (MODE != kModeOnce && !live_row) return;
+    if (!kCluster && !live_row) return;
     float acc[16];
 #pragma unroll
     for (int c = 0; c < 16; ++c) acc[c] = 0.f;
@@ -443,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
         }
       }
     }
-    if constexpr (MODE == kModeOnce) {
+    if constexpr (kCluster) {
       // This CTA's keys are done: sums (not yet divided), maximum and weight of each row to where the others read them;
       // then every CTA joins 16 channels of all rows.
       float* xo = so + 4 * 16 * kHeadDim + 128;  // [16][128], behind so and sm
@@ -550,14 +558,15 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
            p.lse == nullptr ? nullptr : p.lse + b * p.lse_st + h * p.lse_sh);
 }
 
-// One launch, clusters of kOnceCtas: request x kv head (x slice of its group).
-int launch_once(const PackedAttnParams& p, cudaStream_t stream) {
-  auto kern = attn_rows_kernel<1, kModeOnce>;
+// One launch, clusters of kOnceCtas: tile x kv head (x slice of its group).
+template <int MODE>
+int launch_once(const PackedAttnParams& p, int64_t tiles, cudaStream_t stream, const char* what) {
+  auto kern = attn_rows_kernel<1, MODE>;
   static std::atomic<uint64_t> devices{0};
-  int rc = check_cuda(allow_smem(kern, kSmemBytes, devices), "attn_decode_shared launch");
+  int rc = check_cuda(allow_smem(kern, kSmemBytes, devices), what);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.B * kOnceCtas), (unsigned)(p.Hkv * p.n_gs));
+  cfg.gridDim = dim3((unsigned)(tiles * kOnceCtas), (unsigned)(p.Hkv * p.n_gs));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
@@ -567,7 +576,7 @@ int launch_once(const PackedAttnParams& p, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), "attn_decode_shared launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), what);
 }
 
 template <int WM, int MODE>
@@ -592,30 +601,48 @@ bool mappable(int64_t st, int rows, int64_t sh, int heads) {
   return (rows == 1 || st > 0) && (heads == 1 || sh > 0);
 }
 
+// Tiles of `tokens` tokens of a packed batch, at most (every sequence may end in a tile that it does not fill).
+int64_t tile_bound(int n_seqs, int total_q, int tokens) {
+  return ((int64_t)total_q + (int64_t)n_seqs * (tokens - 1)) / tokens;
+}
+
 // How a packed batch runs:
 //   kShort: one launch, every CTA of 64 rows finds its tile in the offsets itself. A CTA takes about 19 ns a key, so it
 //     is for keys (times the waves of CTAs) that are done before a plan would be.
+//   kOnce: one launch, every tile of 16 rows is found in the same way and taken by a cluster that cuts its keys in
+//     eight: few tiles with more keys.
 //   kThin: tiles of 16 rows from a plan, long sequences split: batches of few rows per sequence, where the time goes to
 //     reading K and V.
 //   kPair: 256 rows per cluster on tcgen05, from a plan: the rest.
-// Measured in us (short / thin / pair), 32 heads over 8, on both sides of each limit:
+// Measured in us on the device (short / thin / pair), 32 heads over 8, on both sides of each limit:
 //   waves x keys: 40 prompts' keys 5.3 / 8.2 / 12.5;  200: 8.6 / 15.8 / 16.9;  250: 9.3 / 17.7 / 17.1;
 //     400: 18.6 / 26.7 / 15.8;  500 (32 single tokens): 19.8 / 14.4 / 27.9;
 //   rows per sequence (64 sequences of 100 to 16000 keys): 4: 657 / 379 / 451;  16: 670 / 392 / 470;
 //     32: 678 / 511 / 466;  32 as one kv head: 299 / 84 / 81;  prompts of 64 to 2048 tokens: 387 / 783 / 124.
 //   a prompt among single tokens (thin / pair): 512 tokens among 60: 338 / 271;  1024 among 400: 754 / 927;  2048 among
 //     800: 1142 / 1042.
-enum class VarlenPath { kShort, kThin, kPair };
+// and once / the better of thin and pair (which take a launch or two and a workspace more on the host, 5 us):
+//   1 wave: 1 token on 500 keys 5.1 / 11.2, on 4000 9.5 / 17.5, on 8000 14.7 / 19.0, on 16000 24.6 / 22.0; 100 on 1000,
+//     1 kv head, 9.0 / 21.6;
+//   2 waves: 8 tokens on 1000 each 14.4 / 17.8, on 2000 17.6 / 18.6, on 100 to 4000 22.3 / 19.3; 3 x 40 tokens of 8
+//     heads over 1 on 500 15.2 / 12.9;  4 waves: 16 tokens on 600 26.0 / 17.2.
+enum class VarlenPath { kShort, kOnce, kThin, kPair };
 constexpr int kShortKeys = 320;
+constexpr int kOnceVarlenKeys = 12000;
 
 VarlenPath varlen_path(int n_seqs, int total_q, int max_k, int Hkv, int G) {
   PackedAttnParams p = {};
   p.G = G;
-  slice_group(p, 64);
-  const int64_t ctas = ((int64_t)total_q / (64 / p.Gs) + n_seqs) * Hkv * p.n_gs;
   const int64_t slots = 2 * num_sms_current_device();
-  if ((ctas + slots - 1) / slots * max_k < kShortKeys) return VarlenPath::kShort;
-  return (int64_t)total_q * G <= (int64_t)n_seqs * 16 ? VarlenPath::kThin : VarlenPath::kPair;
+  auto waves = [&](int rows, int ctas) {  // of CTAs on all SMs, with `rows` rows and `ctas` CTAs a tile
+    slice_group(p, rows);
+    return (tile_bound(n_seqs, total_q, rows / p.Gs) * Hkv * p.n_gs * ctas + slots - 1) / slots;
+  };
+  if (waves(64, 1) * max_k < kShortKeys) return VarlenPath::kShort;
+  const bool thin = (int64_t)total_q * G <= (int64_t)n_seqs * 16;
+  const int64_t w = waves(16, kOnceCtas);
+  if (w <= (thin ? 2 : 1) && w * w * max_k <= kOnceVarlenKeys) return VarlenPath::kOnce;
+  return thin ? VarlenPath::kThin : VarlenPath::kPair;
 }
 
 PackedPlan thin_plan(int n_seqs, int total_q, int max_k, int Hkv, PackedAttnParams& p) {
@@ -680,7 +707,8 @@ size_t attn_varlen_workspace_bytes(int n_seqs, int total_q, int max_k, int Hq, i
   PackedAttnParams p = {};
   p.G = Hq / Hkv;
   switch (varlen_path(n_seqs, total_q, max_k, Hkv, p.G)) {
-    case VarlenPath::kShort: return 0;
+    case VarlenPath::kShort:
+    case VarlenPath::kOnce: return 0;
     case VarlenPath::kThin: return thin_plan(n_seqs, total_q, max_k, Hkv, p).total;
     default: return attn_pair_plan(n_seqs, total_q, max_k, Hq, Hkv).total;
   }
@@ -695,9 +723,11 @@ int launch_attn_varlen(PackedAttnParams p, int max_k, void* workspace, cudaStrea
       (path == VarlenPath::kPair &&
        (!mappable(p.q_st, p.total_q, p.q_sh, p.Hq) || !mappable(p.kv_st, p.total_k, p.kv_sh, p.Hkv)))) {
     slice_group(p, 64);
-    const int tpt = 64 / p.Gs;
-    const int64_t tiles = (int64_t)p.total_q / tpt + p.n_seqs;  // at least one tile ends in every sequence
-    return launch_rows<4, kModeVarlen>(p, tiles, false, stream, "attn_varlen launch");
+    return launch_rows<4, kModeVarlen>(p, tile_bound(p.n_seqs, p.total_q, 64 / p.Gs), false, stream, "attn_varlen launch");
+  }
+  if (path == VarlenPath::kOnce) {
+    slice_group(p, 16);
+    return launch_once<kModeOnceVarlen>(p, tile_bound(p.n_seqs, p.total_q, 16 / p.Gs), stream, "attn_varlen launch");
   }
   PackedPlan w = path == VarlenPath::kThin ? thin_plan(p.n_seqs, p.total_q, max_k, p.Hkv, p)
                                            : attn_pair_plan(p.n_seqs, p.total_q, max_k, p.Hq, p.Hkv);
@@ -727,7 +757,7 @@ int launch_attn_decode_shared(PackedAttnParams p, void* workspace, cudaStream_t 
   if (!mappable(p.q_st, p.B, p.q_sh, p.Hq) || !mappable(p.kp_st, p.P, p.kp_sh, p.Hkv)) s.pair = false;
   if (s.once) {
     slice_group(p, 16);
-    return launch_once(p, stream);
+    return launch_once<kModeOnce>(p, p.B, stream, "attn_decode_shared launch");
   }
   const int parts = s.prefix_splits + s.own_splits;
   p.part_o = static_cast<float*>(workspace);

@@ -89,7 +89,8 @@ def test_workspace_sizes_of_bad_shapes_are_zero(lib):
 def test_small_problems_need_no_workspace(lib):
     assert lib.fmka_attn_varlen_workspace_size(2, 8, 8, 4, 2) == 0
     assert lib.fmka_attn_decode_shared_workspace_size(2, 4, 2, 8, 8) == 0
-    assert lib.fmka_attn_varlen_workspace_size(2, 8, 5000, 4, 2) > 0
+    assert lib.fmka_attn_varlen_workspace_size(2, 8, 5000, 4, 2) == 0
+    assert lib.fmka_attn_varlen_workspace_size(2, 8, 50000, 4, 2) > 0
     assert lib.fmka_attn_decode_shared_workspace_size(2, 4, 2, 5000, 8) > 0
 
 

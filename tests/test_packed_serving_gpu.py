@@ -575,6 +575,40 @@ def test_varlen_few_tokens_do_not_see_later_keys(ops, poison, Hq, Hkv):
     assert not torch.isfinite(o[last].float()).all(-1).any()
 
 
+@pytest.mark.parametrize("q_lens,k_lens,Hq,Hkv", [
+    ([2, 4, 1, 3, 4], [700, 900, 64, 3, 1097], 4, 1), ([1], [8000], 32, 8), ([1], [12001], 8, 8),
+    ([0, 1, 0, 7], [5, 3000, 0, 9], 20, 1), ([33], [1500], 16, 1), ([1, 1], [513, 512], 40, 8), ([40, 3], [450, 1], 4, 4),
+    ([16], [4000], 32, 8), ([130], [900], 1, 1), ([1] * 8, [1000] * 7 + [1], 32, 8), ([6, 90], [400, 40], 5, 1),
+    ([1] * 3, [0, 0, 4000], 8, 2), ([17, 1], [16, 2000], 7, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_varlen_few_rows(ops, q_lens, k_lens, Hq, Hkv, causal):
+    """Few rows behind short to long histories, the longest given; a bad last key reaches its own row only."""
+    g = _gen(sum(k_lens) + Hq)
+    Tq = sum(q_lens)
+    q, k, v = _randn(g, Tq, Hq, 128), _randn(g, sum(k_lens), Hkv, 128), _randn(g, sum(k_lens), Hkv, 128)
+    cu_q, cu_k = _cu(q_lens), _cu(k_lens)
+    buf = torch.full((Tq + 2, Hq, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+    o, lse = ops.attn_varlen(q, k, v, cu_q, cu_k, max_k=max(k_lens), causal=causal, out=buf[1:-1])
+    _check_varlen(o, lse, q, k, v, q_lens, k_lens, causal)
+    assert (buf[0] == 7).all() and (buf[-1] == 7).all()
+    want, want_lse = o.clone(), lse.clone()
+    ends = [int(cu_k[i + 1]) - 1 for i, (a, b) in enumerate(zip(q_lens, k_lens)) if a and b]
+    last = [int(cu_q[i + 1]) - 1 for i, (a, b) in enumerate(zip(q_lens, k_lens)) if a and b]
+    rest = [i for i in range(Tq) if i not in last]
+    for poison in (float("nan"), -float("inf")):
+        k2, v2 = k.clone(), v.clone()
+        k2[ends] = v2[ends] = poison
+        o, lse = ops.attn_varlen(q, k2, v2, cu_q, cu_k, max_k=max(k_lens), causal=causal)
+        if causal:
+            assert torch.equal(o[rest], want[rest]) and torch.equal(lse[:, rest], want_lse[:, rest])
+        assert not torch.isfinite(o[last].float()).all(-1).any()
+    bad = cu_k.clone()
+    bad[-1] = sum(k_lens) + 1
+    out = torch.full_like(q, 7.0)
+    ops.attn_varlen(q, k, v, cu_q, bad, max_k=max(k_lens), causal=causal, out=out)
+    assert ops.device_status() == ops.STATUS_BAD_LAUNCH and (out == 7).all()
+
+
 @pytest.mark.parametrize("q_lens,k_lens", [([3, 40], [3, 40]), ([1, 1, 1], [9000, 30, 4000]), ([300, 700], [900, 800])])
 def test_varlen_expanded_views(ops, q_lens, k_lens):
     """One kv head under all, one query row for all heads or tokens: strides of zero."""
