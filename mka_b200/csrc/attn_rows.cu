@@ -617,6 +617,8 @@ int64_t tile_bound(int n_seqs, int total_q, int tokens) {
 // Measured in us on the device (short / thin / pair), 32 heads over 8, on both sides of each limit:
 //   waves x keys: 40 prompts' keys 5.3 / 8.2 / 12.5;  200: 8.6 / 15.8 / 16.9;  250: 9.3 / 17.7 / 17.1;
 //     400: 18.6 / 26.7 / 15.8;  500 (32 single tokens): 19.8 / 14.4 / 27.9;
+//     the offsets cost a key for eight sequences in every CTA, and a wave 5 us: short / better plan for 300 x 8 tokens, 2
+//     kv heads, 3 waves, 24 / 43;  256 x 1, 7 waves, 41 / 26;  1000 x 1, 1 kv head, 4 waves, 55 / 21;
 //   rows per sequence (64 sequences of 100 to 16000 keys): 4: 657 / 379 / 451;  16: 670 / 392 / 470;
 //     32: 678 / 511 / 466;  32 as one kv head: 299 / 84 / 81;  prompts of 64 to 2048 tokens: 387 / 783 / 124.
 //   a prompt among single tokens (thin / pair): 512 tokens among 60: 338 / 271;  1024 among 400: 754 / 927;  2048 among
@@ -638,7 +640,8 @@ VarlenPath varlen_path(int n_seqs, int total_q, int max_k, int Hkv, int G) {
     slice_group(p, rows);
     return (tile_bound(n_seqs, total_q, rows / p.Gs) * Hkv * p.n_gs * ctas + slots - 1) / slots;
   };
-  if (waves(64, 1) * max_k < kShortKeys) return VarlenPath::kShort;
+  const int64_t shorts = waves(64, 1);
+  if (shorts <= 5 && shorts * ((int64_t)max_k + n_seqs / 8) < kShortKeys) return VarlenPath::kShort;
   const bool thin = (int64_t)total_q * G <= (int64_t)n_seqs * 16;
   const int64_t w = waves(16, kOnceCtas);
   if (w <= (thin ? 2 : 1) && w * w * max_k <= kOnceVarlenKeys) return VarlenPath::kOnce;
