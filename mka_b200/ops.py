@@ -575,16 +575,18 @@ def qk_norm_rope(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: Optional[
     Hkv, kst = 0, (0,) * nd
     if k is not None:
         ks, kst = k.shape, k.stride()
-        if len(ks) != nd or ks[:-2] != qs[:-2] or ks[-1] != HEAD_DIM or kst[-1] != 1:
+        if len(ks) != nd or ks[0] != qs[0] or ks[nd - 3] != qs[nd - 3] or ks[-1] != HEAD_DIM or kst[-1] != 1:
             raise RuntimeError("qk_norm_rope: k must be q's shape with Hkv heads and contiguous channels")
         Hkv = ks[-2]
     w_f32 = 0
     for bit, w in ((1, q_weight), (2, k_weight)):
-        if w is not None and w.dtype is not _BF16:
+        if w is None:
+            continue
+        if w.dtype is not _BF16:
             w_f32 |= bit
             if w.dtype is not _F32:
                 raise RuntimeError("qk_norm_rope: the norm weights must be contiguous bf16 or fp32 [128] tensors")
-        if w is not None and (w.dim() != 1 or w.shape[0] != HEAD_DIM or w.stride(0) != 1):
+        if w.dim() != 1 or w.numel() != HEAD_DIM or not w.is_contiguous():
             raise RuntimeError("qk_norm_rope: the norm weights must be contiguous bf16 or fp32 [128] tensors")
     T, Hq = qs[-3], qs[-2]
     B = qs[0] if nd == 4 else 1
