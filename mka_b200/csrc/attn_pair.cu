@@ -18,7 +18,7 @@
 // registers, so S of the next tiles is made during the exponentials and nothing
 // waits for the chain S -> softmax -> P V -> next S of a tile. (With P written
 // over S, three S buffers and that chain, a tile took 1700 cycles; it takes 1412
-// now, the rate of the MMAs under the power limit, and an item 5000 to 6000 more
+// now, the rate of the MMAs under the power limit, and an item about 3000 more
 // for its start and end.) 4 causal sequences of 4096 to 12288 tokens, 28 heads
 // over 4: 1.48 ms, 1286 TFLOP/s; what bounds long items is the tensor pipe, what
 // bounds short ones their start (Q and the first K, TMEM hand-over of O).
@@ -30,10 +30,12 @@
 //   warp 2      TMEM allocation; issues O += P V (the even CTA's). Two issuers,
 //               because one warp's waits, commits and bookkeeping for both
 //               products took longer (2050 cycles a tile) than the MMAs (1024)
-//   warp 3      V gate: hands each V tile to the MMA; on tiles with masked keys
-//               it first puts zeros over the rows past the last key and over
-//               infinities and NaNs in rows that only some queries see, because
-//               a zero weight times such a value would not be zero
+//   warp 3      V gate: hands each V tile to the MMA. On tiles with keys that some
+//               rows do not see it first looks for infinities and NaNs, because a
+//               zero weight times such a value would not be zero. Only if there are
+//               any, zeros go over the rows past the last key and over those values
+//               (when every such tile was rewritten, the products waited for it:
+//               32 x 512 tokens took 166 us instead of 138)
 //   warps 4-7   output: O of a finished item from TMEM, divided by the joined sums,
 //               while the softmax warps are already in the next item (when the
 //               warpgroup with the last tile did this, an item cost 10000 cycles
@@ -475,11 +477,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int j = 0; j < n; ++j) {
         if (!(ok = warp_wait(&v_land[vr.s], vr.ph, p.status))) break;
         const int some = max(0, see - j * kBN);  // rows that every query sees
-        if (some < kBN) {
+        // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes 32 rows at a time
+        uint8_t* tile = sV + vr.s * kVBytes + (lane >> 3) * 128 + (lane & 7) * 16;
+        uint32_t odd = 0;
+#pragma unroll 1
+        for (int row0 = some & ~31; row0 < kBN; row0 += 32) {
+          uint4 x[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[k] = *reinterpret_cast<const uint4*>(tile + (row0 + k * 4) * 128);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) odd |= nonfinite_bits(x[k]);
+        }
+        if (__any_sync(0xffffffffu, odd != 0)) {
           const int live = klen - j * kBN;  // rows that hold keys
-          // 16-byte chunk (row, ch) sits at ch ^ (row & 7) of its 128-byte row; a warp takes 16 rows at a time
           bool bad = false;
-          uint8_t* tile = sV + vr.s * kVBytes + (lane >> 3) * 128 + (lane & 7) * 16;
 #pragma unroll 1
           for (int row0 = some & ~15; row0 < kBN; row0 += 16) {
             uint4 x[4];

@@ -519,6 +519,12 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 __device__ __forceinline__ float bf16lo_to_f32(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16hi_to_f32(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
 
+// Not zero if one of eight bf16 is an infinity or NaN: an exponent of all ones carries into the sign's place.
+__device__ __forceinline__ uint32_t nonfinite_bits(const uint4& x) {
+  constexpr uint32_t kExp = 0x7F807F80u, kOne = 0x00800080u;
+  return (((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne)) & 0x80008000u;
+}
+
 // Infinities and NaNs among the eight bf16 of a 16-byte chunk are replaced by zeros; true if there were any.
 __device__ __forceinline__ bool zero_nonfinite(uint4& c) {
   uint32_t* w = reinterpret_cast<uint32_t*>(&c);
