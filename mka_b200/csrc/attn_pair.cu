@@ -35,7 +35,7 @@
 //               zero weight times such a value would not be zero. Only if there are
 //               any, zeros go over the rows past the last key and over those values
 //               (when every such tile was rewritten, the products waited for it:
-//               32 x 512 tokens took 166 us instead of 138)
+//               32 x 512 tokens took 166 us instead of 140)
 //   warps 4-7   output: O of a finished item from TMEM, divided by the joined sums,
 //               while the softmax warps are already in the next item (when the
 //               warpgroup with the last tile did this, an item cost 10000 cycles
