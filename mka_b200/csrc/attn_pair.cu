@@ -116,7 +116,7 @@ struct PairParams {
   int Hq, G, Gs, n_gs, nh;   // nh = kv heads x group slices
   int tpt;                   // tokens per CTA
   FastDiv by_nh, by_ngs, by_nrt;
-  float scale_log2;
+  float scale_log2;          // not zero and no denormal: masked scores are -inf before they are multiplied by it
   const int* header;         // [0] list entries; null: uniform items
   const int4* list;          // {q0, nq, k0, kb}, {ke, lim0, part, 0}
   int B, P, n_rt, n_splits, keys_per_split;  // uniform items

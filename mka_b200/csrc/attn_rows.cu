@@ -18,6 +18,7 @@
 // half a step of 2^-9 on each weight, the same size as the rounding of the
 // output.
 #include <algorithm>
+#include <cfloat>
 
 #include "fmka_internal.h"
 #include "ptx.cuh"
@@ -601,6 +602,10 @@ bool mappable(int64_t st, int rows, int64_t sh, int heads) {
   return (rows == 1 || st > 0) && (heads == 1 || sh > 0);
 }
 
+// Whether the pair kernel may scale by this: it masks scores with -inf first and multiplies then, and a factor of zero
+// (or one that the kernels flush to zero) would make NaNs of them. This file's kernel masks behind the multiplication.
+bool pair_scale(float scale_log2) { return scale_log2 >= FLT_MIN; }
+
 // Tiles of `tokens` tokens of a packed batch, at most (every sequence may end in a tile that it does not fill).
 int64_t tile_bound(int n_seqs, int total_q, int tokens) {
   return ((int64_t)total_q + (int64_t)n_seqs * (tokens - 1)) / tokens;
@@ -676,8 +681,9 @@ constexpr int kOnceKeys = 2048;
 // with much room in parts as large as 8 waves of CTAs, or 8 parts, make them: parts that turn out empty are not free.
 // 16 requests, 8 kv heads, room for 131072 keys, 8 / 32 / 256 parts, in us: 100 keys each 22 / 41 / 213; all full 816 /
 // 815 / 1050; one full 224 / 128 / 323. 64 requests, room for 32768, 8 / 32 / 64 parts: 39 / 115 / 209; 800 / 878 / 991.
-// A stride of zero over several heads or tokens (an expanded view) is not for tensor maps; it stays here, and with
-// the parts that the sizes ask for, as the workspace's size is asked for without the strides.
+// A stride of zero over several heads or tokens (an expanded view) is not for tensor maps, and a scale of zero not for
+// the pair kernel; they stay here, and with the parts that the sizes ask for, as the workspace's size is asked for
+// without strides and scale.
 SharedPlan plan_shared(int B, int Hq, int Hkv, int P, int cap) {
   SharedPlan s{0, kTileKeys, 0, kTileKeys, false, false};
   PackedAttnParams r = {};
@@ -721,10 +727,10 @@ int launch_attn_varlen(PackedAttnParams p, int max_k, void* workspace, cudaStrea
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_varlen: device status word unavailable");
   const VarlenPath path = varlen_path(p.n_seqs, p.total_q, max_k, p.Hkv, p.G);
-  // expanded views are right on the first path whatever the size, and it needs no workspace
+  // expanded views and a scale of zero are right on the first path whatever the size, and it needs no workspace
   if (path == VarlenPath::kShort || p.total_k == 0 ||
-      (path == VarlenPath::kPair &&
-       (!mappable(p.q_st, p.total_q, p.q_sh, p.Hq) || !mappable(p.kv_st, p.total_k, p.kv_sh, p.Hkv)))) {
+      (path == VarlenPath::kPair && (!pair_scale(p.scale_log2) || !mappable(p.q_st, p.total_q, p.q_sh, p.Hq) ||
+                                     !mappable(p.kv_st, p.total_k, p.kv_sh, p.Hkv)))) {
     slice_group(p, 64);
     return launch_rows<4, kModeVarlen>(p, tile_bound(p.n_seqs, p.total_q, 64 / p.Gs), false, stream, "attn_varlen launch");
   }
@@ -757,7 +763,8 @@ int launch_attn_decode_shared(PackedAttnParams p, void* workspace, cudaStream_t 
   p.status = device_status_word();
   if (p.status == nullptr) return set_error(kErrDevice, "attn_decode_shared: device status word unavailable");
   SharedPlan s = plan_shared(p.B, p.Hq, p.Hkv, p.P, p.cap);
-  if (!mappable(p.q_st, p.B, p.q_sh, p.Hq) || !mappable(p.kp_st, p.P, p.kp_sh, p.Hkv)) s.pair = false;
+  if (!pair_scale(p.scale_log2) || !mappable(p.q_st, p.B, p.q_sh, p.Hq) || !mappable(p.kp_st, p.P, p.kp_sh, p.Hkv))
+    s.pair = false;
   if (s.once) {
     slice_group(p, 16);
     return launch_once<kModeOnce>(p, p.B, stream, "attn_decode_shared launch");

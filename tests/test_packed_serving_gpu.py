@@ -837,3 +837,36 @@ def test_a_packed_serving_step(ops, Hq, Hkv):
         od, ld = ops.attn_decode_shared(q1, k_prefix, v_prefix, kc, vc, lens)
         _check_shared(od, ld, q1, k_prefix, v_prefix, kc, vc, lens.tolist())
     assert ops.device_status() == 0
+
+
+# ------------------------------------------------------ scales next to zero --
+# Every path: found in the kernel, clusters, plan of few rows (cut along the keys), pairs of CTAs (direct and cut).
+SCALE_CASES = [
+    ([5, 8, 30], [5, 8, 30], 8, 2), ([1], [4000], 32, 8), ([1] * 40, [37 * i + 11 for i in range(40)], 32, 8),
+    ([1, 2], [9000, 30000], 8, 1), ([700, 300, 33], [700, 300, 33], 8, 2), ([260], [9001], 4, 4),
+    ([300, 40], [100, 900], 16, 4)]
+
+
+@pytest.mark.parametrize("q_lens,k_lens,Hq,Hkv", SCALE_CASES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("scale", [0.0, 1e-39, 1e-30])
+def test_varlen_scales_next_to_zero(ops, q_lens, k_lens, Hq, Hkv, causal, scale):
+    """Equal weights for all keys that a row sees: masked scores stay out whatever the scale multiplies them by."""
+    g = _gen(sum(k_lens))
+    q, k, v = _randn(g, sum(q_lens), Hq, 128), _randn(g, sum(k_lens), Hkv, 128), _randn(g, sum(k_lens), Hkv, 128)
+    o, lse = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(k_lens), max_k=max(k_lens), causal=causal, scale=scale)
+    _check_varlen_heads(o, lse, q, k, v, q_lens, k_lens, causal, scale)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,P,cap", [(2, 8, 2, 100, 70), (40, 8, 2, 700, 600), (60, 8, 2, 6001, 70),
+                                            (33, 40, 8, 5003, 0), (1, 4, 4, 70000, 5)])
+@pytest.mark.parametrize("scale", [0.0, 1e-39, 1e-30])
+def test_shared_scales_next_to_zero(ops, B, Hq, Hkv, P, cap, scale):
+    g = _gen(B + P)
+    q, kp, vp = _randn(g, B, Hq, 128), _randn(g, Hkv, P, 128), _randn(g, Hkv, P, 128)
+    k, v = _randn(g, B, Hkv, cap, 128), _randn(g, B, Hkv, cap, 128)
+    n = [i * cap // B for i in range(B)]
+    o, lse = ops.attn_decode_shared(q, kp, vp, k, v, torch.tensor(n, device=DEV, dtype=torch.int32), scale=scale)
+    _check_shared(o, lse, q, kp, vp, k, v, n, scale)
+    assert ops.device_status() == 0
