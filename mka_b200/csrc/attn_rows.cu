@@ -286,6 +286,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
     }
   }
 
+  if constexpr (kCausal) __syncthreads();  // bad_v is zero before any warp may set it (a first tile can be masked)
+
   float o[16][4];
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;

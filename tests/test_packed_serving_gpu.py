@@ -870,3 +870,40 @@ def test_shared_scales_next_to_zero(ops, B, Hq, Hkv, P, cap, scale):
     o, lse = ops.attn_decode_shared(q, kp, vp, k, v, torch.tensor(n, device=DEV, dtype=torch.int32), scale=scale)
     _check_shared(o, lse, q, kp, vp, k, v, n, scale)
     assert ops.device_status() == 0
+
+
+# ------------------------------------- bad values in V alone, K left finite --
+def _check_bad_v(ops, q, k, v, q_lens, k_lens, Hkv, spots, want, want_lse, **kw):
+    """spots: (sequence, key of it, kv head, channel, value) with different channels. The value shows, in this channel
+    of the rows and heads that see the key and nowhere else; everything else keeps its bits."""
+    G = q.shape[1] // Hkv
+    cu_q, cu_k = _cu(q_lens), _cu(k_lens)
+    q0, k0 = cu_q.tolist(), cu_k.tolist()
+    v2, expect = v.clone(), want.clone()
+    for s, key, hk, ch, x in spots:
+        v2[k0[s] + key, hk, ch] = x
+        first = max(0, key + q_lens[s] - k_lens[s])
+        expect[q0[s] + first:q0[s + 1], hk * G:(hk + 1) * G, ch] = x
+    o, lse = ops.attn_varlen(q, k, v2, cu_q, cu_k, **kw)
+    assert torch.equal(torch.nan_to_num(o, 7e4, 8e4, 9e4), torch.nan_to_num(expect, 7e4, 8e4, 9e4)), (
+        (o != expect) & ~(o.isnan() & expect.isnan())).nonzero()[:8].tolist()
+    assert torch.equal(lse, want_lse)
+
+
+BAD = (float("nan"), float("inf"), -float("inf"))
+
+
+def test_varlen_bad_values_in_the_first_tile(ops):
+    """Prompts so short that their first tile holds masked keys: what the rows that see a bad value get is decided before
+    the first product."""
+    g = _gen(90)
+    q_lens, Hq, Hkv = [5, 8, 30, 64, 17], 8, 2
+    T = sum(q_lens)
+    q, k, v = _randn(g, T, Hq, 128), _randn(g, T, Hkv, 128), _randn(g, T, Hkv, 128)
+    want, want_lse = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(q_lens), max_k=64)
+    _check_varlen(want, want_lse, q, k, v, q_lens, q_lens, True)
+    for i in range(60):
+        spots = [(s, (7 * i + 3 * s + hk) % n, hk, (31 * i + 5 * s) % 128, BAD[(i + s + hk) % 3])
+                 for s, n in enumerate(q_lens) for hk in range(Hkv)]
+        _check_bad_v(ops, q, k, v, q_lens, q_lens, Hkv, spots, want, want_lse, max_k=64)
+    assert ops.device_status() == 0
