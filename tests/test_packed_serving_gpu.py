@@ -907,3 +907,57 @@ def test_varlen_bad_values_in_the_first_tile(ops):
                  for s, n in enumerate(q_lens) for hk in range(Hkv)]
         _check_bad_v(ops, q, k, v, q_lens, q_lens, Hkv, spots, want, want_lse, max_k=64)
     assert ops.device_status() == 0
+
+
+# Rows in one launch, in clusters, from a plan with cut keys, and pairs of CTAs (whole rows, cut keys, rows without keys).
+BAD_V_CASES = [
+    ([70, 5, 40], [70, 5, 40], 8, 2), ([20, 3], [90, 200], 10, 2),
+    ([3], [4000], 32, 8), ([2, 4], [700, 900], 4, 1), ([9], [65], 20, 1),
+    ([2, 3, 4] * 20, [150 * i + 40 for i in range(60)], 4, 1), ([4, 1, 2], [20000, 30, 3333], 12, 4),
+    ([300, 700, 33], [300, 700, 33], 8, 2), ([129, 1, 64], [400, 500, 64], 32, 8), ([513], [513], 2, 2),
+    ([260], [9001], 4, 4), ([100, 30], [6000, 20000], 10, 2), ([300, 140], [100, 900], 16, 4),
+    ([60 + i % 70 for i in range(150)], [60 + i % 70 + (i % 3) * 50 for i in range(150)], 8, 8)]  # many per pair
+
+
+@pytest.mark.parametrize("q_lens,k_lens,Hq,Hkv", BAD_V_CASES)
+@pytest.mark.parametrize("seed", range(4))
+def test_varlen_bad_values_in_v_show_in_the_rows_that_see_them(ops, q_lens, k_lens, Hq, Hkv, seed):
+    import random
+
+    r = random.Random(seed)
+    g = _gen(91 + seed)
+    q, k, v = _randn(g, sum(q_lens), Hq, 128), _randn(g, sum(k_lens), Hkv, 128), _randn(g, sum(k_lens), Hkv, 128)
+    cu_q, cu_k, max_k = _cu(q_lens), _cu(k_lens), max(k_lens)
+    want, want_lse = ops.attn_varlen(q, k, v, cu_q, cu_k, max_k=max_k)
+    _check_varlen_heads(want, want_lse, q, k, v, q_lens, k_lens)
+    for x in BAD:
+        spots = []
+        for s, (lq, lk) in enumerate(zip(q_lens, k_lens)):
+            for hk in range(Hkv):
+                # the last key, one that only some rows see, one anywhere; in both halves of the channels
+                keys = {lk - 1, r.randrange(max(0, lk - lq), lk), r.randrange(lk)}
+                chans = r.sample(range(64), 3) if r.random() < 0.3 else r.sample(range(128), 3)
+                spots += [(s, key, hk, ch, x) for key, ch in zip(sorted(keys), chans)]
+        _check_bad_v(ops, q, k, v, q_lens, k_lens, Hkv, spots, want, want_lse, max_k=max_k)
+        # every channel of one key at once
+        s = r.randrange(len(q_lens))
+        key = r.randrange(max(0, k_lens[s] - q_lens[s]), k_lens[s])
+        _check_bad_v(ops, q, k, v, q_lens, k_lens, Hkv, [(s, key, hk, slice(None), x) for hk in range(Hkv)], want,
+                     want_lse, max_k=max_k)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("q_lens,k_lens,Hq,Hkv", [([70, 5], [70, 5], 8, 2), ([2, 4], [700, 900], 4, 1),
+                                                  ([300, 33], [700, 33], 8, 2), ([260], [9001], 4, 4)])
+def test_varlen_bad_values_of_both_signs_make_a_nan(ops, q_lens, k_lens, Hq, Hkv):
+    """+inf and -inf in one channel: the rows between them show the first, the rows that see both a NaN."""
+    g = _gen(92)
+    q, k, v = _randn(g, sum(q_lens), Hq, 128), _randn(g, sum(k_lens), Hkv, 128), _randn(g, sum(k_lens), Hkv, 128)
+    cu_q, cu_k = _cu(q_lens), _cu(k_lens)
+    want, want_lse = ops.attn_varlen(q, k, v, cu_q, cu_k)
+    v[k_lens[0] - 2, :, 77], v[k_lens[0] - 1, :, 77] = math.inf, -math.inf
+    o, lse = ops.attn_varlen(q, k, v, cu_q, cu_k)
+    n = q_lens[0]
+    assert (o[n - 2, :, 77] == math.inf).all() and torch.isnan(o[n - 1, :, 77].float()).all()
+    o[n - 2:n, :, 77] = want[n - 2:n, :, 77]
+    assert torch.equal(o, want) and torch.equal(lse, want_lse)
