@@ -6,7 +6,7 @@
  * fmka_get_last_error() returns the message of the calling thread's last error.
  * The caller owns every buffer; scratch memory ("workspace") is passed in by the
  * caller with its size, and each *_workspace_size() function reports how much a
- * call needs. No entry point but fmka_peer_alloc allocates device memory; kernels report bounded-
+ * call needs on the current device. No entry point but fmka_peer_alloc allocates device memory; kernels report bounded-
  * wait timeouts through a status word that lives in the library's own device
  * data. Calls on distinct streams with distinct buffers may run concurrently.
  *

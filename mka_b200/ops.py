@@ -521,6 +521,21 @@ def _on_device(dev: torch.device, name: str, *args) -> None:
         _lib.check(rc, name)
 
 
+def _workspace(q: torch.Tensor, name: str, *sizes: int) -> Tuple[Optional[torch.Tensor], int]:
+    """Scratch memory for one call, of the size that `name` gives on q's device (it depends on its SMs).
+
+    One allocation per call: a buffer kept between calls would be shared by
+    captured graphs that replay on different streams.
+    """
+    fn = getattr(_lib._lib or _lib.load(), name)
+    if q.get_device() == _current_device():
+        size = fn(*sizes)
+    else:
+        with torch.cuda.device(q.device):
+            size = fn(*sizes)
+    return (q.new_empty((size,), dtype=torch.uint8) if size else None), size
+
+
 def _strides(t: torch.Tensor) -> Tuple[int, ...]:
     """Element strides, 0 for dimensions of one element (whose stride says nothing)."""
     return tuple([0 if n == 1 else st for n, st in zip(t.shape, t.stride())])
@@ -695,10 +710,7 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     lse = q.new_empty((Hq, Tq), dtype=_F32) if want_lse else None
     if Tq == 0 or S == 0:
         return out, lse
-    # one allocation per call: a buffer kept between calls would be shared by
-    # captured graphs that replay on different streams
-    ws_bytes = _lib.load().fmka_attn_varlen_workspace_size(S, Tq, max_k, Hq, Hkv)
-    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    ws, ws_bytes = _workspace(q, "fmka_attn_varlen_workspace_size", S, Tq, max_k, Hq, Hkv)
     _on_device(dev, "fmka_attn_varlen", q.data_ptr(), qs[0], qs[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
                cu_q.data_ptr(), cu_k.data_ptr(), S, out.data_ptr(), os_[0], os_[1], _ptr(lse), 1, Tq, Tq, Tk, max_k,
                Hq, Hkv, Dh, int(causal), _DEFAULT_SCALE if scale is None else scale, _ptr(ws), ws_bytes)
@@ -751,8 +763,7 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     lse = q.new_empty((B, Hq), dtype=_F32) if want_lse else None
     if B == 0:
         return out, lse
-    ws_bytes = _lib.load().fmka_attn_decode_shared_workspace_size(B, Hq, Hkv, P, Tcap)
-    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None  # as in attn_varlen
+    ws, ws_bytes = _workspace(q, "fmka_attn_decode_shared_workspace_size", B, Hq, Hkv, P, Tcap)
     _on_device(dev, "fmka_attn_decode_shared", q.data_ptr(), qs[0], qs[1], k_prefix.data_ptr(), v_prefix.data_ptr(),
                ps[-3], ps[-2], k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], _ptr(lens), out.data_ptr(), os_[0],
                os_[2], _ptr(lse), Hq, B, Hq, Hkv, P, Tcap, Dh, _DEFAULT_SCALE if scale is None else scale, _ptr(ws),

@@ -108,3 +108,47 @@ def test_cpu_tensors_raise():
 def test_strides_of_single_elements_are_ignored():
     t = torch.empty_strided((1, 3, 128), (777, 128, 1))
     assert ops._strides(t) == (0, 128, 1)
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer of FakeTensor")
+@pytest.mark.parametrize("current", [0, 1])
+def test_workspace_size_is_asked_on_the_tensors_device(monkeypatch, current):
+    """The size depends on the SMs of the device that the call runs on, not on those of the current one."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    at, calls = [current], []
+
+    class Device:
+        def __init__(self, dev):
+            self.index = torch.device(dev).index
+
+        def __enter__(self):
+            self.before, at[0] = at[0], self.index
+
+        def __exit__(self, *exc):
+            at[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            def entry(*args):
+                calls.append((name, at[0], args))
+                return 4096 if name.endswith("workspace_size") else 0
+            return entry
+
+    lib = Lib()
+    monkeypatch.setattr(ops._lib, "_lib", lib)
+    monkeypatch.setattr(ops._lib, "load", lambda: lib)
+    monkeypatch.setattr(ops, "_current_device", lambda: at[0])
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    with FakeTensorMode():
+        x = torch.empty(4, 2, 128, dtype=torch.bfloat16, device="cuda:1")
+        cu = torch.empty(2, dtype=torch.int32, device="cuda:1")
+        ops.attn_varlen(x, x, x, cu, cu)
+        own = torch.empty(4, 2, 9, 128, dtype=torch.bfloat16, device="cuda:1")
+        ops.attn_decode_shared(x, own[0], own[0], own, own)
+    assert [(name, dev) for name, dev, _ in calls] == [
+        ("fmka_attn_varlen_workspace_size", 1), ("fmka_attn_varlen", 1),
+        ("fmka_attn_decode_shared_workspace_size", 1), ("fmka_attn_decode_shared", 1)]
+    assert all(args[-2] == 4096 for _, _, args in calls[1::2])
+    assert at == [current]
