@@ -340,10 +340,10 @@ FMKA_API int fmka_qk_norm_rope_bf16(const void* q, int64_t q_sb, int64_t q_st, i
  * queries and Lk keys sees keys j <= i + Lk - Lq (new tokens behind a history);
  * a row that sees no key gives zeros and a log-sum-exp of -inf. Rows outside
  * every sequence are left as they were. lse[row * lse_st + head * lse_sh]
- * (natural log) may be NULL. scale (here and below): finite and >= 0; 0, and
- * what is denormal times log2(e), weighs all visible keys alike. max_k: an upper
- * bound on the keys of one sequence (total_k if unknown); it sizes the workspace
- * and never limits what is read. */
+ * (natural log) may be NULL. scale (here and below): >= 0 and finite, times
+ * log2(e) as well; 0, and what is denormal then, weighs all visible keys alike.
+ * max_k: an upper bound on the keys of one sequence (total_k if unknown); it
+ * sizes the workspace and never limits what is read. */
 FMKA_API size_t fmka_attn_varlen_workspace_size(int n_seqs, int total_q, int max_k, int Hq, int Hkv);
 FMKA_API int fmka_attn_varlen(const void* q, int64_t q_st, int64_t q_sh, const void* k, const void* v, int64_t kv_st,
                               int64_t kv_sh, const int32_t* cu_q, const int32_t* cu_k, int n_seqs, void* o,

@@ -726,8 +726,8 @@ int check_packed_attn(PackedAttnParams& p, int rows, int keys, int head_dim, flo
   if (head_dim != 128) return set_error(kErrUnsupported, w + ": head_dim must be 128");
   if (p.Hq % p.Hkv != 0)
     return set_error(kErrInvalidArgument, w + ": query heads must be a multiple of kv heads");
-  if (!std::isfinite(scale) || scale < 0.f)
-    return set_error(kErrInvalidArgument, w + ": scale must be finite and >= 0");
+  if (!std::isfinite(p.scale_log2) || scale < 0.f)
+    return set_error(kErrInvalidArgument, w + ": scale must be >= 0 and finite, times log2(e) as well");
   if ((p.q_st | p.q_sh | p.kv_sb | p.kv_st | p.kv_sh | p.o_st | p.o_sh) & 7)
     return set_error(kErrInvalidArgument, w + ": strides must be multiples of 8 elements");
   if (!al16(p.q) || !al16(p.k) || !al16(p.v) || !al16(p.o))

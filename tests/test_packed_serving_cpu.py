@@ -152,3 +152,11 @@ def test_workspace_size_is_asked_on_the_tensors_device(monkeypatch, current):
         ("fmka_attn_decode_shared_workspace_size", 1), ("fmka_attn_decode_shared", 1)]
     assert all(args[-2] == 4096 for _, _, args in calls[1::2])
     assert at == [current]
+
+
+@pytest.mark.parametrize("entry,base", [("fmka_attn_varlen", VARLEN), ("fmka_attn_decode_shared", SHARED)])
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_c_abi_refuses_scales_that_overflow_in_base_two(lib, entry, base, scale):
+    """The kernels work with scale * log2(e), which has to be finite too: 0 * inf would be NaN."""
+    assert getattr(lib, entry)(*{**base, "scale": scale}.values()) == 1
+    assert "scale" in _lib.last_error()[1]
