@@ -444,13 +444,15 @@ __global__ void __launch_bounds__(kThreads, 2) attn_rows_kernel(const __grid_con
         acc[q4 * 4 + 3] = fmaf(wt[w], x.w, acc[q4 * 4 + 3]);
       }
     }
-    if (kCausal && n_tiles > diag_tile && *bad_v) {
+    if constexpr (kCausal) {
       // rare: the infinities and NaNs taken out above go to the rows that see them
-      for (int j = it.kb + diag_tile * kTileKeys; j <= lim_row; ++j) {
+      if (n_tiles > diag_tile && *bad_v) {
+        for (int j = it.kb + diag_tile * kTileKeys; j <= lim_row; ++j) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float x = __bfloat162float(vp[j * kv_st + seg * 16 + c]);
-          if (!(fabsf(x) <= 3.4e38f)) acc[c] += x;
+          for (int c = 0; c < 16; ++c) {
+            const float x = __bfloat162float(vp[j * kv_st + seg * 16 + c]);
+            if (!(fabsf(x) <= 3.4e38f)) acc[c] += x;
+          }
         }
       }
     }
