@@ -846,14 +846,14 @@ int launch_pair(const PairParams& given, const __nv_bfloat16* q, int64_t q_rows,
   if (rc) return rc;
   rc = rows_map(&tmV, v, kv_rows, kv_st, p.Hq / p.G, kv_sh, 1, 128, false);
   if (rc) return rc;
-  static int launch_regs = 0;
-  if (launch_regs == 0) {
+  static std::atomic<int> launch_regs{0};
+  if (launch_regs.load(std::memory_order_relaxed) == 0) {
     cudaFuncAttributes fa;
     rc = check_cuda(cudaFuncGetAttributes(&fa, attn_pair_kernel), what);
     if (rc) return rc;
-    launch_regs = fa.numRegs;
+    launch_regs.store(fa.numRegs, std::memory_order_relaxed);
   }
-  if (launch_regs < kMinLaunchRegs)
+  if (launch_regs.load(std::memory_order_relaxed) < kMinLaunchRegs)
     return set_error(kErrUnsupported, std::string(what) + ": compiled register count too small for the warpgroup split");
   static std::atomic<uint64_t> devices{0};
   rc = check_cuda(allow_smem(attn_pair_kernel, kSmemBytes, devices), what);
