@@ -21,12 +21,15 @@ update and the layer attends to what it returns; `return_present=False`
 gives the two-value return (attn_output, attn_weights) that the decoder
 layers of transformers >= 4.48 unpack, and with it RoPE follows that
 version's contract (position_embeddings from the model, no rotary_emb on the
-module). Additive masks are not supported
-(causal only): with the default sdpa attention implementation transformers
-passes no mask for unpadded prefill and cached decode.
+module). Norms of the wrapped module's query and key heads (q_norm, k_norm) are
+left out with a warning: like the reference (hf/attention.py:64-67), the wrapper
+takes the four projections. Additive masks are not supported (causal only): with
+the default sdpa attention implementation transformers passes no mask for
+unpadded prefill and cached decode.
 """
 from __future__ import annotations
 
+import warnings
 from typing import Optional, Tuple
 
 import torch
@@ -69,6 +72,11 @@ class HFFastMKAAttention(nn.Module):
         self.k_proj = original_attn.k_proj
         self.v_proj = original_attn.v_proj
         self.o_proj = original_attn.o_proj
+        norms = [n for n in ("q_norm", "k_norm")
+                 if not isinstance(getattr(original_attn, n, None), (type(None), nn.Identity))]
+        if norms:
+            warnings.warn(f"HFFastMKAAttention takes the wrapped module's projections and leaves out its "
+                          f"{' and '.join(norms)}", stacklevel=2)
         self.rotary_emb = getattr(original_attn, "rotary_emb", None)
         self.attention_dropout = float(getattr(original_attn, "attention_dropout", 0.0))
 

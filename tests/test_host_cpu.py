@@ -261,3 +261,25 @@ def test_peer_timeout_in_status_word_raises(monkeypatch):
     with pytest.raises(sharded.PeerExchangeError, match="peer barrier"):
         sharded.raise_on_peer_timeout()
     assert seen == [False, False, False]  # the word is left for the caller's own poll
+
+
+@pytest.mark.parametrize("norms", [(), ("q_norm",), ("q_norm", "k_norm")])
+def test_hf_wrapper_says_which_norms_it_leaves_out(norms):
+    """The layer takes the wrapped module's projections only; per-head norms that it has do not vanish silently."""
+    import warnings
+
+    from transformers import LlamaConfig
+    from transformers.models.llama.modeling_llama import LlamaAttention, LlamaRMSNorm
+
+    from mka_b200 import HFFastMKAAttention
+
+    attn = LlamaAttention(LlamaConfig(hidden_size=512, num_attention_heads=4, num_key_value_heads=1,
+                                      intermediate_size=64, vocab_size=16), layer_idx=0)
+    for name in ("q_norm", "k_norm"):
+        setattr(attn, name, LlamaRMSNorm(128) if name in norms else nn.Identity() if norms else None)
+    with warnings.catch_warnings(record=True) as seen:
+        warnings.simplefilter("always")
+        HFFastMKAAttention(attn)
+    text = [str(w.message) for w in seen if "norm" in str(w.message)]
+    assert len(text) == (1 if norms else 0)
+    assert all((n in text[0]) == (n in norms) for n in ("q_norm", "k_norm")) if norms else True
