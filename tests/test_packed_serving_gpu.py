@@ -961,3 +961,110 @@ def test_varlen_bad_values_of_both_signs_make_a_nan(ops, q_lens, k_lens, Hq, Hkv
     assert (o[n - 2, :, 77] == math.inf).all() and torch.isnan(o[n - 1, :, 77].float()).all()
     o[n - 2:n, :, 77] = want[n - 2:n, :, 77]
     assert torch.equal(o, want) and torch.equal(lse, want_lse)
+
+
+# ----------------------------------------------- calls between the others --
+@pytest.mark.parametrize("q_lens,k_lens,Hq,Hkv", [([70, 5], [70, 5], 8, 2), ([2, 4], [700, 900], 4, 1),
+                                                  ([300, 33], [700, 33], 8, 2), ([260], [9001], 4, 4)])
+def test_varlen_a_key_of_infinite_score(ops, q_lens, k_lens, Hq, Hkv):
+    """An infinity in K alone: rows whose score it makes -inf go on without that key, the others turn NaN."""
+    g = _gen(95)
+    q, k, v = _randn(g, sum(q_lens), Hq, 128), _randn(g, sum(k_lens), Hkv, 128), _randn(g, sum(k_lens), Hkv, 128)
+    q[:, :, 3] = q[:, :, 3].abs() + 1
+    q[::2, :, 3] *= -1
+    at = k_lens[0] - q_lens[0] // 2 - 1
+    first = at + q_lens[0] - k_lens[0]                 # the first row that sees the key
+    k[at, :, 3] = math.inf
+    o, lse = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(k_lens))
+    n = q_lens[0]
+    odd = [i for i in range(max(0, first), n) if i % 2]
+    assert torch.isnan(o[odd].float()).all() and torch.isnan(lse[:, odd]).all()
+    rows = [i for i in range(sum(q_lens)) if i not in odd]
+    # without the key: a score of -inf has no weight
+    k[at, :, 3] = 0
+    see = torch.arange(k_lens[0], device=DEV)[None] <= torch.arange(n, device=DEV)[:, None] + k_lens[0] - n
+    see[:, at] = False
+    for h in range(Hq):
+        ref = _ref_rows(q[:n, h], k[:k_lens[0], h * Hkv // Hq], v[:k_lens[0], h * Hkv // Hq], see, 128 ** -0.5)
+        here = [i for i in rows if i < n]
+        _check_attn(o[here, h], lse[h, here], *(t[here] for t in ref), what=h)
+    assert torch.isfinite(o[n:].float()).all()
+
+
+def test_shared_more_items_than_one_launch_takes(ops):
+    g = _gen(96)
+    B, Hq, P, cap = 20001, 128, 300, 3
+    q, kp, vp = _randn(g, B, Hq, 128), _randn(g, 1, P, 128), _randn(g, 1, P, 128)
+    k, v = _randn(g, B, 1, cap, 128), _randn(g, B, 1, cap, 128)
+    lens = torch.randint(0, cap + 1, (B,), device=DEV, generator=g, dtype=torch.int32)
+    o, lse = ops.attn_decode_shared(q, kp, vp, k, v, lens)
+    at = torch.tensor([0, 1, 9999, 18943, 18944, 18945, 20000], device=DEV)
+    _check_shared(o[at], lse[at], q[at], kp, vp, k[at], v[at], lens[at].tolist())
+    # every request, by products of all rows at once in fp32 (which may be off by as much as the kernel)
+    sc = (q.view(-1, 128).float() @ kp[0].float().t()).view(B, Hq, P) * 128 ** -0.5
+    own = torch.einsum("bhd,bcd->bhc", q.float(), k[:, 0].float()) * 128 ** -0.5
+    own.masked_fill_(torch.arange(cap, device=DEV)[None, None] >= lens[:, None, None], -math.inf)
+    ref = torch.logsumexp(torch.cat([sc, own], -1), -1)
+    assert ((lse - ref).abs() <= 2e-4 + 2.0 ** -20 * ref.abs()).all()
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("q_lens,k_lens", [([5, 9], [30, 9]), ([1], [3000]), ([1] * 40, [500] * 40), ([300, 200], [300, 900])])
+def test_varlen_overlapping_rows(ops, q_lens, k_lens):
+    """Views whose rows overlap in memory (a window that slides by eight channels): read as any other strides."""
+    g = _gen(97)
+    Tq, Tk = sum(q_lens), sum(k_lens)
+    q = _randn(g, 4, 8 * Tq + 128).as_strided((Tq, 4, 128), (8, 8 * Tq + 128, 1))
+    kv = _randn(g, 2, 2, 8 * Tk + 128)
+    k, v = (t.as_strided((Tk, 2, 128), (8, 8 * Tk + 128, 1), t.storage_offset()) for t in (kv[0], kv[1]))
+    o, lse = ops.attn_varlen(q, k, v, _cu(q_lens), _cu(k_lens), max_k=max(k_lens))
+    _check_varlen_heads(o, lse, q, k, v, q_lens, k_lens)
+
+
+def test_nothing_to_see_in_a_captured_graph(ops):
+    """A batch without prefix and slots behind a copy in the same graph: the join alone is launched."""
+    g = _gen(98)
+    B, Hq = 300, 8
+    src, q = _randn(g, B, Hq, 128), torch.zeros(B, Hq, 128, device=DEV, dtype=torch.bfloat16)
+    own = q.new_empty(B, 2, 0, 128)
+    none = q.new_empty(2, 0, 128)
+    out = torch.full((B, 1, Hq, 128), 7.0, device=DEV, dtype=torch.bfloat16)
+    ops.attn_decode_shared(q, none, none, own, own, out=out)
+    assert (out == 0).all()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        q.copy_(src)
+        _, lse = ops.attn_decode_shared(q, none, none, own, own, out=out)
+    out.fill_(7.0)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_two_threads_at_once(ops):
+    """Two host threads, each with its stream and inputs; the first calls of a path may meet."""
+    import threading
+
+    runs = [_calls(ops, _gen(200 + i))[0] for i in range(2)]
+    want = [[t.clone() for t in r()] for r in runs]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i] = runs[i]()
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for w, o in zip(want, got):
+        assert all(torch.equal(a, b) for a, b in zip(w, o))
+    assert ops.device_status() == 0
