@@ -91,7 +91,8 @@ struct PairItem {
 };
 static_assert(sizeof(PairItem) == 48, "three 16-byte words");
 
-// Division by a number known on the host: q = (umulhi(n, m) + n) >> s for 0 <= n < 2^31.
+// Division by a number known on the host, by Granlund and Montgomery's multiplication for invariant integers:
+// q = (umulhi(n, m) + n) >> s for 0 <= n < 2^31.
 struct FastDiv {
   uint32_t m, s;
   int d;

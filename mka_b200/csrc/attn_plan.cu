@@ -18,8 +18,9 @@ constexpr int kBN = 128;  // keys per unit of work
 // turn or as CTAs are scheduled, get about the same. A tile with more work than a
 // worker's fair share is cut along its keys into parts that are joined afterwards.
 // Offsets that fall or leave the tensors give an empty list and a status bit.
-// It takes 5 to 6 us for lists that fit shared memory, nearly all of it latency
-// (smaller code in loops and calls measured no faster).
+// It takes 4 to 6 us in a stream of calls for lists that fit shared memory (6.7 with
+// cold caches), nearly all of it latency (smaller code in loops and calls measured no
+// faster).
 // (List, header and parts are read past L1: the reading kernels start before their writers end.)
 constexpr int kPlanThreads = 512;
 constexpr int kBins = 512;

@@ -15,8 +15,8 @@
 //
 // Online softmax in fp32 (running max m and sum l per row, base 2); P is
 // rounded to bf16 for the second product because the tensor cores take bf16:
-// half a step of 2^-9 on each weight, the same size as the rounding of the
-// output.
+// up to 2^-8 of each weight (half a step of 8 bits), the same size as the
+// rounding of the output.
 #include <algorithm>
 #include <cfloat>
 
@@ -628,10 +628,12 @@ int64_t tile_bound(int n_seqs, int total_q, int tokens) {
 //     400: 18.6 / 26.7 / 15.8;  500 (32 single tokens): 19.8 / 14.4 / 27.9;
 //     the offsets cost a key for eight sequences in every CTA, and a wave 5 us: short / better plan for 300 x 8 tokens, 2
 //     kv heads, 3 waves, 24 / 43;  256 x 1, 7 waves, 41 / 26;  1000 x 1, 1 kv head, 4 waves, 55 / 21;
-//   rows per sequence (64 sequences of 100 to 16000 keys): 4: 657 / 379 / 451;  16: 670 / 392 / 470;
-//     32: 678 / 511 / 466;  32 as one kv head: 299 / 84 / 81;  prompts of 64 to 2048 tokens: 387 / 783 / 124.
-//   a prompt among single tokens (thin / pair): 512 tokens among 60: 338 / 271;  1024 among 400: 754 / 927;  2048 among
-//     800: 1142 / 1042.
+//   rows per sequence (64 sequences of 100 to 16000 keys in even steps, 515 k keys): 4: 648 / 362 / 438;
+//     16: 670 / 380 / 460;  32: 740 / 510 / 460;  32 as one kv head: 308 / 96 / 89;  prompts of 64 to 2048 tokens:
+//     340 / 775 / 104.
+//   a prompt among single tokens of 100 keys and more in even steps (thin / pair): 512 tokens among 60 of up to 4000:
+//     118 / 117, of up to 16000: 369 / 412;  1024 among 400 of up to 4000: 530 / 786;  2048 among 800 of up to 2000:
+//     654 / 888. (The rule goes by sizes that the host knows, and takes the pair for the first two.)
 // and once / the better of thin and pair (which take a launch or two and a workspace more on the host, 5 us):
 //   1 wave: 1 token on 500 keys 5.1 / 11.2, on 4000 9.5 / 17.5, on 8000 14.7 / 19.0, on 16000 24.6 / 22.0; 100 on 1000,
 //     1 kv head, 9.0 / 21.6;

@@ -17,9 +17,9 @@
 // time, and the heads of one token in turn, so that weights and angles are
 // multiplied once per token (y = r * (x * w cos + partner * w' sin)) and a row
 // costs three packed operations per pair of channels. 32768 tokens of 28 + 4
-// heads: 108 us, 5.04 TB/s of 6.56 measured for a copy (192 us with one group of
-// rows per warp; 115 with weights and angles apart; 114 with the next rows
-// prefetched, which costs registers and so warps; 137 at 80 registers).
+// heads: 104 us, 5.24 TB/s of 6.56 measured for a copy (192 us with one group of
+// rows per warp; when it took 108: 115 with weights and angles apart, 114 with the
+// next rows prefetched, which costs registers and so warps, 137 at 80 registers).
 #include "fmka_internal.h"
 #include "ptx.cuh"
 
@@ -30,7 +30,7 @@ namespace {
 constexpr int kHeadDim = 128;
 constexpr int kWarps = 4;
 constexpr int kRowsPerWarp = 4;
-constexpr int kGroupsAhead = 2;   // four-row groups loaded before the first is used (32768 tokens: 119 us, with one 142)
+constexpr int kGroupsAhead = 2;   // four-row groups loaded before the first is used (32768 tokens of 28 + 4 heads: 104 us, with one 121)
 // A token's heads share one warp once that still leaves this many warps per SM (20 are resident). 32 + 8 heads, in us with
 // 1 / 13 / 32 of them: 256 tokens 5.9 / 3.5 / 3.5;  512: 7.3 / 4.7 / 5.6;  1024: 8.3 / 7.0 / 7.0;  2048: 9.8 / 9.9 / 12.0.
 constexpr int kWarpsPerSm = 13;

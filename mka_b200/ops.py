@@ -673,6 +673,7 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     sequence of Lq queries and Lk keys sees keys j <= i + Lk - Lq, so prompts
     (Lq == Lk), chunks of prompts behind a history and single tokens mix freely
     in one call; a row that sees no key gives zeros and a log-sum-exp of -inf.
+    scale: 1 / sqrt(128) unless given; >= 0 and finite (times log2(e) as well), 0 weighs all keys alike.
     max_k: the longest sequence's keys if the caller knows it (a bound that
     sizes the scratch memory; it limits nothing). The offsets must be
     non-decreasing and within the tensors: if not, nothing is written and
@@ -728,7 +729,7 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     prefix is read once for the whole batch); k / v [B, Hkv, Tcap, 128], each request's own cache
     behind the prefix, of which the first lens[b] slots are valid (int32 [B] on
     the GPU, clamped to [0, Tcap]; None: all of them). Strided views are fine.
-    The result is attn_decode's over the concatenated keys. Either part may be
+    scale as in attn_varlen. The result is attn_decode's over the concatenated keys. Either part may be
     empty; a request without any key gives zeros and a log-sum-exp of -inf.
     Returns o [B, 1, Hq, 128] and lse [B, Hq].
     """
