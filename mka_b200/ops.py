@@ -521,21 +521,6 @@ def _on_device(dev: torch.device, name: str, *args) -> None:
         _lib.check(rc, name)
 
 
-def _workspace(q: torch.Tensor, name: str, *sizes: int) -> Tuple[Optional[torch.Tensor], int]:
-    """Scratch memory for one call, of the size that `name` gives on q's device (it depends on its SMs).
-
-    One allocation per call: a buffer kept between calls would be shared by
-    captured graphs that replay on different streams.
-    """
-    fn = getattr(_lib._lib or _lib.load(), name)
-    if q.get_device() == _current_device():
-        size = fn(*sizes)
-    else:
-        with torch.cuda.device(q.device):
-            size = fn(*sizes)
-    return (q.new_empty((size,), dtype=torch.uint8) if size else None), size
-
-
 def _strides(t: torch.Tensor) -> Tuple[int, ...]:
     """Element strides, 0 for dimensions of one element (whose stride says nothing)."""
     return tuple([0 if n == 1 else st for n, st in zip(t.shape, t.stride())])
@@ -673,9 +658,9 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     sequence of Lq queries and Lk keys sees keys j <= i + Lk - Lq, so prompts
     (Lq == Lk), chunks of prompts behind a history and single tokens mix freely
     in one call; a row that sees no key gives zeros and a log-sum-exp of -inf.
-    scale: 1 / sqrt(128) unless given; >= 0 and finite (times log2(e) as well), 0 weighs all keys alike.
-    max_k: the longest sequence's keys if the caller knows it (a bound that
-    sizes the scratch memory; it limits nothing). The offsets must be
+    scale: 1 / sqrt(128) unless given; >= 0 and finite (times log2(e) as well), 0
+    weighs all keys alike. max_k: the longest sequence's keys if the caller knows
+    it (a bound that sizes the scratch memory; it limits nothing). The offsets must be
     non-decreasing and within the tensors: if not, nothing is written and
     STATUS_BAD_LAUNCH is set in the device status word. Returns o [Tq, Hq, 128]
     (or `out`, any strides; rows outside every sequence are left as they were)
@@ -684,6 +669,9 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     dev = q.device
     if not q.is_cuda:
         raise RuntimeError("FastMKA B200 ops need CUDA tensors (there is no CPU fallback)")
+    if dev.index != _current_device():  # the scratch memory's size depends on the device too
+        with torch.cuda.device(dev):
+            return attn_varlen(q, k, v, cu_q, cu_k, max_k, causal, scale, out, want_lse)
     if q.dtype is not _BF16 or k.dtype is not _BF16 or v.dtype is not _BF16:
         _check_bf16(q, k, v)
     _same_device("attn_varlen", dev, k, v, cu_q, cu_k)
@@ -711,7 +699,10 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     lse = q.new_empty((Hq, Tq), dtype=_F32) if want_lse else None
     if Tq == 0 or S == 0:
         return out, lse
-    ws, ws_bytes = _workspace(q, "fmka_attn_varlen_workspace_size", S, Tq, max_k, Hq, Hkv)
+    # one allocation per call: a buffer kept between calls would be shared by
+    # captured graphs that replay on different streams
+    ws_bytes = _lib.load().fmka_attn_varlen_workspace_size(S, Tq, max_k, Hq, Hkv)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
     _on_device(dev, "fmka_attn_varlen", q.data_ptr(), qs[0], qs[1], k.data_ptr(), v.data_ptr(), ks[0], ks[1],
                cu_q.data_ptr(), cu_k.data_ptr(), S, out.data_ptr(), os_[0], os_[1], _ptr(lse), 1, Tq, Tq, Tk, max_k,
                Hq, Hkv, Dh, int(causal), _DEFAULT_SCALE if scale is None else scale, _ptr(ws), ws_bytes)
@@ -729,13 +720,16 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     prefix is read once for the whole batch); k / v [B, Hkv, Tcap, 128], each request's own cache
     behind the prefix, of which the first lens[b] slots are valid (int32 [B] on
     the GPU, clamped to [0, Tcap]; None: all of them). Strided views are fine.
-    scale as in attn_varlen. The result is attn_decode's over the concatenated keys. Either part may be
-    empty; a request without any key gives zeros and a log-sum-exp of -inf.
+    scale as in attn_varlen. The result is attn_decode's over the concatenated
+    keys. Either part may be empty; a request without any key gives zeros and a log-sum-exp of -inf.
     Returns o [B, 1, Hq, 128] and lse [B, Hq].
     """
     dev = q.device
     if not q.is_cuda:
         raise RuntimeError("FastMKA B200 ops need CUDA tensors (there is no CPU fallback)")
+    if dev.index != _current_device():  # as in attn_varlen
+        with torch.cuda.device(dev):
+            return attn_decode_shared(q, k_prefix, v_prefix, k, v, lens, scale, out, want_lse)
     if not (q.dtype is _BF16 and k_prefix.dtype is _BF16 and v_prefix.dtype is _BF16 and k.dtype is _BF16
             and v.dtype is _BF16):
         _check_bf16(q, k_prefix, v_prefix, k, v)
@@ -764,7 +758,8 @@ def attn_decode_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.
     lse = q.new_empty((B, Hq), dtype=_F32) if want_lse else None
     if B == 0:
         return out, lse
-    ws, ws_bytes = _workspace(q, "fmka_attn_decode_shared_workspace_size", B, Hq, Hkv, P, Tcap)
+    ws_bytes = _lib.load().fmka_attn_decode_shared_workspace_size(B, Hq, Hkv, P, Tcap)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None  # as in attn_varlen
     _on_device(dev, "fmka_attn_decode_shared", q.data_ptr(), qs[0], qs[1], k_prefix.data_ptr(), v_prefix.data_ptr(),
                ps[-3], ps[-2], k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], _ptr(lens), out.data_ptr(), os_[0],
                os_[2], _ptr(lse), Hq, B, Hq, Hkv, P, Tcap, Dh, _DEFAULT_SCALE if scale is None else scale, _ptr(ws),
